@@ -78,6 +78,22 @@ SIGNATURES = {
                      _i32, _vp, _i64, _vp, _vp],
     "gsq_nll_rows": [_vp, _i32, _i32, _i64, _vp, _vp, _vp],
     "gsq_scale_grad": [_vp, _vp, _i32, _i32, _i32, _i32, _vp, _vp],
+    "gsq_fp8_quant": [_vp, _i32, _i32, _i32, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64,
+                      _vp],
+    "gsq_fp8_quant_blocks": [_vp, _i32, _i32, _i32, _i64, _vp, _i64, _vp, _i64, _vp],
+    "gsq_fp8_dequant": [_vp, _i64, _vp, _i64, _i32, _i32, _vp, _i32, _i64, _vp],
+    "gsq_fp8_gemm": [_i32, _i32, _i32, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i32, _i64, _i64,
+                     _vp, _i32, _i64, _i32, _vp, _vp],
+    "gsq_fp8_linear": [_vp, _i32, _i32, _i32, _i64, _vp, _i64, _vp, _i64, _i32, _vp, _i32, _i64,
+                       _vp, _i64, _vp, _vp],
+    "gsq_rope": [_vp, _i64, _i64, _i32, _vp, _i64, _i64, _i32, _i64, _i32, _i32, _i32, _i32, _vp,
+                 _i32, _vp, _f32, _i32, _vp, _i64, _i64, _vp, _i64, _i64, _vp],
+    "gsq_residual_norm": [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _f32,
+                          _f32, _f32, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp],
+    "gsq_residual_norm_bwd_workspace": [_i32, _i32, _i32, _vp],
+    "gsq_residual_norm_bwd": [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _i32, _vp, _vp, _i64, _vp,
+                              _i64, _i32, _i32, _i32, _f32, _f32, _vp, _i64, _vp, _i64, _vp, _vp,
+                              _vp, _vp, _i64, _vp],
 }
 
 _lib = None

@@ -26,6 +26,7 @@ import torch
 from .. import _lib
 from ..gemm import Terms, gemm
 from ..gsq.e2e import LIN_ORDER, BlockConfig, BlockWeights, Qwen2Block
+from .fp8 import Fp8Linear
 from ..gsq.export import BKEY, NKEY, SafetensorsFile, mlx_bits, module_path, to_mlx_affine
 
 QGEMV_MAX_ROWS = 8
@@ -113,9 +114,9 @@ def C_view_ptr(t):
 
 
 class PackedModel:
-    """A Qwen2-architecture decoder whose block linears are PackedLinear (dense tensors are
-    accepted for linears the checkpoint left unquantized), with the tied bf16 embedding, the
-    bf16 norms and biases."""
+    """A Qwen2-architecture decoder whose block linears are PackedLinear or Fp8Linear (dense
+    tensors are accepted for linears the checkpoint left unquantized), with the tied bf16
+    embedding, the bf16 norms and biases."""
 
     def __init__(self, cfg: BlockConfig, embed, norm, layers: list):
         self.cfg, self.embed, self.norm, self.layers = cfg, embed, norm, layers
@@ -145,20 +146,22 @@ class PackedModel:
         """Dequantize layer L's linears into the scratch set; its block weights."""
         for name in LIN_ORDER:
             lin, dst = self.layers[L][name], self._scratch[name]
-            if isinstance(lin, PackedLinear):
+            if isinstance(lin, (PackedLinear, Fp8Linear)):
                 lin.dequant(dst)
             else:
                 dst.copy_(lin)
         return self._bw[L]
 
     def packed_bytes(self) -> int:
-        """Bytes of the packed words, scales and biases of every linear."""
+        """Bytes of the packed words (or e4m3 codes), scales and biases of every linear."""
         n = 0
         for W in self.layers:
             for name in LIN_ORDER:
                 lin = W[name]
                 if isinstance(lin, PackedLinear):
                     n += lin.words.numel() * 4 + 2 * lin.scales.numel() * lin.scales.element_size()
+                elif isinstance(lin, Fp8Linear):
+                    n += lin.N * lin.K + 4 * lin.scales.numel()
         return n
 
     @classmethod

@@ -1,0 +1,217 @@
+"""Linears in 8-bit floating point: e4m3 values with a float32 scale per block of 128.
+
+The packed eval's other weight format beside PackedLinear (common/evaluate.py): half the bytes
+of bf16, both operands of the product in 8 bits on the tensor cores, no calibration. With a the
+largest magnitude of a block and a' = max(a, 2^-100),
+
+  scale = a' / 448,  code = e4m3(x * (448 / a'))        (448: the largest e4m3 value)
+
+  Fp8Tensor      rows of activations: codes [R, C] and a scale per row and 128 columns
+  quantize_rows  x -> Fp8Tensor
+  Fp8Linear      a weight [N, K] with a scale per 128 x 128: y = x W^T with x quantized in rows,
+                 and its vector-Jacobian product
+
+Reference: none (src/gsq_rco/gsq/export.py:52-91 exports integer codes only).
+"""
+from __future__ import annotations
+
+import torch
+
+from .. import _lib
+from ..gemm import err_flag
+from .operands import DTYPES, matrix, on_device, output, pitch
+
+BLOCK = 128
+E4M3 = torch.float8_e4m3fn
+
+
+def _blocks(n):
+    return -(-n // BLOCK)
+
+
+def pad16(n):
+    return -(-n // 16) * 16
+
+
+class Fp8Tensor:
+    """Activations [R, C] in e4m3: codes float8_e4m3fn [R, C] (a view of rows padded to 16
+    bytes) and scales float32 [R, ceil(C / 128)] (a view: stored block-major, as the product
+    reads them)."""
+
+    def __init__(self, codes, scales):
+        R, C = codes.shape
+        if codes.dtype != E4M3 or scales.dtype != torch.float32:
+            raise ValueError("codes must be float8_e4m3fn and scales float32")
+        if tuple(scales.shape) != (R, _blocks(C)):
+            raise ValueError(f"scales must be [{R}, {_blocks(C)}], got {tuple(scales.shape)}")
+        on_device(codes, "codes")
+        on_device(scales, "scales")
+        if R and (codes.stride(1) != 1 or pitch(codes) % 16 or codes.data_ptr() % 16):
+            raise ValueError("codes rows must be contiguous with a pitch of a multiple of 16")
+        if R > 1 and scales.stride(0) != 1 or scales.shape[1] > 1 and scales.stride(1) < R:
+            raise ValueError("scales must be stored block-major ([blocks, rows] transposed)")
+        self.codes, self.scales = codes, scales
+        self.shape = (R, C)
+
+    @classmethod
+    def empty(cls, R, C, dev):
+        codes = torch.empty(R, pad16(C), device=dev, dtype=E4M3)
+        return cls(codes[:, :C], torch.empty(_blocks(C), R, device=dev, dtype=torch.float32).t())
+
+    def float(self):
+        """The float32 values that the codes stand for."""
+        s = self.scales.repeat_interleave(BLOCK, 1)[:, :self.shape[1]]
+        return self.codes.float() * s
+
+
+def quantize_rows(x) -> Fp8Tensor:
+    """x [R, C] (bf16, float16 or float32) in e4m3 with a scale per row and 128 columns."""
+    x = matrix(x, "x")
+    R, C = x.shape
+    q = Fp8Tensor.empty(R, C, x.device)
+    if R and C:
+        _lib.call("gsq_fp8_quant", x.data_ptr(), DTYPES[x.dtype], R, C, pitch(x),
+                  q.codes.data_ptr(), pad16(C), q.scales.data_ptr(), R, None, 0, None, 0,
+                  _lib.stream_ptr())
+    return q
+
+
+def _padded(codes):
+    """codes [R, C] with rows on 16 bytes (a copy where they are not)."""
+    R, C = codes.shape
+    if codes.stride(1) == 1 and codes.stride(0) % 16 == 0 and codes.stride(0) >= C \
+            and codes.data_ptr() % 16 == 0:
+        return codes
+    out = torch.zeros(R, pad16(C), device=codes.device, dtype=torch.uint8)
+    out[:, :C].copy_(codes.view(torch.uint8))
+    return out.view(E4M3)[:, :C]
+
+
+class Fp8Linear:
+    """One linear W [N, K] in e4m3: codes float8_e4m3fn [N, K], scales float32
+    [ceil(N / 128), ceil(K / 128)]. codes_t: the codes transposed [K, N], which the
+    vector-Jacobian product reads (made on its first use otherwise)."""
+
+    def __init__(self, codes, scales, codes_t=None):
+        if codes.dtype != E4M3 or codes.dim() != 2 or not codes.numel():
+            raise ValueError(f"codes must be a float8_e4m3fn matrix, got {codes.dtype} "
+                             f"{tuple(codes.shape)}")
+        self.N, self.K = int(codes.shape[0]), int(codes.shape[1])
+        if scales.dtype != torch.float32 or \
+                tuple(scales.shape) != (_blocks(self.N), _blocks(self.K)):
+            raise ValueError(f"scales must be float32 [{_blocks(self.N)}, {_blocks(self.K)}], "
+                             f"got {scales.dtype} {tuple(scales.shape)}")
+        on_device(codes, "codes")
+        on_device(scales, "scales")
+        self.codes, self.scales = _padded(codes), scales.contiguous()
+        self._t = None
+        if codes_t is not None:
+            if codes_t.dtype != E4M3 or tuple(codes_t.shape) != (self.K, self.N):
+                raise ValueError(f"codes_t must be float8_e4m3fn [{self.K}, {self.N}]")
+            on_device(codes_t, "codes_t")
+            self._t = _padded(codes_t)
+        self._err = err_flag(codes.device)
+
+    @classmethod
+    def from_weight(cls, W, transposed=False):
+        """Quantize a dense weight [N, K] (bf16, float16 or float32); transposed: also keep the
+        codes transposed, for vjp."""
+        W = matrix(W, "W")
+        N, K = W.shape
+        if not N or not K:
+            raise ValueError("W must not be empty")
+        codes = torch.empty(N, pad16(K), device=W.device, dtype=E4M3)
+        scales = torch.empty(_blocks(N), _blocks(K), device=W.device, dtype=torch.float32)
+        _lib.call("gsq_fp8_quant_blocks", W.data_ptr(), DTYPES[W.dtype], N, K, pitch(W),
+                  codes.data_ptr(), pad16(K), scales.data_ptr(), _blocks(K), _lib.stream_ptr())
+        lin = cls(codes[:, :K], scales)
+        if transposed:
+            lin.codes_t()
+        return lin
+
+    def codes_t(self):
+        """The codes transposed [K, N]."""
+        if self._t is None:
+            t = torch.zeros(self.K, pad16(self.N), device=self.codes.device, dtype=torch.uint8)
+            t[:, :self.N].copy_(self.codes.view(torch.uint8).t())
+            self._t = t.view(E4M3)[:, :self.N]
+        return self._t
+
+    def dequant(self, out):
+        """out [N, K] (bf16, float16 or float32; rows may be strided) = the dense weight."""
+        if out.dtype not in DTYPES:
+            raise ValueError(f"unsupported out dtype {out.dtype}")
+        output(out, self.N, self.K, out.dtype, out.device, "out")
+        _lib.call("gsq_fp8_dequant", self.codes.data_ptr(), self.codes.stride(0),
+                  self.scales.data_ptr(), self.scales.shape[1], self.N, self.K, out.data_ptr(),
+                  DTYPES[out.dtype], pitch(out), _lib.stream_ptr())
+        return out
+
+    def _gemm(self, M, N, K, a, sa, b, sb, sb_rows, sb_n, sb_k, out, accumulate=False):
+        _lib.call("gsq_fp8_gemm", M, N, K, a.data_ptr(), a.stride(0), sa.data_ptr(), M,
+                  b.data_ptr(), b.stride(0), sb.data_ptr(), sb_rows, sb_n, sb_k, out.data_ptr(),
+                  DTYPES[out.dtype], pitch(out), int(accumulate), self._err.data_ptr(),
+                  _lib.stream_ptr())
+
+    def __call__(self, x, out=None, y_f32=False):
+        """y = x W^T [M, N] in x's type (or float32): x [M, K] (bf16, float16 or float32),
+        quantized per row and 128 columns on the way; or x an Fp8Tensor (y in bf16)."""
+        on_device(self.codes, "the weight")
+        if isinstance(x, Fp8Tensor):
+            M = x.shape[0]
+            if x.shape[1] != self.K:
+                raise ValueError(f"x must be [M, {self.K}], got {x.shape}")
+            y = output(out, M, self.N, torch.float32 if y_f32 else torch.bfloat16,
+                     self.codes.device, "out")
+            if M:
+                self._gemm(M, self.N, self.K, x.codes, x.scales, self.codes, self.scales, 0,
+                           self.scales.shape[1], 1, y)
+            return y
+        x = matrix(x, "x", cols=self.K)
+        M = x.shape[0]
+        y = output(out, M, self.N, torch.float32 if y_f32 else x.dtype, x.device, "out")
+        if not M:
+            return y
+        # allocated per call on the calling stream: nothing is shared between calls
+        ws = torch.empty(M * (pad16(self.K) + 4 * _blocks(self.K)), device=x.device,
+                         dtype=torch.uint8)
+        _lib.call("gsq_fp8_linear", x.data_ptr(), DTYPES[x.dtype], M, self.K, pitch(x),
+                  self.codes.data_ptr(), self.codes.stride(0), self.scales.data_ptr(),
+                  self.scales.shape[1], self.N, y.data_ptr(), DTYPES[y.dtype], pitch(y),
+                  ws.data_ptr(), ws.numel(), self._err.data_ptr(), _lib.stream_ptr())
+        return y
+
+    def vjp(self, x, dy, dx=None, dw=None, accumulate=False):
+        """Vector-Jacobian product at x [M, K] for the cotangent dy [M, N]: (dx, dw).
+        dx = dy W [M, K] in x's type, dy quantized per row and 128 columns, W the weight's own
+        codes. dw = dy^T x float32 [N, K] (added to dw when accumulate), both quantized per
+        column and 128 rows; rounding counts as the identity (straight through)."""
+        x = matrix(x, "x", cols=self.K)
+        M, N, K = x.shape[0], self.N, self.K
+        dy = matrix(dy, "dy", rows=M, cols=N)
+        dev = x.device
+        on_device(self.codes, "the weight")
+        if accumulate and dw is None:
+            raise ValueError("accumulate needs dw")
+        dx = output(dx, M, K, x.dtype, dev, "dx")
+        dw = output(dw, N, K, torch.float32, dev, "dw")
+        if not M:
+            if not accumulate:
+                dw.zero_()
+            return dx, dw
+        wt, sw = self.codes_t(), self.scales
+        st = _lib.stream_ptr()
+        lm, ln, mb = pad16(M), pad16(N), _blocks(M)
+        q = torch.empty(M * ln + (N + K) * lm, device=dev, dtype=torch.uint8)
+        s = torch.empty(_blocks(N) * M + mb * (N + K), device=dev, dtype=torch.float32)
+        dyq, dyt, xt = q[:M * ln].view(M, ln), q[M * ln:M * ln + N * lm].view(N, lm), \
+            q[M * ln + N * lm:].view(K, lm)
+        s0, s1 = _blocks(N) * M, _blocks(N) * M + mb * N
+        _lib.call("gsq_fp8_quant", dy.data_ptr(), DTYPES[dy.dtype], M, N, pitch(dy),
+                  dyq.data_ptr(), ln, s.data_ptr(), M, dyt.data_ptr(), lm, s[s0:].data_ptr(), N,
+                  st)
+        _lib.call("gsq_fp8_quant", x.data_ptr(), DTYPES[x.dtype], M, K, pitch(x), None, 0, None, 0,
+                  xt.data_ptr(), lm, s[s1:].data_ptr(), K, st)
+        self._gemm(M, K, N, dyq, s, wt, sw, 0, 1, sw.shape[1], dx)
+        self._gemm(N, K, M, dyt, s[s0:], xt, s[s1:], 1, 0, K, dw, accumulate)
+        return dx, dw

@@ -504,6 +504,93 @@ int qgemm_packed(const void *X, int M, int K, int64_t ld_x, const uint32_t *word
 int gsq_nll_rows(const void *z, int n, int V, int64_t ld, const int32_t *targets, double *nll,
                  void *stream);
 
+/* ---- 8-bit floating point: e4m3 values with a float32 scale per block of 128 ----
+ * A block's scale and codes, with a = max(largest magnitude, 2^-100): scale = a / 448,
+ * code = e4m3(x (448 / a)), each operation float32, rounded once; NaN or infinity in a block
+ * make its values NaN. Codes are one byte, rows of ld elements (ld % 16 == 0, 16-byte aligned
+ * base; the bytes between the last column and ld may be written). Types: 0 = bf16, 1 = f16,
+ * 2 = f32. No counterpart in the reference, whose eval packs integers only. */
+
+/* Row form (codes): a scale per row and 128 columns: codes [rows][ld_codes], scales
+ * [ceil(cols / 128)][ld_scales]. Column form (codes_t): a scale per column and 128 rows:
+ * codes_t [cols][ld_codes_t], scales_t [ceil(rows / 128)][ld_scales_t]. Either or both, from
+ * one read of x [rows][ld_x]. */
+int gsq_fp8_quant(const void *x, int dtype, int rows, int cols, int64_t ld_x, void *codes,
+                  int64_t ld_codes, float *scales, int64_t ld_scales, void *codes_t,
+                  int64_t ld_codes_t, float *scales_t, int64_t ld_scales_t, void *stream);
+
+/* Weight form: one scale per 128 x 128: codes [N][ld_codes], scales [ceil(N / 128)][ld_scales]. */
+int gsq_fp8_quant_blocks(const void *w, int dtype, int N, int K, int64_t ld_w, void *codes,
+                         int64_t ld_codes, float *scales, int64_t ld_scales, void *stream);
+
+/* out [N][ld_out] = scale * code of a weight form, rounded once to dtype. */
+int gsq_fp8_dequant(const void *codes, int64_t ld_codes, const float *scales, int64_t ld_scales,
+                    int N, int K, void *out, int dtype, int64_t ld_out, void *stream);
+
+/* out[m][n] = sum over 128-wide k-blocks b of sa[b][m] sb(b, n) sum_k a[m][k] b[n][k]
+ * (+ out[m][n] if accumulate, float32 out only): the block sums on the tensor cores in float32,
+ * the sum over blocks in float32 registers, one rounding to dtype. a [M][lda], b [N][ldb] codes;
+ * sa [ceil(K / 128)][ld_sa] (row form); sb: sb_rows == 0 one scale per 128 x 128 at
+ * sb[(n / 128) sb_n + b sb_k], else per row of b at sb[b sb_k + n]. err: device word, nonzero
+ * after a bounded wait gave up. */
+int gsq_fp8_gemm(int M, int N, int K, const void *a, int64_t lda, const float *sa, int64_t ld_sa,
+                 const void *b, int64_t ldb, const float *sb, int sb_rows, int64_t sb_n,
+                 int64_t sb_k, void *out, int dtype, int64_t ld_out, int accumulate, int *err,
+                 void *stream);
+
+/* y [M][ld_y] = x W^T with x [M][ld_x] quantized in row form on the way and W in weight form.
+ * workspace: 16-byte aligned, >= M ceil16(K) + 4 M ceil(K / 128) bytes. */
+int gsq_fp8_linear(const void *x, int dtype, int M, int K, int64_t ld_x, const void *codes,
+                   int64_t ld_codes, const float *scales, int64_t ld_scales, int N, void *y,
+                   int y_dtype, int64_t ld_y, void *workspace, int64_t workspace_bytes, int *err,
+                   void *stream);
+
+/* ---- rotary positions ----
+ * q [T][nq][head_dim] and k [T][nk][head_dim] (nk 0: none) through element strides of tokens
+ * and heads (the head's elements contiguous) to q_out, k_out (strides of their own; the inputs
+ * themselves for a rotation in place). The first rotary_dim elements of a head turn in pairs
+ * (j, j + rotary_dim / 2), or (2 j, 2 j + 1) if interleaved, by positions[t] turns[j] turns:
+ * (a, b) -> factor (a cos - b sin, a sin + b cos); inverse: by the opposite angle (the
+ * vector-Jacobian product). The rest of the head is copied. dtype 0 / 1 / 2 = bf16 / f16 / f32;
+ * positions int32 or int64 [T] of any sign; turns float64 [rotary_dim / 2], the pairs'
+ * frequencies over 2 pi. float32 arithmetic, the angle reduced in 64 bits.
+ * The general form of gsq_rope_split's rotation (src/gsq_rco/gsq/e2e.py:96-108). */
+int gsq_rope(const void *q, int64_t q_t, int64_t q_h, int nq, const void *k, int64_t k_t,
+             int64_t k_h, int nk, int64_t T, int head_dim, int rotary_dim, int interleaved,
+             int dtype, const void *positions, int positions64, const double *turns, float factor,
+             int inverse, void *q_out, int64_t qo_t, int64_t qo_h, void *k_out, int64_t ko_t,
+             int64_t ko_h, void *stream);
+
+/* ---- RMS norms around a block, with its gate, residual scale and sum ----
+ *   n = y r1 (w_post + offset) (n = y without w_post), h_out = h + alpha gate n,
+ *   x = h' r2 (w_pre + offset) with h' the unrounded h_out (no x without w_pre),
+ *   r1 = 1 / sqrt(mean y^2 + eps), r2 likewise of h'; stats float32 [2][T] = r1, r2 (1 where
+ * there is no such norm). Rows of H <= 32768 of one dtype (0 / 1 / 2 = bf16 / f16 / f32), the
+ * weights [H] and gate [gate_rows][H] too; gate row i belongs to the rows
+ * [i T / gate_rows, (i + 1) T / gate_rows). x either as rows, or as e4m3 codes [T][ld_codes]
+ * and scales [ceil(H / 128)][ld_scales] (the row form of gsq_fp8_quant). h_out may be NULL.
+ * The fused, general form of gsq_rmsnorm and the residual sums (src/gsq_rco/gsq/e2e.py:90-93,
+ * 160-174). */
+int gsq_residual_norm(const void *h, int64_t ld_h, const void *y, int64_t ld_y,
+                      const void *w_post, const void *w_pre, const void *gate, int gate_rows,
+                      int T, int H, int dtype, float alpha, float eps, float offset, void *h_out,
+                      int64_t ld_ho, void *x, int64_t ld_x, void *codes, int64_t ld_codes,
+                      float *scales, int64_t ld_scales, float *stats, void *stream);
+
+/* Bytes of workspace of gsq_residual_norm_bwd (gate_rows 0: no gate), on the current device. */
+int gsq_residual_norm_bwd_workspace(int T, int H, int gate_rows, int64_t *bytes);
+
+/* Its vector-Jacobian product: dh, dy [T][H] in dtype and the float32 gradients dw_post [H],
+ * dw_pre [H], dgate [gate_rows][H] of the parameters present, for the cotangents dh2 of h_out
+ * (NULL: zero) and dx of x (with w_pre only), from the inputs and stats of the forward pass. */
+int gsq_residual_norm_bwd(const void *h, int64_t ld_h, const void *y, int64_t ld_y,
+                          const void *w_post, const void *w_pre, const void *gate, int gate_rows,
+                          const float *stats, const void *dh2, int64_t ld_dh2, const void *dx,
+                          int64_t ld_dx, int T, int H, int dtype, float alpha, float offset,
+                          void *dh, int64_t ld_dh, void *dy, int64_t ld_dy, float *dw_post,
+                          float *dw_pre, float *dgate, float *workspace, int64_t workspace_bytes,
+                          void *stream);
+
 #ifdef __cplusplus
 }
 #endif

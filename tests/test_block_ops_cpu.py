@@ -1,0 +1,235 @@
+"""The oracles of the 8-bit linear, the rotary positions and the residual norms (known values,
+gradients against differences), and the refusals of the operators: host checks and the C ABI's
+checks, which need no GPU."""
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+from gsq_rco_mlx_b200 import _lib
+from gsq_rco_mlx_b200.common import fp8, norm, rotary
+from oracle import blockops as ob
+from oracle import fp8 as of
+
+P = C.c_void_p(4096)   # 16-byte aligned, never dereferenced: every call below is refused first
+
+
+def test_e4m3_rounding():
+    """All 256 codes are fixed points, torch's own cast agrees, ties go to even."""
+    codes = torch.arange(256, dtype=torch.int32).to(torch.uint8).view(torch.float8_e4m3fn)
+    vals = codes.float().numpy().astype(np.float64)
+    ok = np.isfinite(vals)
+    assert ok.sum() == 254
+    assert np.array_equal(of.e4m3(vals[ok]), vals[ok])
+    x = np.concatenate([np.linspace(-460, 460, 100001), np.ldexp(1.0, np.arange(-14, 9)),
+                        np.arange(-64, 65) * 2.0 ** -10]).astype(np.float32)
+    t = torch.from_numpy(x).clamp(-448, 448).to(torch.float8_e4m3fn).float().numpy()
+    assert np.array_equal(of.e4m3(x.astype(np.float64)), t)
+    assert of.e4m3(np.array([17.0]))[0] == 16.0 and of.e4m3(np.array([19.0]))[0] == 20.0
+    assert np.isnan(of.e4m3(np.array([np.nan])))[0]
+
+
+def test_quantized_blocks_hold_their_bounds():
+    """Half a step of e4m3 (2^-4 of the value) or of its least step (2^-10, times the scale)."""
+    rng = np.random.default_rng(0)
+    x = (rng.standard_normal((7, 300)) * np.exp(3 * rng.standard_normal((7, 300)))).astype(
+        np.float32)
+    x[2, :128] = 0
+    q, s = of.quantize_rows(x)
+    v = of.rows_value(q, s)
+    sc = np.repeat(s, 128, 1)[:, :300]
+    # (the product by the reciprocal, and the scale, round by 2^-24 each: 2^-22 covers them)
+    assert np.all(np.abs(v - x) <= np.maximum(2.0 ** -4 * np.abs(x), 2.0 ** -10 * sc)
+                  * (1 + 2.0 ** -18) + 2.0 ** -22 * np.abs(x))
+    assert np.all(np.max(np.abs(q).reshape(7, -1)[:, :128], 1)[[0, 1, 3, 4, 5, 6]] == 448)
+    assert np.all(v[2, :128] == 0)
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_rotation_is_its_own_transpose_inverse(layout):
+    rng = np.random.default_rng(1)
+    q, u = rng.standard_normal((2, 5, 3, 10))
+    pos = np.array([0, 1, -7, 100000, 3])
+    w, f = rotary.frequencies(8, 1e4, {"type": "yarn", "factor": 4.0, "original": 64})
+    r = ob.rotate(q, pos, w, 8, layout, f)
+    # <R q, u> = <q, R^T u>
+    np.testing.assert_allclose((r * u).sum(),
+                               (q * ob.rotate(u, pos, w, 8, layout, f, inverse=True)).sum(),
+                               rtol=1e-12)
+    assert np.array_equal(r[..., 8:], q[..., 8:])
+    np.testing.assert_allclose(np.linalg.norm(r[..., :8]), f * np.linalg.norm(q[..., :8]))
+
+
+def test_frequencies():
+    w, f = rotary.frequencies(64, 1e6)
+    np.testing.assert_allclose(w, 1e6 ** (-np.arange(32) / 32), rtol=1e-15)
+    assert f == 1.0
+    assert np.array_equal(rotary.frequencies(64, 1e6, {"type": "linear", "factor": 4.0})[0], w / 4)
+    n = rotary.frequencies(64, 1e6, {"type": "ntk", "factor": 4.0})[0]
+    assert n[0] == 1.0 and n[-1] == pytest.approx(w[-1] / 4, rel=1e-12)
+    y, fy = rotary.frequencies(64, 1e4, {"type": "yarn", "factor": 8.0, "original": 4096})
+    w4 = rotary.frequencies(64, 1e4)[0]
+    turns = 4096 * w4 / (2 * np.pi)
+    assert np.all(y[turns > 40] == w4[turns > 40]) and np.allclose(y[turns < 0.7],
+                                                                   w4[turns < 0.7] / 8)
+    assert np.all(np.diff(y) < 0) and fy == pytest.approx(0.1 * np.log(8.0) + 1)
+    b = rotary.frequencies(64, 1e4, {"type": "bands", "factor": 8.0, "original": 4096})[0]
+    assert np.all(b[turns >= 4] == w4[turns >= 4]) and np.allclose(b[turns <= 1],
+                                                                   w4[turns <= 1] / 8)
+    for bad in ({"type": "other", "factor": 2.0}, {"type": "linear"},
+                {"type": "linear", "factor": 0.5}, {"type": "linear", "factor": float("inf")},
+                {"type": "yarn", "factor": 2.0}, {"type": "linear", "factor": 2.0, "low": 1},
+                {"type": "bands", "factor": 2.0, "original": 64, "low": 4.0, "high": 1.0},
+                {"type": "yarn", "factor": 2.0, "original": 64, "slow": 0.0}):
+        with pytest.raises(ValueError):
+            rotary.frequencies(64, 1e4, bad)
+
+
+@pytest.mark.parametrize("post,pre,gates", [(True, True, 0), (True, True, 1), (True, True, 3),
+                                            (False, True, 6), (True, False, 2)])
+def test_norm_gradients_against_differences(post, pre, gates):
+    """The oracle's gradients against central differences of its forward pass: step 1e-5, so the
+    truncation is 1e-10 of third derivatives of order 1 and the rounding 1e-16 / 1e-5."""
+    rng = np.random.default_rng(2)
+    T, H = 6, 9
+    v = {"h": rng.standard_normal((T, H)), "y": rng.standard_normal((T, H))}
+    if post:
+        v["w_post"] = rng.standard_normal(H)
+    if pre:
+        v["w_pre"] = rng.standard_normal(H)
+    if gates:
+        v["gate"] = rng.standard_normal((gates, H))
+    dh = rng.standard_normal((T, H))
+    dx = rng.standard_normal((T, H)) if pre else None
+
+    def value(v):
+        h2, x, *_ = ob.residual_norm(v["h"], v["y"], v.get("w_post"), v.get("w_pre"),
+                                     v.get("gate"), 0.7, 1e-3, 1.0)
+        return (h2 * dh).sum() + (0.0 if x is None else (x * dx).sum())
+
+    g, _ = ob.residual_norm_vjp(v["h"], v["y"], v.get("w_post"), v.get("w_pre"), dh, dx,
+                                v.get("gate"), 0.7, 1e-3, 1.0)
+    for name in v:
+        grad = g["d" + name]
+        assert grad.shape == v[name].shape
+        for i in np.ndindex(v[name].shape):
+            up, dn = dict(v), dict(v)
+            up[name], dn[name] = v[name].copy(), v[name].copy()
+            up[name][i] += 1e-5
+            dn[name][i] -= 1e-5
+            assert grad[i] == pytest.approx((value(up) - value(dn)) / 2e-5, rel=1e-6, abs=1e-7)
+
+
+def test_fp8_gradients_against_differences():
+    """dx of y = q(x) W^T with the rounding counted as the identity is the gradient through W's
+    values, dw that through the (column-quantized) x: both against differences of the bilinear
+    form, which is exact up to rounding for any step."""
+    rng = np.random.default_rng(3)
+    x, dy = (rng.standard_normal(s).astype(np.float32) for s in ((150, 200), (150, 140)))
+    qw, sw = of.quantize_blocks(rng.standard_normal((140, 200)).astype(np.float32))
+    dx, _, dw, _ = of.vjp(x, dy, qw, sw)
+    dv, wv = of.rows_value(*of.quantize_rows(dy)), of.blocks_value(qw, sw)
+    dt, xt = of.rows_value(*of.quantize_rows(dy.T)).T, of.rows_value(*of.quantize_rows(x.T)).T
+    for (i, k) in ((0, 0), (149, 199), (70, 130)):
+        f = lambda e: ((x[i] + e * (np.arange(200) == k)) @ wv.T * dv[i]).sum()  # noqa: E731
+        assert dx[i, k] == pytest.approx(f(1.0) - f(0.0), rel=1e-6, abs=1e-9)
+    for (n, k) in ((0, 0), (139, 199), (128, 127)):
+        f = lambda e: (xt @ (wv[n] + e * (np.arange(200) == k)) * dt[:, n]).sum()  # noqa: E731
+        assert dw[n, k] == pytest.approx(f(1.0) - f(0.0), rel=1e-6, abs=1e-9)
+
+
+def test_operators_refuse_host_tensors():
+    x = torch.zeros(4, 64)
+    with pytest.raises(ValueError):
+        fp8.quantize_rows(x)
+    with pytest.raises(ValueError):
+        fp8.Fp8Linear.from_weight(x)
+    with pytest.raises(ValueError):
+        fp8.Fp8Linear(torch.zeros(4, 64, dtype=torch.float8_e4m3fn), torch.zeros(1, 1))
+    with pytest.raises(ValueError):
+        fp8.Fp8Linear(x, torch.zeros(1, 1))
+    with pytest.raises(ValueError):
+        norm.residual_norm(x, x, w_pre=torch.zeros(64))
+    for kw in ({"rotary_dim": 3}, {"rotary_dim": 66}, {"rotary_dim": 0}, {"layout": "pairs"},
+               {"theta": 1.0}, {"scaling": {"type": "linear", "factor": -1}}):
+        with pytest.raises(ValueError):
+            rotary.Rotary(64, device="cpu", **kw)
+    r = rotary.Rotary(64, device="cpu")
+    for q, k, pos in ((torch.zeros(4, 2, 64), None, torch.zeros(4, dtype=torch.int32)),
+                      (torch.zeros(4, 64), None, torch.zeros(4, dtype=torch.int32)),
+                      (torch.zeros(4, 2, 64, dtype=torch.float64), None,
+                       torch.zeros(4, dtype=torch.int32))):
+        with pytest.raises(ValueError):
+            r(q, k, pos)
+
+
+def _refused(fn, ok, bad, status=_lib.GSQ_EINVAL):
+    for i, v in bad:
+        args = list(ok)
+        args[i] = v
+        assert fn(*args) == status, (i, v)
+
+
+def test_fp8_entry_points_refuse_bad_arguments():
+    lib = _lib.load()
+    odd = C.c_void_p(4097)
+    _refused(lib.gsq_fp8_quant,
+             [P, 0, 5, 200, 200, P, 208, P, 5, P, 16, P, 200, None],
+             [(0, None), (1, 3), (1, -1), (2, 0), (3, 0), (4, 199), (6, 200), (6, 192), (7, None),
+              (8, 4), (5, odd), (9, odd), (10, 5), (11, None), (12, 199), (0, odd)])
+    assert lib.gsq_fp8_quant(P, 0, 5, 200, 200, None, 0, None, 0, None, 0, None, 0,
+                             None) == _lib.GSQ_EINVAL
+    _refused(lib.gsq_fp8_quant_blocks, [P, 0, 5, 200, 200, P, 208, P, 2, None],
+             [(0, None), (1, 5), (2, 0), (3, 0), (4, 10), (5, None), (6, 200), (7, None), (8, 1)])
+    _refused(lib.gsq_fp8_dequant, [P, 208, P, 2, 5, 200, P, 0, 200, None],
+             [(0, None), (1, 200), (2, None), (3, 1), (4, 0), (5, 0), (6, None), (7, 3), (8, 199)])
+    gemm = [8, 16, 200, P, 208, P, 8, P, 208, P, 0, 2, 1, P, 0, 16, 0, P, None]
+    _refused(lib.gsq_fp8_gemm, gemm,
+             [(0, 0), (1, 0), (2, 0), (3, None), (3, odd), (4, 200), (4, 192), (5, None), (6, 7),
+              (7, None), (8, 200), (9, None), (11, -1), (13, None), (13, odd), (14, 3), (15, 15),
+              (16, 1), (17, None)])
+    rows = list(gemm)
+    rows[10], rows[12] = 1, 15   # a scale per row needs its 16 rows in every block
+    assert lib.gsq_fp8_gemm(*rows) == _lib.GSQ_EINVAL
+    _refused(lib.gsq_fp8_linear, [P, 0, 8, 200, 200, P, 208, P, 2, 16, P, 0, 16, P, 8 * 216, P, None],
+             [(0, None), (2, 0), (5, None), (6, 200), (8, 1), (9, 0), (10, None), (13, None),
+              (13, odd), (14, 8 * 216 - 1), (15, None)])
+
+
+def test_rope_entry_point_refuses_bad_arguments():
+    lib = _lib.load()
+    ok = [P, 128, 64, 2, P, 128, 64, 1, 4, 64, 32, 0, 0, P, 0, P, 1.0, 0, P, 128, 64, P, 64, 64, None]
+    _refused(lib.gsq_rope, ok,
+             [(0, None), (3, 0), (4, None), (7, -1), (8, 0), (9, 0), (10, 0), (10, 31), (10, 66),
+              (12, 3), (13, None), (13, C.c_void_p(4098)), (15, None), (15, C.c_void_p(4100)),
+              (18, None), (21, None), (0, C.c_void_p(4097))])
+
+
+def test_norm_entry_points_refuse_bad_arguments():
+    lib = _lib.load()
+    fwd = [P, 64, P, 64, P, P, P, 2, 4, 64, 0, 1.0, 1e-6, 0.0, P, 64, P, 64, None, 0, None, 0, P, None]
+    _refused(lib.gsq_residual_norm, fwd,
+             [(0, None), (1, 63), (2, None), (3, 63), (5, None), (7, 3), (7, 0), (8, 0), (9, 0),
+              (10, 3), (15, 63), (16, None), (17, 63), (18, P), (22, None), (0, C.c_void_p(4097))])
+    q = list(fwd)
+    q[16], q[18], q[19], q[20], q[21] = None, P, 64, P, 4
+    _refused(lib.gsq_residual_norm, q, [(19, 65), (19, 48), (20, None), (21, 3),
+                                        (18, C.c_void_p(4104))])
+    wide = list(fwd)
+    for i in (1, 3, 9, 15, 17):
+        wide[i] = 32769
+    assert lib.gsq_residual_norm(*wide) == _lib.GSQ_ENOTSUP
+    n = C.c_int64()
+    for bad in ((0, 64, 0), (4, 0, 0), (4, 64, 3), (4, 64, -1)):
+        assert lib.gsq_residual_norm_bwd_workspace(*bad, C.byref(n)) == _lib.GSQ_EINVAL
+    assert lib.gsq_residual_norm_bwd_workspace(4, 64, 0, None) == _lib.GSQ_EINVAL
+    bwd = [P, 64, P, 64, P, P, P, 2, P, P, 64, P, 64, 4, 64, 0, 1.0, 0.0, P, 64, P, 64, P, P, P, P,
+           1 << 40, None]
+    _refused(lib.gsq_residual_norm_bwd, bwd,
+             [(0, None), (1, 63), (2, None), (6, None), (7, 3), (8, None), (10, 63), (11, None),
+              (12, 63), (13, 0), (14, 0), (15, 3), (18, None), (20, None), (22, None), (23, None),
+              (24, None), (25, None), (26, 16)])
+    none = list(bwd)
+    none[5], none[9], none[11], none[23] = None, None, None, None   # neither cotangent
+    assert lib.gsq_residual_norm_bwd(*none) == _lib.GSQ_EINVAL

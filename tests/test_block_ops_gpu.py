@@ -1,0 +1,612 @@
+"""The 8-bit linear, the rotary positions and the residual norms on the GPU against the float64
+oracles, at the sizes, layouts and values where they can go wrong. The tolerances count roundings:
+u = 2^-24 of float32, half a step of the output's type, and the number of float32 operations
+between input and output, each applied to the magnitudes that the operation adds up."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import blockops as ob
+from oracle import fp8 as of
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+DT = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
+
+
+def half(dtype):
+    """Half a step of the type, relative (float32 outputs round by U)."""
+    return torch.finfo(dtype).eps / 2
+
+
+def tiny(dtype):
+    """Half the least step of the type (its denormals)."""
+    return torch.finfo(dtype).tiny * torch.finfo(dtype).eps / 2
+
+
+def f64(t):
+    return t.detach().double().cpu().numpy()
+
+
+def f32(t):
+    return t.detach().float().cpu().numpy()
+
+
+def rnd(shape, seed, dtype=torch.float32, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (scale * torch.randn(*shape, generator=g)).to(dtype).cuda()
+
+
+def near(got, want, tol, what=""):
+    d = np.abs(got - want) - tol
+    assert np.all(d <= 0), f"{what}: off by {d.max()} more than allowed at {np.argmax(d)}"
+
+
+# ------------------------------------------------------------------------------ 8-bit linear ---
+def _err_ok():
+    from gsq_rco_mlx_b200.gemm import check_err
+    torch.cuda.synchronize()
+    check_err(torch.device("cuda", torch.cuda.current_device()))
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("R,C", [(1, 1), (1, 128), (3, 129), (130, 127), (17, 896), (257, 1000),
+                                 (128, 256), (5, 4864)])
+def test_quantized_codes_are_the_oracles(R, C, dtype):
+    """Rows, weights (128 x 128) and columns: codes and scales bit for bit."""
+    from gsq_rco_mlx_b200 import _lib
+    from gsq_rco_mlx_b200.common.fp8 import Fp8Linear, quantize_rows
+    x = rnd((R, C), R + C, DT[dtype]) * torch.exp(2 * rnd((R, 1), 1)).to(DT[dtype])
+    x[0, :100] = 0
+    q = quantize_rows(x)
+    qo, so = of.quantize_rows(f32(x))
+    assert np.array_equal(f32(q.codes), qo) and np.array_equal(f32(q.scales), so)
+    lin = Fp8Linear.from_weight(x)
+    qo, so = of.quantize_blocks(f32(x))
+    assert np.array_equal(f32(lin.codes), qo) and np.array_equal(f32(lin.scales), so)
+    assert np.array_equal(f32(lin.codes_t()), qo.T)
+    ld, rb = -(-R // 16) * 16, -(-R // 128)
+    codes_t = torch.zeros(C, ld, device="cuda", dtype=torch.uint8)
+    scales_t = torch.zeros(rb, C, device="cuda")
+    _lib.call("gsq_fp8_quant", x.data_ptr(), list(DT).index(dtype), R, C, C, None, 0, None, 0,
+              codes_t.data_ptr(), ld, scales_t.data_ptr(), C, _lib.stream_ptr())
+    qo, so = of.quantize_rows(f32(x).T)
+    assert np.array_equal(f32(codes_t.view(torch.float8_e4m3fn)[:, :R]), qo)
+    assert np.array_equal(f32(scales_t), so.T)
+    out = torch.empty(R, C, device="cuda", dtype=DT[dtype])
+    lin.dequant(out)
+    v = of.blocks_value(*of.quantize_blocks(f32(x)))
+    near(f64(out), v, (half(DT[dtype]) + U) * np.abs(v) + tiny(DT[dtype]))
+
+
+def _tol_gemm(mag, K, dtype, ref):
+    """A block's 128 products are exact; their float32 sum on the tensor cores may truncate, one
+    step (2 u) for each of 128 additions; the scales' product, the multiply by it (two with a
+    scale per row of both sides) and the addition over blocks round by u each."""
+    return (256 + 3 + -(-K // 128)) * U * mag + half(dtype) * np.abs(ref) * (1 + 1e-6) + tiny(dtype)
+
+
+SHAPES = [(1, 1, 1), (1, 896, 1152), (2, 130, 257), (8, 128, 128), (16, 4864, 896), (17, 1000, 64),
+          (64, 896, 4864), (65, 257, 333), (129, 128, 1), (300, 129, 1000), (1000, 896, 900),
+          (2047, 64, 4864)]
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("M,K,N", SHAPES)
+def test_fp8_linear(M, K, N, dtype):
+    from gsq_rco_mlx_b200.common.fp8 import Fp8Linear, quantize_rows
+    lin = Fp8Linear.from_weight(rnd((N, K), 1, scale=0.05))
+    x = rnd((M, K), 2, DT[dtype])
+    y = lin(x)
+    y32 = lin(x, y_f32=True)
+    yq = lin(quantize_rows(x))
+    _err_ok()
+    ref, mag = of.linear(f32(x), f32(lin.codes), f32(lin.scales))
+    assert y.dtype == DT[dtype] and y32.dtype == torch.float32 and yq.dtype == torch.bfloat16
+    near(f64(y), ref, _tol_gemm(mag, K, DT[dtype], ref))
+    near(f64(y32), ref, _tol_gemm(mag, K, torch.float32, ref))
+    near(f64(yq), ref, _tol_gemm(mag, K, torch.bfloat16, ref))
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("M,K,N", SHAPES[1:])
+def test_fp8_vjp(M, K, N, dtype):
+    from gsq_rco_mlx_b200.common.fp8 import Fp8Linear
+    lin = Fp8Linear.from_weight(rnd((N, K), 3, scale=0.05), transposed=M % 2 == 0)
+    x, dy = rnd((M, K), 4, DT[dtype]), rnd((M, N), 5, DT[dtype], 0.01)
+    dx, dw = lin.vjp(x, dy)
+    base = rnd((N, K), 6)
+    acc = base.clone()
+    lin.vjp(x, dy, dw=acc, accumulate=True)
+    _err_ok()
+    rx, mx, rw, mw = of.vjp(f32(x), f32(dy), f32(lin.codes), f32(lin.scales))
+    near(f64(dx), rx, _tol_gemm(mx, N, DT[dtype], rx), "dx")
+    near(f64(dw), rw, _tol_gemm(mw, M, torch.float32, rw), "dw")
+    near(f64(acc), rw + f64(base), _tol_gemm(mw, M, torch.float32, rw)
+         + U * np.abs(rw + f64(base)), "dw added")
+
+
+def test_fp8_strides_outputs_and_refusals():
+    """Rows of a wider buffer, a transposed input, outputs inside a wider buffer (whose other
+    columns stay), no rows at all; and what is refused."""
+    from gsq_rco_mlx_b200.common.fp8 import Fp8Linear, Fp8Tensor, quantize_rows
+    K, N = 200, 130
+    lin = Fp8Linear.from_weight(rnd((N, K), 7))
+    wide = rnd((9, 333), 8, torch.bfloat16)
+    x = wide[:, 7:7 + K]
+    buf = torch.full((9, 200), 7.0, device="cuda", dtype=torch.bfloat16)
+    lin(x, out=buf[:, 3:3 + N])
+    want = lin(x.contiguous())
+    assert torch.equal(buf[:, 3:3 + N], want)
+    assert bool((buf[:, :3] == 7).all()) and bool((buf[:, 3 + N:] == 7).all())
+    xt = x.t().contiguous().t()
+    assert torch.equal(lin(xt), want)
+    e = lin(x[:0])
+    assert e.shape == (0, N)
+    dx, dw = lin.vjp(x[:0], want[:0])
+    assert dx.shape == (0, K) and not bool(dw.any())
+    W = torch.empty(N, K, device="cuda", dtype=torch.bfloat16)
+    lin.dequant(W)
+    # a weight whose rows are not on 16 bytes, and scales of other strides
+    c = torch.zeros(N, K + 3, device="cuda", dtype=torch.uint8)
+    c[:, 3:] = lin.codes.view(torch.uint8)
+    other = Fp8Linear(c[:, 3:].view(torch.float8_e4m3fn), lin.scales.t().contiguous().t())
+    assert torch.equal(other(x), want)
+    for bad in (lambda: lin(x[:, :K - 1]), lambda: lin(x.double()), lambda: lin(x.cpu()),
+                lambda: lin(x, out=buf), lambda: lin(x, out=buf[:, :N].float()),
+                lambda: lin(x.reshape(1, 9, K)), lambda: lin.vjp(x, want[:8]),
+                lambda: lin.vjp(x, want, accumulate=True),
+                lambda: lin.vjp(x, want, dw=torch.empty(N, K, device="cuda").half()),
+                lambda: lin(quantize_rows(x[:, :K - 1])),
+                lambda: Fp8Linear(lin.codes, lin.scales[:1]),
+                lambda: Fp8Linear(lin.codes, lin.scales.double()),
+                lambda: Fp8Linear(lin.codes.view(torch.uint8), lin.scales),
+                lambda: Fp8Linear(lin.codes, lin.scales, codes_t=lin.codes),
+                lambda: Fp8Tensor(lin.codes, lin.scales)):
+        with pytest.raises(ValueError):
+            bad()
+
+
+@pytest.mark.parametrize("M", [3, 200])
+def test_fp8_not_finite_and_extreme_values(M):
+    """NaN or infinity in a row reaches that row only; zeros, denormals and the type's largest
+    values stay finite where the product does."""
+    from gsq_rco_mlx_b200.common.fp8 import Fp8Linear
+    K, N = 300, 140
+    lin = Fp8Linear.from_weight(rnd((N, K), 9))
+    x = rnd((M, K), 10)
+    clean = lin(x)
+    x2 = x.clone()
+    x2[1, 290] = float("inf")
+    x2[2, 5] = float("nan")
+    y = lin(x2)
+    _err_ok()
+    assert bool(torch.isnan(y[1:3]).all())
+    assert torch.equal(y[0], clean[0]) and torch.equal(y[3:], clean[3:])
+    z = torch.zeros(M, K, device="cuda")
+    assert not bool(lin(z).any())
+    z[:, ::2] = 1e-42   # denormal: below the floor of the scale, rounds to zero codes
+    assert not bool(lin(z).any())
+    big = torch.full((M, K), 3e37, device="cuda")
+    ref, mag = of.linear(f32(big), f32(lin.codes), f32(lin.scales))
+    # 300 products of 3e37 and weights of order 1 add up to 5e38 and more, beyond float32's
+    # 3.4e38, where infinity is the right answer: an output is finite exactly where the sums over
+    # the first one, two and three blocks all are (the sum inside a block is in units of the
+    # codes, at most 128 * 448^2)
+    xv = of.rows_value(*of.quantize_rows(f32(big)))
+    wv = of.blocks_value(f32(lin.codes), f32(lin.scales))
+    part = np.cumsum([xv[:, a:a + 128] @ wv[:, a:a + 128].T for a in range(0, K, 128)], 0)
+    top = np.abs(part).max(0) / float(np.finfo(np.float32).max)
+    got = f64(lin(big))
+    fits, over = top < 1 - 1e-4, top > 1 + 1e-4
+    assert fits.any() and over.any() and not np.isfinite(got[over]).any()
+    near(got[fits], ref[fits], _tol_gemm(mag, K, torch.float32, ref)[fits])
+
+
+# ------------------------------------------------------------------------------------- rotary ---
+SCALINGS = [None, {"type": "linear", "factor": 4.0}, {"type": "ntk", "factor": 8.0},
+            {"type": "yarn", "factor": 8.0, "original": 4096},
+            {"type": "bands", "factor": 8.0, "original": 8192}]
+
+
+def _rope_tol(x, positions, w, rot, layout, factor, dtype, ref):
+    """The remainder of the angle (in half turns) is rounded to float32 (2^-25 half turns, 2^-25 pi
+    radians), the whole angle in 64 bits carries 4 2^-53 of itself; sine and cosine are good to 2
+    steps (4 u), the factor and the two products and their sum round by u each."""
+    a = np.abs(x)
+    mag = a.copy()
+    t = np.abs(np.asarray(positions, np.float64))[:, None]
+    ang = np.zeros_like(a)
+    for j in range(rot // 2):
+        p, q = (j, j + rot // 2) if layout == "half" else (2 * j, 2 * j + 1)
+        mag[..., p] = mag[..., q] = a[..., p] + a[..., q]
+        ang[..., p] = ang[..., q] = 4 * 2.0 ** -53 * t * w[j]
+    return factor * mag * (np.pi * 2.0 ** -25 + 8 * U + ang) + half(dtype) * np.abs(ref) + tiny(dtype)
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("T,nq,nk,hd,rot", [(1, 14, 2, 64, 64), (1, 1, 0, 2, 2), (7, 8, 1, 128, 64),
+                                            (33, 3, 3, 80, 20), (513, 4, 2, 96, 96),
+                                            (5, 2, 1, 33, 6), (2, 7, 1, 256, 128),
+                                            (70, 64, 8, 128, 128)])
+def test_rotary(T, nq, nk, hd, rot, layout, dtype):
+    from gsq_rco_mlx_b200.common.rotary import Rotary
+    d = DT[dtype]
+    sc = SCALINGS[(T + nq + hd) % len(SCALINGS)]
+    r = Rotary(hd, 1e6, rot, layout, sc)
+    packed = rnd((T, (nq + 2 * nk) * hd), T, d)
+    q = packed[:, :nq * hd].view(T, nq, hd)
+    k = packed[:, nq * hd:(nq + nk) * hd].view(T, nk, hd) if nk else None
+    rng = np.random.default_rng(T)
+    pos = rng.integers(-5, 4000000, T)
+    pos[0] = 2 ** 31 - 1 if T > 1 else 1000003
+    p = torch.from_numpy(pos).cuda()
+    keep = packed.clone()
+    for inverse in (False, True):
+        f = r.vjp if inverse else r
+        qo, ko = f(q, k, p.int() if pos.max() < 2 ** 31 else p)
+        for x, o in ((q, qo), (k, ko)):
+            if x is None:
+                assert o is None
+                continue
+            ref = ob.rotate(f64(x), pos, r.freqs, rot, layout, r.factor, inverse)
+            near(f64(o), ref, _rope_tol(f64(x), pos, r.freqs, rot, layout, r.factor, d, ref))
+            assert torch.equal(o[..., rot:], x[..., rot:])
+        q64, _ = f(q, k, p)   # int64 positions: the same bits
+        assert torch.equal(q64, qo)
+    assert torch.equal(packed, keep)
+    # in place on the packed rows: q and k as above, v untouched
+    qo, ko = r(q, k, p)
+    r(q, k, p, out=(q, k))
+    assert torch.equal(q, qo) and (k is None or torch.equal(k, ko))
+    assert torch.equal(packed[:, (nq + nk) * hd:], keep[:, (nq + nk) * hd:])
+
+
+def test_rotary_far_positions_and_layouts():
+    """int64 positions beyond 2^31, head-major buffers, unaligned rows, a broadcast key input."""
+    from gsq_rco_mlx_b200.common.rotary import Rotary
+    r = Rotary(64, 1e6)
+    T = 19
+    pos = np.arange(T) + 5 * 2 ** 32
+    p = torch.from_numpy(pos).cuda()
+    hm = rnd((3, T, 64), 1).transpose(0, 1)
+    q, _ = r(hm, None, p)
+    ref = ob.rotate(f64(hm), pos, r.freqs, 64, "half")
+    near(f64(q), ref, _rope_tol(f64(hm), pos, r.freqs, 64, "half", 1.0, torch.float32, ref))
+    odd = rnd((T, 3 * 65 + 1), 2, torch.float16)
+    v = odd[:, 1:].view(T, 3, 65)[:, :, :64] if odd[:, 1:].is_contiguous() else \
+        torch.as_strided(odd, (T, 3, 64), (3 * 65 + 1, 65, 1), 1)
+    assert torch.equal(r(v, None, p)[0], r(v.contiguous(), None, p)[0])
+    k1 = rnd((T, 1, 64), 3).expand(T, 4, 64)   # a shared key head read four times
+    _, ko = r(hm, k1, p)
+    assert torch.equal(ko, r(hm, k1.contiguous(), p)[1])
+    out = torch.zeros(3, T, 64, device="cuda").transpose(0, 1)
+    r(hm, None, p, out=(out, None))
+    assert torch.equal(out, q)
+    e, _ = r(hm[:0], None, p[:0])
+    assert e.shape == (0, 3, 64)
+    for bad in (lambda: r(hm, None, p[:-1]), lambda: r(hm, None, p.float()),
+                lambda: r(hm, None, p.cpu()), lambda: r(hm, hm.half(), p),
+                lambda: r(hm[..., :32], None, p), lambda: r(hm, hm[:5], p),
+                lambda: r(hm, hm, p, out=(out, None)),
+                lambda: r(hm, None, p, out=(k1, None)),
+                lambda: r(hm[:, :0], None, p),
+                lambda: r(torch.zeros(T, 64, 3, device="cuda").transpose(1, 2), None, p),
+                lambda: r(hm, None, p, out=(torch.as_strided(hm, (T, 3, 64), (192, 64, 1)), None))):
+        with pytest.raises(ValueError):
+            bad()
+
+
+def test_rotary_values_that_are_not_finite():
+    """NaN and infinity stay inside their pair."""
+    from gsq_rco_mlx_b200.common.rotary import Rotary
+    r = Rotary(16, 1e4, 8, "interleaved")
+    q = rnd((3, 2, 16), 4)
+    p = torch.arange(3, device="cuda")
+    clean, _ = r(q, None, p)
+    q[1, 0, 3] = float("nan")
+    q[2, 1, 15] = float("inf")
+    o, _ = r(q, None, p)
+    assert bool(torch.isnan(o[1, 0, 2:4]).all()) and float(o[2, 1, 15]) == float("inf")
+    same = torch.ones_like(o, dtype=torch.bool)
+    same[1, 0, 2:4] = False
+    same[2, 1, 15] = False
+    assert torch.equal(o[same], clean[same])
+
+
+# ------------------------------------------------------------------------------ residual norms ---
+def _norm_inputs(T, H, dtype, post, pre, gates, seed=0):
+    d = DT[dtype]
+    v = {"h": rnd((T, H), seed + 1, d, 2.0), "y": rnd((T, H), seed + 2, d)}
+    v["w_post"] = (1 + rnd((H,), seed + 3, scale=0.2)).to(d) if post else None
+    v["w_pre"] = (1 + rnd((H,), seed + 4, scale=0.2)).to(d) if pre else None
+    v["gate"] = rnd((gates, H), seed + 5, d) if gates else None
+    v["dh"] = rnd((T, H), seed + 6, d)
+    v["dx"] = rnd((T, H), seed + 7, d) if pre else None
+    return v
+
+
+def _o(v):
+    return {k: None if t is None else f64(t) for k, t in v.items()}
+
+
+NORMS = [(1, 1, True, True, 0), (1, 896, True, True, 1), (5, 128, False, True, 0),
+         (6, 257, True, False, 3), (33, 896, True, True, 0), (40, 1000, True, True, 40),
+         (12, 1025, False, True, 4), (9, 2048, True, True, 1), (7, 4097, True, True, 7),
+         (1200, 64, True, True, 2), (3, 8192, True, False, 1), (2, 12345, True, True, 1),
+         (2, 32768, True, True, 2), (2500, 100, False, True, 1), (3, 5, True, True, 3)]
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("T,H,post,pre,gates", NORMS)
+def test_residual_norm(T, H, post, pre, gates, dtype):
+    """The squares' sum adds at most 32 values a thread, 32 threads and 32 warps in trees or
+    chains of at most 48 roundings; half of it reaches the reciprocal root, which rounds by 4 u
+    more; then at most 6 products: 40 u covers n, and once more x."""
+    from gsq_rco_mlx_b200.common.norm import residual_norm
+    d = DT[dtype]
+    v = _norm_inputs(T, H, dtype, post, pre, gates)
+    off = 0.0 if T % 2 else 1.0
+    h2, x, stats = residual_norm(v["h"], v["y"], v["w_post"], v["w_pre"], gate=v["gate"], scale=0.7,
+                                 eps=1e-5, offset=off)
+    o = _o(v)
+    rh, rx, r1, r2, n = ob.residual_norm(o["h"], o["y"], o["w_post"], o["w_pre"], o["gate"], 0.7,
+                                         1e-5, off)
+    hm = np.abs(o["h"]) + np.abs(rh - o["h"])
+    near(f64(h2), rh, 40 * U * hm + half(d) * np.abs(rh) + tiny(d), "h")
+    # r2 moves by the relative error of the root mean square of h'
+    e2 = 40 * U * (1 + np.sqrt((hm ** 2).mean(1, keepdims=True)) * r2)
+    near(f64(stats), np.stack([r1[:, 0], r2[:, 0]]),
+         np.stack([40 * U * r1[:, 0], (e2 * r2)[:, 0] if pre else 0 * r2[:, 0]]), "stats")
+    if not pre:
+        assert x is None
+        return
+    b = np.abs(o["w_pre"] + off)
+    near(f64(x), rx, 40 * U * hm * r2 * b + e2 * np.abs(rx) + half(d) * np.abs(rx) + tiny(d), "x")
+    h3, q, s3 = residual_norm(v["h"], v["y"], v["w_post"], v["w_pre"], gate=v["gate"], scale=0.7,
+                              eps=1e-5, offset=off, fp8=True)
+    assert torch.equal(h3, h2) and torch.equal(s3, stats)
+    # the codes' values within half a step of x (2^-4, or 2^-10 of the scale), x as above
+    sc = np.repeat(f64(q.scales), 128, 1)[:, :H]
+    xt = 40 * U * hm * r2 * b + e2 * np.abs(rx)
+    near(f64(q.float()), rx, xt + np.maximum(2.0 ** -4 * (np.abs(rx) + xt), 2.0 ** -10 * sc)
+         * (1 + 2.0 ** -18) + 2.0 ** -22 * np.abs(rx), "e4m3")
+    amax = np.abs(np.pad(rx, ((0, 0), (0, -H % 128)))).reshape(T, -1, 128).max(2)
+    xm = np.pad(xt, ((0, 0), (0, -H % 128))).reshape(T, -1, 128).max(2)
+    near(f64(q.scales), np.maximum(amax, 2.0 ** -100) / 448, (xm + 2 * U * amax) / 448, "scales")
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("T,H,post,pre,gates", NORMS)
+def test_residual_norm_vjp(T, H, post, pre, gates, dtype):
+    """Along a row: the statistics carry 40 u, each mean of products at most 48 roundings more and
+    there are two of them, each formed from at most 12 products: 200 u of the magnitudes (of the
+    first gradient, and once more through the second). Over rows: one rounding a row at most."""
+    from gsq_rco_mlx_b200.common.norm import residual_norm, residual_norm_vjp
+    d = DT[dtype]
+    v = _norm_inputs(T, H, dtype, post, pre, gates, seed=20)
+    off = 1.0 if T % 2 else 0.0
+    _, _, stats = residual_norm(v["h"], v["y"], v["w_post"], v["w_pre"], gate=v["gate"], scale=0.7,
+                                eps=1e-5, offset=off)
+    dh = None if (T % 3 == 0 and pre) else v["dh"]
+    g = residual_norm_vjp(v["h"], v["y"], v["w_post"], v["w_pre"], stats, dh, v["dx"],
+                          gate=v["gate"], scale=0.7, offset=off)
+    again = residual_norm_vjp(v["h"], v["y"], v["w_post"], v["w_pre"], stats, dh, v["dx"],
+                              gate=v["gate"], scale=0.7, offset=off)
+    o = _o(v)
+    ref, mag = ob.residual_norm_vjp(o["h"], o["y"], o["w_post"], o["w_pre"],
+                                    None if dh is None else o["dh"], o["dx"], o["gate"], 0.7, 1e-5,
+                                    off)
+    for name in ("dh", "dy", "dw_post", "dw_pre", "dgate"):
+        if name not in ref:
+            assert g[name] is None
+            continue
+        assert torch.equal(g[name], again[name]), name
+        if name in ("dh", "dy"):
+            tol = 400 * U * mag[name] + half(d) * np.abs(ref[name]) + tiny(d)
+        else:
+            assert g[name].dtype == torch.float32
+            tol = (400 + T) * U * mag[name]
+        near(f64(g[name]), ref[name], tol, name)
+
+
+def test_residual_norm_rows_strides_and_refusals():
+    """Rows of wider and odd buffers, h updated in place, rows behind the last left alone, a row of
+    zeros, values that are not finite, no rows; and what is refused."""
+    from gsq_rco_mlx_b200.common.norm import residual_norm, residual_norm_vjp
+    T, H = 6, 200
+    v = _norm_inputs(T, H, "bf16", True, True, 2)
+    kw = dict(gate=v["gate"], scale=0.5)
+    args = (v["w_post"], v["w_pre"])
+    h2, x, st = residual_norm(v["h"], v["y"], *args, **kw)
+    for pad in (8, 3):
+        wide = torch.full((T + 2, H + pad), 9.0, device="cuda", dtype=torch.bfloat16)
+        rows = wide[:T, pad:]
+        rows.copy_(v["h"])
+        out, x2, st2 = residual_norm(rows, v["y"], *args, out=rows, **kw)
+        assert out.data_ptr() == rows.data_ptr() and torch.equal(rows, h2) and torch.equal(x2, x)
+        assert torch.equal(st2, st)
+        assert bool((wide[T:] == 9).all()) and bool((wide[:, :pad] == 9).all())
+        rows.copy_(v["h"])
+        g = residual_norm_vjp(rows, v["y"], *args, st, v["dh"], v["dx"], **kw)
+        want = residual_norm_vjp(v["h"], v["y"], *args, st, v["dh"], v["dx"], **kw)
+        assert all(torch.equal(g[n], want[n]) for n in g)
+    z = torch.zeros_like(v["h"])
+    h0, x0, s0 = residual_norm(z, z, *args, **kw)
+    assert not bool(h0.any()) and not bool(x0.any())
+    near(f64(s0), np.full((2, T), 1e3), 4 * U * 1e3)
+    bad = v["y"].clone()
+    bad[1, 7], bad[3, 0] = float("nan"), float("inf")
+    h3, x3, _ = residual_norm(v["h"], bad, *args, **kw)
+    ok = [0, 2, 4, 5]
+    assert torch.equal(h3[ok], h2[ok]) and torch.equal(x3[ok], x[ok])
+    assert bool(torch.isnan(x3[[1, 3]]).any(1).all())
+    one, xo, _ = residual_norm(v["h"], v["y"], *args, gate=v["gate"][0], scale=0.5)
+    assert torch.equal(one[:3], h2[:3]) and torch.equal(xo[:3], x[:3])
+    e = residual_norm(v["h"][:0], v["y"][:0], *args, gate=v["gate"][0])
+    assert e[0].shape == (0, H) and e[2].shape == (2, 0)
+    ge = residual_norm_vjp(v["h"][:0], v["y"][:0], *args, e[2], v["dh"][:0], v["dx"][:0],
+                           gate=v["gate"][0])
+    assert not bool(ge["dw_pre"].any()) and ge["dgate"].shape == (H,)
+    f = residual_norm
+    for call in (lambda: f(v["h"], v["y"][:5], *args), lambda: f(v["h"], v["y"].float(), *args),
+                 lambda: f(v["h"], v["y"], v["w_post"][:9]), lambda: f(v["h"].double(), v["y"]),
+                 lambda: f(v["h"], v["y"], *args, gate=v["gate"].float()),
+                 lambda: f(v["h"], v["y"], *args, gate=torch.zeros(4, H, device="cuda").bfloat16()),
+                 lambda: f(v["h"], v["y"], v["w_post"], fp8=True), lambda: f(v["h"].cpu(), v["y"]),
+                 lambda: f(v["h"], v["y"], v["w_post"].cpu()),
+                 lambda: f(v["h"], v["y"], *args, out=h2.float()),
+                 lambda: f(torch.zeros(1, 32769, device="cuda"), torch.zeros(1, 32769, device="cuda"),
+                           torch.zeros(32769, device="cuda")),
+                 lambda: residual_norm_vjp(v["h"], v["y"], *args, st[:, :5], v["dh"], v["dx"]),
+                 lambda: residual_norm_vjp(v["h"], v["y"], *args, st, v["dh"], None),
+                 lambda: residual_norm_vjp(v["h"], v["y"], v["w_post"], None, st, v["dh"], v["dx"]),
+                 lambda: residual_norm_vjp(v["h"], v["y"], v["w_post"], None, st, None, None)):
+        with pytest.raises(ValueError):
+            call()
+
+
+# ------------------------------------------------------------------------------------ together ---
+def _block(seed=0, H=256, T=300, heads=4, kv=2, hd=64):
+    from gsq_rco_mlx_b200.common.fp8 import Fp8Linear
+    from gsq_rco_mlx_b200.common.rotary import Rotary
+    W = rnd(((heads + 2 * kv) * hd, H), seed, torch.bfloat16, 0.05)
+    lin = Fp8Linear.from_weight(W, transposed=True)
+    rot = Rotary(hd, 1e4, 32, "half", SCALINGS[3])
+    v = _norm_inputs(T, H, "bf16", True, True, 1, seed)
+    pos = torch.arange(T, device="cuda")
+    return lin, rot, v, pos, heads, kv, hd
+
+
+def _forward(lin, rot, v, pos, heads, kv, hd, fp8=True):
+    from gsq_rco_mlx_b200.common.norm import residual_norm
+    h2, x, st = residual_norm(v["h"], v["y"], v["w_post"], v["w_pre"], gate=v["gate"], scale=0.7,
+                              fp8=fp8)
+    qkv = lin(x)
+    T = qkv.shape[0]
+    q = qkv[:, :heads * hd].view(T, heads, hd)
+    k = qkv[:, heads * hd:(heads + kv) * hd].view(T, kv, hd)
+    qr, kr = rot(q, k, pos)
+    return h2, x, st, qkv, qr, kr
+
+
+def _backward(lin, rot, v, pos, heads, kv, hd, st, x, dq, dk, dv):
+    """Cotangents of (q, k, v) back to h, y and every parameter."""
+    from gsq_rco_mlx_b200.common.norm import residual_norm_vjp
+    T = pos.shape[0]
+    dqkv = torch.empty(T, (heads + 2 * kv) * hd, device="cuda", dtype=torch.bfloat16)
+    rot.vjp(dq, dk, pos, out=(dqkv[:, :heads * hd].view(T, heads, hd),
+                              dqkv[:, heads * hd:(heads + kv) * hd].view(T, kv, hd)))
+    dqkv[:, (heads + kv) * hd:] = dv
+    dx, dw = lin.vjp(x, dqkv)
+    g = residual_norm_vjp(v["h"], v["y"], v["w_post"], v["w_pre"], st, v["dh"], dx,
+                          gate=v["gate"], scale=0.7)
+    return dict(g, dw=dw, dx=dx)
+
+
+def test_norm_linear_rotary_in_a_row():
+    """The norm into 8-bit rows, the projection and the rotation as a block runs them, each stage
+    against the oracle on the stage's own inputs; the 8-bit rows are those of the float32 norm."""
+    lin, rot, v, pos, heads, kv, hd = args = _block()
+    h2, x, st, qkv, qr, kr = _forward(*args)
+    _err_ok()
+    wv = of.blocks_value(f32(lin.codes), f32(lin.scales))
+    xv = f64(x.float())
+    ref, mag = xv @ wv.T, np.abs(xv) @ np.abs(wv).T
+    near(f64(qkv), ref, _tol_gemm(mag, 256, torch.bfloat16, ref), "qkv")
+    for a, b, o in ((0, heads, qr), (heads, heads + kv, kr)):
+        z = f64(qkv[:, a * hd:b * hd]).reshape(-1, b - a, hd)
+        ref = ob.rotate(z, f64(pos), rot.freqs, 32, "half", rot.factor)
+        near(f64(o), ref, _rope_tol(z, f64(pos), rot.freqs, 32, "half", rot.factor, torch.bfloat16,
+                                    ref), "rotary")
+    _, xb, _, qkvb, _, _ = _forward(*args, fp8=False)
+    g = _backward(*args, st, xb, v["dh"].view(300, 4, 64), v["dx"][:, :128].reshape(300, 2, 64),
+                  v["dx"][:, 128:])
+    assert all(bool(torch.isfinite(t).all()) for t in g.values())
+
+
+def test_captured_graphs_streams_and_overlapping_calls():
+    """Two graphs of the same objects replayed in turn and on two streams at once give what eager
+    calls give; so does a call on a side stream."""
+    argsA, argsB = _block(0), _block(50)
+    v = argsA[2]
+
+    def step(a):
+        h2, x, st, qkv, qr, kr = _forward(*a, fp8=False)
+        g = _backward(*a, st, x, qr, kr, a[2]["dx"][:, 128:])
+        return [h2, x, st, qkv, qr, kr] + list(g.values())
+
+    # one weight and plan, two inputs
+    argsB = (argsA[0], argsA[1], argsB[2], *argsA[3:])
+    eager = [step(a) for a in (argsA, argsB)]
+    graphs, outs = [], []
+    for a in (argsA, argsB):
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            step(a)
+        torch.cuda.current_stream().wait_stream(s)
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            outs.append(step(a))
+        graphs.append(gr)
+    for _ in range(2):
+        for gr in graphs:
+            gr.replay()
+    torch.cuda.synchronize()
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    for o in outs:
+        for t in o:
+            t.zero_()
+    torch.cuda.synchronize()
+    for _ in range(3):
+        with torch.cuda.stream(s1):
+            graphs[0].replay()
+        with torch.cuda.stream(s2):
+            graphs[1].replay()
+    torch.cuda.synchronize()
+    for o, e in zip(outs, eager):
+        assert all(torch.equal(a, b) for a, b in zip(o, e))
+    # eager calls on two streams at once
+    with torch.cuda.stream(s1):
+        r1 = step(argsA)
+    with torch.cuda.stream(s2):
+        r2 = step(argsB)
+    torch.cuda.synchronize()
+    for o, e in zip((r1, r2), eager):
+        assert all(torch.equal(a, b) for a, b in zip(o, e))
+    _err_ok()
+
+
+def test_fp8_layers_in_the_packed_eval():
+    """PackedModel takes Fp8Linear layers: its scratch weights are their dequantized values, and
+    the perplexity is that of the dense model with those weights."""
+    from gsq_rco_mlx_b200.common.evaluate import PackedModel, perplexity
+    from gsq_rco_mlx_b200.common.fp8 import Fp8Linear
+    from gsq_rco_mlx_b200.gsq.e2e import LIN_ORDER, BlockConfig
+    cfg = BlockConfig(hidden=128, n_heads=2, n_kv=1, head_dim=64, inter=256)
+    shapes = {"q_proj": (128, 128), "k_proj": (64, 128), "v_proj": (64, 128), "o_proj": (128, 128),
+              "gate_proj": (256, 128), "up_proj": (256, 128), "down_proj": (128, 256)}
+    bf = torch.bfloat16
+    layers8, layers16 = [], []
+    for L in range(2):
+        d = {"q_bias": rnd((128,), 100 + L, bf, 0.1), "k_bias": rnd((64,), 110 + L, bf, 0.1),
+             "v_bias": rnd((64,), 120 + L, bf, 0.1),
+             "in_norm": torch.ones(128, device="cuda", dtype=bf),
+             "post_norm": torch.ones(128, device="cuda", dtype=bf)}
+        d8, d16 = dict(d), dict(d)
+        for i, name in enumerate(LIN_ORDER):
+            lin = Fp8Linear.from_weight(rnd(shapes[name], 10 * L + i, bf, 0.08))
+            d8[name] = lin
+            d16[name] = torch.empty(shapes[name], device="cuda", dtype=bf)
+            lin.dequant(d16[name])
+        layers8.append(d8)
+        layers16.append(d16)
+    embed, nw = rnd((512, 128), 200, bf), torch.ones(128, device="cuda", dtype=bf)
+    win = np.random.default_rng(0).integers(0, 512, (3, 128))
+    m8, m16 = PackedModel(cfg, embed, nw, layers8), PackedModel(cfg, embed, nw, layers16)
+    a, b = perplexity(m8, win), perplexity(m16, win)
+    assert a == b and np.isfinite(a["ppl"])
+    n = sum(r * c + 4 * -(-r // 128) * -(-c // 128) for r, c in shapes.values())
+    assert m8.packed_bytes() == 2 * n and m16.packed_bytes() == 0
