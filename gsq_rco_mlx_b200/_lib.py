@@ -90,10 +90,10 @@ SIGNATURES = {
                  _i32, _vp, _f32, _i32, _vp, _i64, _i64, _vp, _i64, _i64, _vp],
     "gsq_residual_norm": [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _f32,
                           _f32, _f32, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp],
-    "gsq_residual_norm_bwd_workspace": [_i32, _i32, _i32, _vp],
+    "gsq_residual_norm_bwd_workspace": [_i32, _i32, _i32, _i32, _vp],
     "gsq_residual_norm_bwd": [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _i32, _vp, _vp, _i64, _vp,
                               _i64, _i32, _i32, _i32, _f32, _f32, _vp, _i64, _vp, _i64, _vp, _vp,
-                              _vp, _vp, _i64, _vp],
+                              _vp, _vp, _i64, _vp, _vp],
 }
 
 _lib = None
@@ -121,10 +121,16 @@ def load():
     return lib
 
 
+_on_gpu = False
+
+
 def lib():
     """The library, on a machine with a CUDA device (the product path requires one)."""
-    if not torch.cuda.is_available():
-        raise RuntimeError("gsq_rco_mlx_b200 needs a CUDA GPU (sm_100a); none is available")
+    global _on_gpu
+    if not _on_gpu:
+        if not torch.cuda.is_available():
+            raise RuntimeError("gsq_rco_mlx_b200 needs a CUDA GPU (sm_100a); none is available")
+        _on_gpu = True
     return load()
 
 
@@ -150,8 +156,10 @@ def ptr(t):
 
 
 def stream_ptr(stream=None):
-    s = stream if stream is not None else torch.cuda.current_stream()
-    return C.c_void_p(s.cuda_stream)
+    if stream is None:
+        # the handle itself: current_stream() builds a Stream object around it (3 us a call)
+        return C.c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
+    return C.c_void_p(stream.cuda_stream)
 
 
 class Launches:

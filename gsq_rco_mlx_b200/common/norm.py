@@ -17,6 +17,7 @@ import ctypes as C
 import torch
 
 from .. import _lib
+from ..gemm import err_flag
 from .fp8 import Fp8Tensor, pad16
 from .operands import DTYPES, matrix, on_device, output, pitch
 
@@ -112,7 +113,7 @@ def residual_norm_vjp(h, y, w_post, w_pre, stats, dh, dx, gate=None, scale=1.0, 
     if not T:
         return g
     n = C.c_int64()
-    _lib.check(_lib.lib().gsq_residual_norm_bwd_workspace(T, H, rows, C.byref(n)),
+    _lib.check(_lib.lib().gsq_residual_norm_bwd_workspace(T, H, DTYPES[dt], rows, C.byref(n)),
                "gsq_residual_norm_bwd_workspace")
     # allocated per call on the calling stream: nothing is shared between calls
     ws = torch.empty(n.value, device=dev, dtype=torch.uint8)
@@ -121,5 +122,5 @@ def residual_norm_vjp(h, y, w_post, w_pre, stats, dh, dx, gate=None, scale=1.0, 
               0 if dh is None else pitch(dh), _ptr(dx), 0 if dx is None else pitch(dx), T, H,
               DTYPES[dt], float(scale), float(offset), g["dh"].data_ptr(), H, g["dy"].data_ptr(),
               H, _ptr(g["dw_post"]), _ptr(g["dw_pre"]), _ptr(g["dgate"]), ws.data_ptr(),
-              ws.numel(), _lib.stream_ptr())
+              ws.numel(), err_flag(dev).data_ptr(), _lib.stream_ptr())
     return g

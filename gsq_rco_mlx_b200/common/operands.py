@@ -10,7 +10,7 @@ def on_device(t, what):
     """t is on the current CUDA device (where the launch and its stream are)."""
     if not t.is_cuda:
         raise ValueError(f"{what} must be a CUDA tensor")
-    if t.device.index != torch.cuda.current_device():
+    if t.get_device() != torch.cuda.current_device():
         raise ValueError(f"{what} is on {t.device}, the current device is "
                          f"cuda:{torch.cuda.current_device()}")
 

@@ -92,57 +92,65 @@ class Rotary:
         self.turns = torch.from_numpy(self.freqs / (2 * math.pi)).to(device or _lib.device())
 
     def _side(self, x, T, dtype, what):
-        if x.dim() != 3 or x.shape[2] != self.head_dim or x.shape[0] != T or x.dtype != dtype:
+        """Strides of tokens and heads, and the heads, of x [T, heads, head_dim]."""
+        if x.dim() != 3 or x.dtype != dtype:
+            raise ValueError(f"{what} must be {dtype} [{T}, heads, {self.head_dim}], got "
+                             f"{x.dtype} {tuple(x.shape)}")
+        t, n, hd = x.shape
+        if hd != self.head_dim or t != T:
             raise ValueError(f"{what} must be {dtype} [{T}, heads, {self.head_dim}], got "
                              f"{x.dtype} {tuple(x.shape)}")
         on_device(x, what)
-        if x.stride(2) != 1 and self.head_dim > 1:
+        st, sh, se = x.stride()
+        if se != 1 and hd > 1:
             raise ValueError(f"{what}: the elements of a head must be contiguous")
-        return x
+        return st, sh, n
+
+    def _out_side(self, o, x, T, dtype, what):
+        st, sh, n = self._side(o, T, dtype, what)
+        if n != x.shape[1]:
+            raise ValueError(f"{what} must be {tuple(x.shape)}, got {tuple(o.shape)}")
+        if st == 0 and T > 1 or sh == 0 and n > 1:
+            raise ValueError(f"{what} must not repeat its elements")
+        if o.data_ptr() == x.data_ptr() and (st, sh) != x.stride()[:2]:
+            raise ValueError(f"{what} in place must have the strides of its input")
+        return st, sh
 
     def _turn(self, q, k, positions, out, inverse):
-        if q.dim() != 3 or q.dtype not in DTYPES:
+        code = DTYPES.get(q.dtype)
+        if q.dim() != 3 or code is None:
             raise ValueError(f"q must be a bf16, float16 or float32 [T, heads, {self.head_dim}] "
                              f"tensor, got {q.dtype} {tuple(q.shape)}")
         T, dt = q.shape[0], q.dtype
-        self._side(q, T, dt, "q")
-        if k is not None:
-            self._side(k, T, dt, "k")
-        if positions.dtype not in (torch.int32, torch.int64) or tuple(positions.shape) != (T,):
+        q_t, q_h, nq = self._side(q, T, dt, "q")
+        if not nq and T:
+            raise ValueError("q must have at least one head")
+        k_t, k_h, nk = (0, 0, 0) if k is None else self._side(k, T, dt, "k")
+        wide = positions.dtype is torch.int64
+        if not wide and positions.dtype is not torch.int32 or positions.shape != (T,):
             raise ValueError(f"positions must be int32 or int64 [{T}], got {positions.dtype} "
                              f"{tuple(positions.shape)}")
         on_device(positions, "positions")
         on_device(self.turns, "the plan")
         positions = positions.contiguous()
+        hd = self.head_dim
         if out is None:
-            qo = torch.empty(q.shape, device=q.device, dtype=dt)
-            ko = None if k is None else torch.empty(k.shape, device=q.device, dtype=dt)
+            qo, qo_t, qo_h = torch.empty((T, nq, hd), device=q.device, dtype=dt), nq * hd, hd
+            ko, ko_t, ko_h = None, nk * hd, hd
+            if k is not None:
+                ko = torch.empty((T, nk, hd), device=q.device, dtype=dt)
         else:
             qo, ko = out
-            if (ko is None) != (k is None):
+            if qo is None or (ko is None) != (k is None):
                 raise ValueError("out must be (q_out, k_out), k_out None without k")
-            for o, x, what in ((qo, q, "q_out"), (ko, k, "k_out")):
-                if x is None:
-                    continue
-                self._side(o, T, dt, what)
-                if o.shape != x.shape:
-                    raise ValueError(f"{what} must be {tuple(x.shape)}, got {tuple(o.shape)}")
-                if any(o.stride(i) == 0 and o.shape[i] > 1 for i in (0, 1)):
-                    raise ValueError(f"{what} must not repeat its elements")
-                if o.data_ptr() == x.data_ptr() and o.stride() != x.stride():
-                    raise ValueError(f"{what} in place must have the strides of its input")
-        if T and q.shape[1] == 0:
-            raise ValueError("q must have at least one head")
+            qo_t, qo_h = self._out_side(qo, q, T, dt, "q_out")
+            ko_t, ko_h = (0, 0) if k is None else self._out_side(ko, k, T, dt, "k_out")
         if T:
-            nk = 0 if k is None else k.shape[1]
-            k_, ko_ = (k, ko) if nk else (q, qo)
-            _lib.call("gsq_rope", q.data_ptr(), q.stride(0), q.stride(1), q.shape[1],
-                      k_.data_ptr(), k_.stride(0), k_.stride(1), nk, T, self.head_dim,
-                      self.rotary_dim, int(self.layout == "interleaved"), DTYPES[dt],
-                      positions.data_ptr(), int(positions.dtype == torch.int64),
-                      self.turns.data_ptr(), self.factor, int(inverse), qo.data_ptr(),
-                      qo.stride(0), qo.stride(1), ko_.data_ptr(), ko_.stride(0), ko_.stride(1),
-                      _lib.stream_ptr())
+            _lib.call("gsq_rope", q.data_ptr(), q_t, q_h, nq, k.data_ptr() if nk else None, k_t,
+                      k_h, nk, T, hd, self.rotary_dim, int(self.layout == "interleaved"), code,
+                      positions.data_ptr(), int(wide), self.turns.data_ptr(), self.factor,
+                      int(inverse), qo.data_ptr(), qo_t, qo_h, ko.data_ptr() if nk else None, ko_t,
+                      ko_h, _lib.stream_ptr())
         return qo, ko
 
     def __call__(self, q, k, positions, out=None):

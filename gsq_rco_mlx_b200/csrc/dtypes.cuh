@@ -61,6 +61,63 @@ __device__ __forceinline__ void store8(T* __restrict__ row, int c, int cols, con
   }
 }
 
+// Pairs of float32 in one instruction (each half rounds as the scalar operation does): the fused
+// multiply-add of a pair issues as fast as a single one.
+struct F2 {
+  float x, y;
+};
+__device__ __forceinline__ uint64_t f2_bits(F2 v) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(v.x), "f"(v.y));
+  return r;
+}
+__device__ __forceinline__ F2 f2_of(uint64_t r) {
+  F2 v;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(r));
+  return v;
+}
+__device__ __forceinline__ F2 f2_fma(F2 a, F2 b, F2 c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(f2_bits(a)), "l"(f2_bits(b)), "l"(f2_bits(c)));
+  return f2_of(r);
+}
+__device__ __forceinline__ F2 f2_mul(F2 a, F2 b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(f2_bits(a)), "l"(f2_bits(b)));
+  return f2_of(r);
+}
+__device__ __forceinline__ F2 f2_add(F2 a, F2 b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(f2_bits(a)), "l"(f2_bits(b)));
+  return f2_of(r);
+}
+__device__ __forceinline__ F2 f2_same(float v) { return {v, v}; }
+
+// Two neighbouring 16-bit values (one word) as a pair, and back.
+template <typename T>
+__device__ __forceinline__ F2 f2_unpack(uint32_t w);
+template <>
+__device__ __forceinline__ F2 f2_unpack<__nv_bfloat16>(uint32_t w) {
+  return {__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)};
+}
+template <>
+__device__ __forceinline__ F2 f2_unpack<__half>(uint32_t w) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+  return {f.x, f.y};
+}
+template <typename T>
+__device__ __forceinline__ uint32_t f2_pack(F2 v);
+template <>
+__device__ __forceinline__ uint32_t f2_pack<__nv_bfloat16>(F2 v) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(v.x, v.y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t f2_pack<__half>(F2 v) {
+  const __half2 h = __floats2half2_rn(v.x, v.y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
 // maximum that keeps NaN (fmaxf drops it)
 __device__ __forceinline__ float max_nan(float a, float b) {
   float d;

@@ -9,12 +9,18 @@
 //   u = X b,  d = D + r2 (u - h' r2^2 mean(u h')),  dh = d
 //   m = alpha g d,  v = m a,  dy = r1 (v - y r1^2 mean(v y))
 //   dw_post = sum m y r1,  dw_pre = sum X h' r2,  dg = sum alpha d n      (over rows, float32)
+// With p = d y r1 the three parameter sums come from one: S = sum p over the rows of one gate row,
+//   dg = alpha a S,  dw_post = sum over gate rows of alpha g S.
 // Both directions are one pass over their rows, held in registers by a team of threads (a warp
-// up to 1024 columns, a block above), so they are bound by the bytes of the rows.
+// up to 256 columns, a block above: eight columns a thread), so they are bound by the bytes of
+// the rows. Rows that start on 16 bytes are read as vectors of eight columns; others column by
+// column with the columns dealt round the team, which keeps every access of a warp one segment
+// (eight neighbouring columns a thread would touch each sector eight times).
 // The column sums of the backward pass: each team adds its rows in registers and writes one
 // partial row; a second kernel adds the partials in a fixed order (no atomics: the same inputs
 // give the same bits).
 #include "dtypes.cuh"
+#include "tc_common.cuh"
 
 namespace gsq {
 namespace norm {
@@ -35,12 +41,12 @@ struct Fwd {
   float* stats;  // [2][T] r1, r2
 };
 
+constexpr int kArrays = 4;  // y, h, dx, dh2
 struct Bwd {
-  const void *h, *y, *w_post, *w_pre, *gate;
-  int64_t ld_h, ld_y;
+  const void* in[kArrays];  // dx NULL without w_pre, dh2 NULL for zeros
+  int64_t ld[kArrays];
+  const void *w_post, *w_pre, *gate;
   const float* stats;
-  const void *dh2, *dx;  // dh2 may be NULL (zeros), dx NULL without w_pre
-  int64_t ld_dh2, ld_dx;
   int T, H, per_gate;
   float alpha, offset;
   void *dh, *dy;
@@ -48,92 +54,150 @@ struct Bwd {
   int groups, splits;  // gate rows, and the parts each one's rows are cut into
   float* part_w;       // [teams][2][H] partials of dw_post, dw_pre
   float* part_g;       // [groups * splits][H] partials of dgate (dgate itself if splits == 1)
+  int slots;           // rows in flight per team
+  uint32_t row_bytes;  // shared memory of one array's row
+  int* err;
 };
 
-// Sum over the TPR threads of a row's team. Teams of more than a warp are a whole block, whose
-// two staging rows alternate so that one barrier per sum is enough.
-template <int TPR>
+// Sum over a row's team: a warp, or a block of up to 32 warps, whose two staging rows alternate
+// so that one barrier per sum is enough. `red` is zero behind the block's warps.
+template <bool WARP>
 __device__ __forceinline__ float team_sum(float v, float (*red)[32], int& turn) {
   v = warp_sum(v);
-  if (TPR == 32) return v;
-  constexpr int NW = TPR / 32;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (WARP) return v;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = blockDim.x >> 5;
   float* r = red[turn & 1];
   ++turn;
   if (lane == 0) r[warp] = v;
   __syncthreads();
-  float s = lane < NW ? r[lane] : 0.f;
-  return warp_sum(s);
+  if (nw <= 8) {
+    const float4 a = *reinterpret_cast<const float4*>(r), b = *reinterpret_cast<const float4*>(r + 4);
+    return ((a.x + a.y) + (a.z + a.w)) + ((b.x + b.y) + (b.z + b.w));
+  }
+  return warp_sum(r[lane]);
 }
 
-template <typename T, bool VEC, int TPR, int NC, bool FP8>
-__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) fwd_kernel(const __grid_constant__ Fwd p) {
-  __shared__ float red[2][32];
+// Column of value j of chunk c: eight neighbours (VEC), or dealt round the team.
+template <bool VEC>
+__device__ __forceinline__ int column(int c, int j, int t, int tpr) {
+  return VEC ? (c * tpr + t) * 8 + j : (c * 8 + j) * tpr + t;
+}
+
+// The thread's eight values of chunk c of a row; columns from H on are zero.
+template <typename T, bool VEC>
+__device__ __forceinline__ void get8(const T* __restrict__ row, int c, int t, int tpr, int H,
+                                     float v[8]) {
+  if (VEC) {
+    load8<T, true>(row, (c * tpr + t) * 8, H, v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int col = column<false>(c, j, t, tpr);
+      v[j] = col < H ? to_f32(row[col]) : 0.f;
+    }
+  }
+}
+
+template <typename T, bool VEC>
+__device__ __forceinline__ void put8(T* __restrict__ row, int c, int t, int tpr, int H,
+                                     const float v[8]) {
+  if (VEC) {
+    store8<T, true>(row, (c * tpr + t) * 8, H, v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int col = column<false>(c, j, t, tpr);
+      if (col < H) row[col] = from_f32<T>(v[j]);
+    }
+  }
+}
+
+__device__ __forceinline__ float sumsq8(const float v[8]) {
+  const float a = fmaf(v[1], v[1], v[0] * v[0]), b = fmaf(v[3], v[3], v[2] * v[2]);
+  const float c = fmaf(v[5], v[5], v[4] * v[4]), d = fmaf(v[7], v[7], v[6] * v[6]);
+  return (a + b) + (c + d);
+}
+
+// One row per team (no loop over rows: enough blocks are resident to hide the loads). The
+// statistics are 1 / sqrt rounded once, so that x rounds no worse than its definition.
+template <typename T, bool VEC, bool WARP, int NC, bool FP8>
+__global__ void __launch_bounds__(WARP ? 256 : 1024, 1) fwd_kernel(const __grid_constant__ Fwd p) {
+  __shared__ __align__(16) float red[2][32];
+  __shared__ uint32_t amax_s[FP8 && !VEC ? 256 : 1];
   int turn = 0;
-  const int t = TPR == 32 ? threadIdx.x & 31 : threadIdx.x;
-  const int teams = TPR == 32 ? 8 : 1;
-  const int row = blockIdx.x * teams + (TPR == 32 ? threadIdx.x >> 5 : 0);
+  const int t = WARP ? threadIdx.x & 31 : threadIdx.x, tpr = WARP ? 32 : blockDim.x;
+  const int row = WARP ? blockIdx.x * 8 + (threadIdx.x >> 5) : blockIdx.x;
+  if (!WARP) {
+    if (threadIdx.x < 64) red[threadIdx.x >> 5][threadIdx.x & 31] = 0.f;
+    if (FP8 && !VEC)
+      for (int i = threadIdx.x; i < 256; i += blockDim.x) amax_s[i] = 0u;
+    __syncthreads();
+  } else if (FP8 && !VEC) {
+    for (int i = threadIdx.x; i < 256; i += blockDim.x) amax_s[i] = 0u;
+    __syncthreads();
+  }
   if (row >= p.T) return;  // (a whole warp, or a whole block)
-  const float inv_H = 1.f / (float)p.H;
   const T* hr = reinterpret_cast<const T*>(p.h) + (int64_t)row * p.ld_h;
   const T* yr = reinterpret_cast<const T*>(p.y) + (int64_t)row * p.ld_y;
   float y[NC][8], h[NC][8];
 #pragma unroll
-  for (int c = 0; c < NC; ++c) load8<T, VEC>(yr, (c * TPR + t) * 8, p.H, y[c]);
+  for (int c = 0; c < NC; ++c) get8<T, VEC>(yr, c, t, tpr, p.H, y[c]);
 #pragma unroll
-  for (int c = 0; c < NC; ++c) load8<T, VEC>(hr, (c * TPR + t) * 8, p.H, h[c]);
+  for (int c = 0; c < NC; ++c) get8<T, VEC>(hr, c, t, tpr, p.H, h[c]);
+  const T* gr = p.gate ? reinterpret_cast<const T*>(p.gate) + (int64_t)(row / p.per_gate) * p.H
+                       : nullptr;
+  const float H = (float)p.H;
   float r1 = 1.f;
   if (p.w_post) {
     float s = 0.f;
 #pragma unroll
-    for (int c = 0; c < NC; ++c)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) s = fmaf(y[c][j], y[c][j], s);
-    r1 = rsqrtf(team_sum<TPR>(s, red, turn) * inv_H + p.eps);
+    for (int c = 0; c < NC; ++c) s += sumsq8(y[c]);
+    r1 = __frsqrt_rn(__fdiv_rn(team_sum<WARP>(s, red, turn), H) + p.eps);
   }
-  const T* gr = p.gate ? reinterpret_cast<const T*>(p.gate) + (int64_t)(row / p.per_gate) * p.H
-                       : nullptr;
   float s = 0.f;
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
-    const int col = (c * TPR + t) * 8;
     if (p.w_post) {
       float a[8];
-      load8<T, VEC>(reinterpret_cast<const T*>(p.w_post), col, p.H, a);
+      get8<T, VEC>(reinterpret_cast<const T*>(p.w_post), c, t, tpr, p.H, a);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) y[c][j] *= r1 * (a[j] + p.offset);
+      for (int j = 0; j < 8; ++j) y[c][j] = (y[c][j] * r1) * (a[j] + p.offset);
     }
     if (gr) {
       float g[8];
-      load8<T, VEC>(gr, col, p.H, g);
+      get8<T, VEC>(gr, c, t, tpr, p.H, g);
 #pragma unroll
       for (int j = 0; j < 8; ++j) y[c][j] *= g[j];
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      h[c][j] = fmaf(p.alpha, y[c][j], h[c][j]);
-      s = fmaf(h[c][j], h[c][j], s);
+      // (columns from H on stay zero whatever the weights' pad would give)
+      h[c][j] = column<VEC>(c, j, t, tpr) < p.H ? fmaf(p.alpha, y[c][j], h[c][j]) : 0.f;
     }
+    s += sumsq8(h[c]);
     if (p.h_out)
-      store8<T, VEC>(reinterpret_cast<T*>(p.h_out) + (int64_t)row * p.ld_ho, col, p.H, h[c]);
+      put8<T, VEC>(reinterpret_cast<T*>(p.h_out) + (int64_t)row * p.ld_ho, c, t, tpr, p.H, h[c]);
   }
   float r2 = 1.f;
   if (p.w_pre) {
-    r2 = rsqrtf(team_sum<TPR>(s, red, turn) * inv_H + p.eps);
+    r2 = __frsqrt_rn(__fdiv_rn(team_sum<WARP>(s, red, turn), H) + p.eps);
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      const int col = (c * TPR + t) * 8;
       float b[8];
-      load8<T, VEC>(reinterpret_cast<const T*>(p.w_pre), col, p.H, b);
+      get8<T, VEC>(reinterpret_cast<const T*>(p.w_pre), c, t, tpr, p.H, b);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) h[c][j] *= r2 * (b[j] + p.offset);
-      if (!FP8) {
-        store8<T, VEC>(reinterpret_cast<T*>(p.x) + (int64_t)row * p.ld_x, col, p.H, h[c]);
-      } else {
-        // a 128-column block is the eight columns of each of 16 neighbouring lanes
+      for (int j = 0; j < 8; ++j) {
+        h[c][j] = (h[c][j] * r2) * (b[j] + p.offset);
+        if (FP8 && column<VEC>(c, j, t, tpr) >= p.H) h[c][j] = 0.f;
+      }
+      if (!FP8)
+        put8<T, VEC>(reinterpret_cast<T*>(p.x) + (int64_t)row * p.ld_x, c, t, tpr, p.H, h[c]);
+    }
+    if (FP8 && VEC) {
+      // a 128-column block is the eight columns of each of 16 neighbouring lanes
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (col + j >= p.H) h[c][j] = 0.f;
+      for (int c = 0; c < NC; ++c) {
+        const int col = (c * tpr + t) * 8;
         float m = amax8(h[c]);
 #pragma unroll
         for (int o = 8; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -146,6 +210,35 @@ __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) fwd_kernel(const __grid
         }
       }
     }
+    if (FP8 && !VEC) {
+      // a warp's 32 columns of one j lie in one block: a warp maximum, then one shared-memory
+      // maximum per warp and block (magnitudes compare as their bits; NaN is above infinity)
+      uint32_t* am = amax_s + (WARP ? (threadIdx.x >> 5) * 2 : 0);
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(h[c][j])));
+          const int col = column<false>(c, j, t, tpr);
+          if ((t & 31) == 0 && col < p.H) atomicMax(am + col / kFp8Block, m);
+        }
+      if (WARP) __syncwarp();
+      else __syncthreads();
+      for (int b = t; b < (p.H + kFp8Block - 1) / kFp8Block; b += tpr)
+        p.scales[(int64_t)b * p.ld_s + row] =
+            __fdiv_rn(max_nan(__uint_as_float(am[b]), kFp8AmaxMin), kFp8Max);
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int col = column<false>(c, j, t, tpr);
+          if (col < p.H) {
+            const float m = max_nan(__uint_as_float(am[col / kFp8Block]), kFp8AmaxMin);
+            p.codes[(int64_t)row * p.ld_c + col] =
+                (uint8_t)cvt4_e4m3(__fmul_rn(h[c][j], __fdiv_rn(kFp8Max, m)), 0.f, 0.f, 0.f);
+          }
+        }
+    }
   }
   if (t == 0) {
     p.stats[row] = r1;
@@ -153,136 +246,363 @@ __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) fwd_kernel(const __grid
   }
 }
 
-template <typename T, bool VEC, int TPR, int NC>
-__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) bwd_kernel(const __grid_constant__ Bwd p) {
-  __shared__ float red[2][32];
-  int turn = 0;
-  const int t = TPR == 32 ? threadIdx.x & 31 : threadIdx.x;
-  const int per_block = TPR == 32 ? 8 : 1;
-  const int team = blockIdx.x * per_block + (TPR == 32 ? threadIdx.x >> 5 : 0);
-  const int teams = gridDim.x * per_block;
-  const float inv_H = 1.f / (float)p.H;
-  float sw_post[NC][8], sw_pre[NC][8];
-#pragma unroll
-  for (int c = 0; c < NC; ++c)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) sw_post[c][j] = sw_pre[c][j] = 0.f;
-  for (int64_t item = team; item < (int64_t)p.groups * p.splits; item += teams) {
-    const int g = (int)(item / p.splits), part = (int)(item - (int64_t)g * p.splits);
-    const int lo = (int)((int64_t)p.per_gate * part / p.splits) + g * p.per_gate;
-    const int hi = (int)((int64_t)p.per_gate * (part + 1) / p.splits) + g * p.per_gate;
-    const T* gr = p.gate ? reinterpret_cast<const T*>(p.gate) + (int64_t)g * p.H : nullptr;
-    float sg[NC][8];
-#pragma unroll
-    for (int c = 0; c < NC; ++c)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) sg[c][j] = 0.f;
-    for (int row = lo; row < hi; ++row) {
-      float y[NC][8], h[NC][8], u[NC][8], d[NC][8];
-      const T* yr = reinterpret_cast<const T*>(p.y) + (int64_t)row * p.ld_y;
-      const T* hr = reinterpret_cast<const T*>(p.h) + (int64_t)row * p.ld_h;
-#pragma unroll
-      for (int c = 0; c < NC; ++c) load8<T, VEC>(yr, (c * TPR + t) * 8, p.H, y[c]);
-#pragma unroll
-      for (int c = 0; c < NC; ++c) load8<T, VEC>(hr, (c * TPR + t) * 8, p.H, h[c]);
-#pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        if (p.dh2)
-          load8<T, VEC>(reinterpret_cast<const T*>(p.dh2) + (int64_t)row * p.ld_dh2,
-                        (c * TPR + t) * 8, p.H, d[c]);
-        else
-#pragma unroll
-          for (int j = 0; j < 8; ++j) d[c][j] = 0.f;
-        if (p.w_pre)
-          load8<T, VEC>(reinterpret_cast<const T*>(p.dx) + (int64_t)row * p.ld_dx,
-                        (c * TPR + t) * 8, p.H, u[c]);
-      }
-      const float r1 = p.w_post ? p.stats[row] : 1.f, r2 = p.w_pre ? p.stats[p.T + row] : 1.f;
-      float s = 0.f;
-#pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        const int col = (c * TPR + t) * 8;
-        float a[8], gv[8];
-        if (p.w_post) load8<T, VEC>(reinterpret_cast<const T*>(p.w_post), col, p.H, a);
-        if (gr) load8<T, VEC>(gr, col, p.H, gv);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          float n = y[c][j] * r1;
-          if (p.w_post) n *= a[j] + p.offset;
-          if (gr) n *= gv[j];
-          h[c][j] = fmaf(p.alpha, n, h[c][j]) * r2;  // h' r2
-        }
-        if (p.w_pre) {
-          float b[8];
-          load8<T, VEC>(reinterpret_cast<const T*>(p.w_pre), col, p.H, b);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            sw_pre[c][j] = fmaf(u[c][j], h[c][j], sw_pre[c][j]);
-            u[c][j] *= b[j] + p.offset;
-            s = fmaf(u[c][j], h[c][j], s);
-          }
-        }
-      }
-      if (p.w_pre) {
-        const float mu = team_sum<TPR>(s, red, turn) * inv_H;
-#pragma unroll
-        for (int c = 0; c < NC; ++c)
-#pragma unroll
-          for (int j = 0; j < 8; ++j) d[c][j] = fmaf(r2, u[c][j] - h[c][j] * mu, d[c][j]);
-      }
-      float s2 = 0.f;
-#pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        const int col = (c * TPR + t) * 8;
-        store8<T, VEC>(reinterpret_cast<T*>(p.dh) + (int64_t)row * p.ld_dh, col, p.H, d[c]);
-        float a[8], gv[8];
-        if (p.w_post) load8<T, VEC>(reinterpret_cast<const T*>(p.w_post), col, p.H, a);
-        if (gr) load8<T, VEC>(gr, col, p.H, gv);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float yn = y[c][j] * r1, ad = p.alpha * d[c][j];
-          const float aj = p.w_post ? a[j] + p.offset : 1.f;
-          sg[c][j] = fmaf(ad, yn * aj, sg[c][j]);
-          const float m = gr ? ad * gv[j] : ad;
-          sw_post[c][j] = fmaf(m, yn, sw_post[c][j]);
-          u[c][j] = m * aj;   // v
-          y[c][j] = yn;
-          s2 = fmaf(u[c][j], yn, s2);
-        }
-      }
-      const float mv = p.w_post ? team_sum<TPR>(s2, red, turn) * inv_H : 0.f;
-#pragma unroll
-      for (int c = 0; c < NC; ++c) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) u[c][j] = r1 * (u[c][j] - y[c][j] * mv);
-        store8<T, VEC>(reinterpret_cast<T*>(p.dy) + (int64_t)row * p.ld_dy, (c * TPR + t) * 8, p.H,
-                       u[c]);
-      }
-    }
-    if (p.part_g) {
-#pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        const int col = (c * TPR + t) * 8;
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (col + j < p.H) p.part_g[item * p.H + col + j] = sg[c][j];
-      }
-    }
+// The rows of a team, in order: items (a part of a gate row's rows) team, team + teams, ...
+struct Rows {
+  int item, row, hi;   // the item, and what is left of its rows; item -1: none
+  __device__ __forceinline__ void open(const Bwd& p, int64_t i) {
+    item = -1;
+    if (i >= (int64_t)p.groups * p.splits) return;
+    item = (int)i;
+    const int g = item / p.splits, part = item - g * p.splits;
+    row = (int)((int64_t)p.per_gate * part / p.splits) + g * p.per_gate;
+    hi = (int)((int64_t)p.per_gate * (part + 1) / p.splits) + g * p.per_gate;
   }
+  __device__ __forceinline__ void next(const Bwd& p, int teams) {
+    if (++row == hi) open(p, (int64_t)item + teams);
+  }
+};
+
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes,
+                                          uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+          tc::smem_u32(dst)),
+      "l"(src), "r"(bytes), "r"(tc::smem_u32(bar))
+      : "memory");
+}
+
+// Copies a row of every array into a slot: from the 16-byte boundary at or below its start to
+// that at or above its end (the few bytes around a row that does not start or end there lie in
+// the same 16 bytes as the row's own).
+template <typename T>
+__device__ __forceinline__ void fetch_row(const Bwd& p, int row, uint8_t* slot, uint64_t* bar) {
+  uint32_t total = 0, bytes[kArrays];
+  const uint8_t* from[kArrays];
 #pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    const int col = (c * TPR + t) * 8;
+  for (int i = 0; i < kArrays; ++i) {
+    bytes[i] = 0;
+    if (!p.in[i]) continue;
+    const uintptr_t s = (uintptr_t)(reinterpret_cast<const T*>(p.in[i]) + (int64_t)row * p.ld[i]);
+    const uintptr_t lo = s & ~(uintptr_t)15, hi = (s + p.H * sizeof(T) + 15) & ~(uintptr_t)15;
+    from[i] = reinterpret_cast<const uint8_t*>(lo);
+    bytes[i] = (uint32_t)(hi - lo);
+    total += bytes[i];
+  }
+  tc::mbar_arrive_expect_tx(bar, total);
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (col + j < p.H) {
-        p.part_w[((int64_t)team * 2) * p.H + col + j] = sw_post[c][j];
-        p.part_w[((int64_t)team * 2 + 1) * p.H + col + j] = sw_pre[c][j];
-      }
+  for (int i = 0; i < kArrays; ++i)
+    if (bytes[i]) bulk_load(slot + i * p.row_bytes, from[i], bytes[i], bar);
+}
+
+constexpr int kMaxSlots = 4;
+
+// The backward pass deals columns in fours: column j < 4 of a thread's chunk q is one of four
+// neighbours (VEC: chunks go round the team), or goes round the team by itself.
+template <bool VEC>
+__device__ __forceinline__ int column4(int q, int j, int t, int tpr) {
+  return VEC ? (q * tpr + t) * 4 + j : (q * 4 + j) * tpr + t;
+}
+
+template <typename T>
+__device__ __forceinline__ float lds1(uint32_t a) {
+  if constexpr (sizeof(T) == 2) {
+    uint16_t v;
+    asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"(a));
+    return to_f32(*reinterpret_cast<const T*>(&v));
+  } else {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a));
+    return v;
   }
 }
 
+// Chunk q of a row, as two pairs: from shared memory (byte address `row`) or from memory;
+// columns from H on read as zero.
+template <typename T, bool VEC>
+__device__ __forceinline__ void sget4(uint32_t row, int q, int t, int tpr, int H, F2 v[2]) {
+  const int c0 = column4<VEC>(q, 0, t, tpr);
+  if (VEC && c0 + 4 <= H) {
+    if constexpr (sizeof(T) == 2) {
+      uint32_t x, y;
+      asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(x), "=r"(y) : "r"(row + c0 * 2));
+      v[0] = f2_unpack<T>(x);
+      v[1] = f2_unpack<T>(y);
+    } else {
+      asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                   : "=f"(v[0].x), "=f"(v[0].y), "=f"(v[1].x), "=f"(v[1].y)
+                   : "r"(row + c0 * 4));
+    }
+  } else {
+    const int step = VEC ? 1 : tpr;
+    uint32_t a = row + c0 * sizeof(T);
+    float f[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      f[j] = c0 + j * step < H ? lds1<T>(a) : 0.f;
+      a += step * sizeof(T);
+    }
+    v[0] = {f[0], f[1]};
+    v[1] = {f[2], f[3]};
+  }
+}
+
+template <typename T, bool VEC>
+__device__ __forceinline__ void get4(const T* __restrict__ row, int q, int t, int tpr, int H,
+                                     F2 v[2]) {
+  const int c0 = column4<VEC>(q, 0, t, tpr), step = VEC ? 1 : tpr;
+  float f[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) f[j] = c0 + j * step < H ? to_f32(row[c0 + j * step]) : 0.f;
+  v[0] = {f[0], f[1]};
+  v[1] = {f[2], f[3]};
+}
+
+template <typename T, bool VEC>
+__device__ __forceinline__ void put4(T* __restrict__ row, int q, int t, int tpr, int H,
+                                     const F2 v[2]) {
+  const int c0 = column4<VEC>(q, 0, t, tpr), step = VEC ? 1 : tpr;
+  if (VEC && c0 + 4 <= H) {
+    if constexpr (sizeof(T) == 2)
+      *reinterpret_cast<uint2*>(row + c0) = make_uint2(f2_pack<T>(v[0]), f2_pack<T>(v[1]));
+    else
+      *reinterpret_cast<float4*>(row + c0) = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+  } else {
+    const float f[4] = {v[0].x, v[0].y, v[1].x, v[1].y};
+    T* o = row + c0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (c0 + j * step < H) *o = from_f32<T>(f[j]);
+      o += step;
+    }
+  }
+}
+
+__device__ __forceinline__ float f2_dot(const F2 a[2], const F2 b[2]) {
+  const F2 s = f2_fma(a[1], b[1], f2_mul(a[0], b[0]));
+  return s.x + s.y;
+}
+__device__ __forceinline__ float f2_at(const F2 v[2], int j) {
+  return j & 1 ? v[j >> 1].y : v[j >> 1].x;
+}
+
+// Where a thread's alpha a g and b are kept: in registers up to 512 threads a team, in shared
+// memory up to 1024, and read anew for every row where a row does not fit shared memory.
+enum Weights { W_REG, W_SMEM, W_MEM };
+
+// Persistent teams, 4 Q columns a thread. Unless W_MEM, a team's rows arrive in shared memory by
+// bulk copies, `slots` rows ahead, so that the loads run on through the two sums of a row, and
+// dh2 is read only after the first of them: 6 of 8 registers a column.
+template <typename T, bool VEC, bool WARP, int Q, int W, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1) bwd_kernel(const __grid_constant__ Bwd p) {
+  constexpr bool STAGED = W != W_MEM;
+  constexpr int QW = W == W_REG ? Q : 1;
+  extern __shared__ __align__(16) uint8_t dyn[];
+  __shared__ __align__(16) float red[2][32];
+  __shared__ __align__(8) uint64_t bars[WARP ? 8 : 1][kMaxSlots];
+  __shared__ Rows ahead_s[WARP ? 8 : 1];   // the next row to fetch (the first thread's)
+  int turn = 0;
+  const int w = WARP ? threadIdx.x >> 5 : 0;
+  const int t = WARP ? threadIdx.x & 31 : threadIdx.x, tpr = WARP ? 32 : blockDim.x;
+  const int team = WARP ? blockIdx.x * 8 + w : blockIdx.x;
+  const int teams = WARP ? gridDim.x * 8 : gridDim.x;
+  const float inv_H = 1.f / (float)p.H;
+  uint64_t* bar = bars[w];
+  const uint32_t slot_bytes = kArrays * p.row_bytes;
+  uint8_t* mine = dyn + (size_t)w * p.slots * slot_bytes;
+  const uint32_t mine_a = tc::smem_u32(mine);
+  float* ag_s = reinterpret_cast<float*>(dyn + (size_t)(WARP ? 8 : 1) * p.slots * slot_bytes);
+  const int ldw = (p.H + 3) / 4 * 4;
+  const uint32_t ag_a = tc::smem_u32(ag_s), b_a = ag_a + ldw * 4;
+  if (!WARP && threadIdx.x < 64) red[threadIdx.x >> 5][threadIdx.x & 31] = 0.f;
+  if (STAGED && t == 0) {
+    for (int i = 0; i < p.slots; ++i) tc::mbar_init(&bar[i], 1);
+    tc::fence_barrier_init();
+  }
+  __syncthreads();
+  Rows it;
+  it.open(p, team);
+  if (STAGED && t == 0) {
+    Rows ahead = it;
+    for (int i = 0; i < p.slots && ahead.item >= 0; ++i, ahead.next(p, teams))
+      fetch_row<T>(p, ahead.row, mine + i * slot_bytes, &bar[i]);
+    ahead_s[w] = ahead;
+  }
+  const T* wpost = reinterpret_cast<const T*>(p.w_post);
+  const T* wpre = reinterpret_cast<const T*>(p.w_pre);
+  auto a_at = [&](int q, F2 v[2]) {
+    if (wpost) get4<T, VEC>(wpost, q, t, tpr, p.H, v);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) v[j] = wpost ? f2_add(v[j], f2_same(p.offset)) : f2_same(1.f);
+  };
+  auto g_at = [&](int g, int q, F2 v[2]) {   // alpha g
+    if (p.gate) get4<T, VEC>(reinterpret_cast<const T*>(p.gate) + (int64_t)g * p.H, q, t, tpr, p.H, v);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) v[j] = p.gate ? f2_mul(v[j], f2_same(p.alpha)) : f2_same(p.alpha);
+  };
+  auto ag_of = [&](int g, int q, F2 v[2]) {   // alpha a g
+    F2 gv[2];
+    a_at(q, v);
+    g_at(g, q, gv);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) v[j] = f2_mul(v[j], gv[j]);
+  };
+  auto b_of = [&](int q, F2 v[2]) {
+    if (wpre) get4<T, VEC>(wpre, q, t, tpr, p.H, v);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) v[j] = wpre ? f2_add(v[j], f2_same(p.offset)) : f2_same(0.f);
+  };
+  F2 S[Q][2], sw[Q][2];     // sums of d y r1 and of dx h' r2
+  F2 ag[QW][2], bw[QW][2];
+#pragma unroll
+  for (int q = 0; q < Q; ++q)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) S[q][j] = sw[q][j] = f2_same(0.f);
+  int held = -1;   // the item whose alpha a g is held
+  bool alive = true, opened = false;
+  int slot = 0;
+  uint32_t phase = 0;
+  for (; it.item >= 0; it.next(p, teams)) {
+    const int row = it.row;
+    if (STAGED && it.item != held) {
+      const int g = it.item / p.splits;
+#pragma unroll
+      for (int q = 0; q < Q; ++q) {
+        F2 v[2], u[2];
+        ag_of(g, q, v);
+        if (held < 0) b_of(q, u);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int col = column4<VEC>(q, j, t, tpr);
+          if (W == W_REG) {
+            if ((j & 1) == 0) {
+              ag[W == W_REG ? q : 0][j >> 1] = v[j >> 1];
+              if (held < 0) bw[W == W_REG ? q : 0][j >> 1] = u[j >> 1];
+            }
+          } else if (col < p.H) {   // (each thread reads only what it wrote)
+            ag_s[col] = f2_at(v, j);
+            if (held < 0) ag_s[ldw + col] = f2_at(u, j);
+          }
+        }
+      }
+      held = it.item;
+    }
+    const float r1 = wpost ? p.stats[row] : 1.f, r2 = wpre ? p.stats[p.T + row] : 1.f;
+    // (after a timeout the rows run on unread, so that the block's barriers keep their count)
+    if (STAGED && alive) alive = tc::mbar_wait(&bar[slot], phase, p.err, 6);
+    auto read = [&](int i, int q, F2 v[2]) {
+      const T* src = reinterpret_cast<const T*>(p.in[i]) + (int64_t)row * p.ld[i];
+      if (STAGED)
+        sget4<T, VEC>(mine_a + slot * slot_bytes + i * p.row_bytes + ((uint32_t)(uintptr_t)src & 15u),
+                      q, t, tpr, p.H, v);
+      else
+        get4<T, VEC>(src, q, t, tpr, p.H, v);
+    };
+    F2 y[Q][2], h[Q][2], u[Q][2];
+    float s = 0.f;
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      F2 wv[2];
+      read(0, q, y[q]);
+      read(1, q, h[q]);
+      if (W == W_SMEM) sget4<float, VEC>(ag_a, q, t, tpr, p.H, wv);
+      if (W == W_MEM) ag_of(it.item / p.splits, q, wv);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        y[q][j] = f2_mul(y[q][j], f2_same(r1));
+        h[q][j] = f2_mul(f2_fma(W == W_REG ? ag[W == W_REG ? q : 0][j] : wv[j], y[q][j], h[q][j]),
+                         f2_same(r2));   // h' r2
+      }
+      if (wpre) {
+        read(2, q, u[q]);
+        if (W == W_SMEM) sget4<float, VEC>(b_a, q, t, tpr, p.H, wv);
+        if (W == W_MEM) b_of(q, wv);
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        if (!wpre) u[q][j] = f2_same(0.f);
+        sw[q][j] = f2_fma(u[q][j], h[q][j], sw[q][j]);
+        if (wpre) u[q][j] = f2_mul(u[q][j], W == W_REG ? bw[W == W_REG ? q : 0][j] : wv[j]);
+      }
+      s += f2_dot(u[q], h[q]);
+    }
+    const float mu = team_sum<WARP>(s, red, turn) * inv_H;
+    s = 0.f;
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      F2 wv[2], d[2], e[2];
+      if (p.in[3]) read(3, q, d);
+      if (W == W_SMEM) sget4<float, VEC>(ag_a, q, t, tpr, p.H, wv);
+      if (W == W_MEM) ag_of(it.item / p.splits, q, wv);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        if (!p.in[3]) d[j] = f2_same(0.f);
+        if (wpre) d[j] = f2_fma(f2_same(r2), f2_fma(f2_same(-mu), h[q][j], u[q][j]), d[j]);
+        e[j] = f2_mul(d[j], y[q][j]);
+        S[q][j] = f2_add(S[q][j], e[j]);
+        u[q][j] = f2_mul(W == W_REG ? ag[W == W_REG ? q : 0][j] : wv[j], d[j]);   // v
+      }
+      s += f2_dot(W == W_REG ? ag[W == W_REG ? q : 0] : wv, e);
+      put4<T, VEC>(reinterpret_cast<T*>(p.dh) + (int64_t)row * p.ld_dh, q, t, tpr, p.H, d);
+    }
+    float mv = team_sum<WARP>(s, red, turn) * inv_H;
+    if (!wpost) mv = 0.f;
+    // every thread has read the slot (the sum's barrier; a warp's shuffles): the next row may land
+    if (STAGED && t == 0 && alive && ahead_s[w].item >= 0) {
+      fetch_row<T>(p, ahead_s[w].row, mine + slot * slot_bytes, &bar[slot]);
+      ahead_s[w].next(p, teams);
+    }
+    if (++slot == p.slots) {
+      slot = 0;
+      phase ^= 1;
+    }
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        u[q][j] = f2_mul(f2_same(r1), f2_fma(f2_same(-mv), y[q][j], u[q][j]));
+      put4<T, VEC>(reinterpret_cast<T*>(p.dy) + (int64_t)row * p.ld_dy, q, t, tpr, p.H, u[q]);
+    }
+    if (row + 1 == it.hi) {
+      const int g = it.item / p.splits;
+#pragma unroll
+      for (int q = 0; q < Q; ++q) {
+        F2 a[2], gv[2];
+        a_at(q, a);
+        g_at(g, q, gv);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int col = column4<VEC>(q, j, t, tpr);
+          if (col < p.H) {
+            const float sj = f2_at(S[q], j);
+            if (p.part_g) p.part_g[(int64_t)it.item * p.H + col] = p.alpha * f2_at(a, j) * sj;
+            float* pw = p.part_w + (int64_t)team * 2 * p.H + col;
+            const float v = f2_at(gv, j) * sj;
+            *pw = opened ? *pw + v : v;
+          }
+        }
+        S[q][0] = S[q][1] = f2_same(0.f);
+      }
+      opened = true;
+    }
+  }
+#pragma unroll
+  for (int q = 0; q < Q; ++q)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int col = column4<VEC>(q, j, t, tpr);
+      if (col < p.H) {
+        p.part_w[((int64_t)team * 2 + 1) * p.H + col] = f2_at(sw[q], j);
+        if (!opened) p.part_w[(int64_t)team * 2 * p.H + col] = 0.f;
+      }
+    }
+  // (every copy issued was waited for, unless a wait gave up: then its last copies are)
+  if (STAGED && !alive && t == 0)
+    for (int i = 0; i < p.slots; ++i)
+      for (int ph = 0; ph < 2; ++ph) tc::mbar_wait(&bar[i], ph, nullptr, 0);
+}
+
 // out[o][c] = sum over i < n of part[(o outer + i) stride + c]: a block takes 32 columns of one
-// output row, eight threads a column; the order of the sums does not depend on the launch.
+// output row, 32 threads a column; the order of the sums does not depend on the launch.
 struct Reduce {
   const float* part;
   float* out;
@@ -290,88 +610,115 @@ struct Reduce {
   int64_t outer, stride;
 };
 
-__global__ void __launch_bounds__(256)
-reduce_kernel(Reduce r0, Reduce r1, Reduce r2, int H, int64_t rows2) {
-  __shared__ float s[8][32];
+__global__ void __launch_bounds__(1024)
+reduce_kernel(Reduce r0, Reduce r1, Reduce r2, int H) {
+  __shared__ float s[32][33];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int col = blockIdx.x * 32 + lane;
   const int64_t o = blockIdx.y < 2 ? 0 : blockIdx.y - 2;
   const Reduce& r = blockIdx.y == 0 ? r0 : (blockIdx.y == 1 ? r1 : r2);
   if (!r.out) return;
   float a = 0.f;
-  if (col < H)
-    for (int i = w; i < r.n; i += 8) a += r.part[(o * r.outer + i) * r.stride + col];
+  if (col < H) {
+#pragma unroll 8
+    for (int i = w; i < r.n; i += 32) a += r.part[(o * r.outer + i) * r.stride + col];
+  }
   s[w][lane] = a;
   __syncthreads();
-  if (w == 0 && col < H) {
-#pragma unroll
-    for (int i = 1; i < 8; ++i) a += s[i][lane];
-    r.out[o * H + col] = a;
-  }
+  a = warp_sum(s[lane][w]);
+  const int c = blockIdx.x * 32 + w;
+  if (lane == 0 && c < H) r.out[o * H + c] = a;
 }
 
 constexpr int kMaxH = 32768;
 
-template <typename T, bool VEC, int TPR, int NC>
-static int fwd_launch(const Fwd& p, cudaStream_t st) {
-  const int per = TPR == 32 ? 8 : 1, threads = TPR == 32 ? 256 : TPR;
-  const unsigned g = (unsigned)((p.T + per - 1) / per);
-  if (p.codes) fwd_kernel<T, VEC, TPR, NC, true><<<g, threads, 0, st>>>(p);
-  else fwd_kernel<T, VEC, TPR, NC, false><<<g, threads, 0, st>>>(p);
+template <typename T, bool VEC, bool WARP, int NC>
+static int fwd_launch(const Fwd& p, int threads, cudaStream_t st) {
+  const unsigned g = (unsigned)(WARP ? (p.T + 7) / 8 : p.T);
+  if (p.codes) fwd_kernel<T, VEC, WARP, NC, true><<<g, threads, 0, st>>>(p);
+  else fwd_kernel<T, VEC, WARP, NC, false><<<g, threads, 0, st>>>(p);
   GSQ_CHECK_LAUNCH();
   return GSQ_OK;
 }
 
+// Threads of a block team with NC chunks of eight columns each.
+inline int team_threads(int H, int nc) { return ((H + 8 * nc - 1) / (8 * nc) + 31) / 32 * 32; }
+
 template <typename T, bool VEC>
 static int fwd_any(const Fwd& p, cudaStream_t st) {
-  const int v = (p.H + 7) / 8;
-  if (v <= 32) return fwd_launch<T, VEC, 32, 1>(p, st);
-  if (v <= 64) return fwd_launch<T, VEC, 32, 2>(p, st);
-  if (v <= 128) return fwd_launch<T, VEC, 32, 4>(p, st);
-  if (v <= 256) return fwd_launch<T, VEC, 64, 4>(p, st);
-  if (v <= 512) return fwd_launch<T, VEC, 128, 4>(p, st);
-  if (v <= 1024) return fwd_launch<T, VEC, 256, 4>(p, st);
-  if (v <= 2048) return fwd_launch<T, VEC, 512, 4>(p, st);
-  return fwd_launch<T, VEC, 1024, 4>(p, st);
+  if (p.H <= 256) return fwd_launch<T, VEC, true, 1>(p, 256, st);
+  if (p.H <= 8192) return fwd_launch<T, VEC, false, 1>(p, team_threads(p.H, 1), st);
+  if (p.H <= 16384) return fwd_launch<T, VEC, false, 2>(p, team_threads(p.H, 2), st);
+  return fwd_launch<T, VEC, false, 4>(p, team_threads(p.H, 4), st);
 }
 
-// Teams of the backward pass, and the parts each gate row's rows are cut into: as many teams as
-// stay resident, and parts so that every team has rows.
+// How the backward pass runs: as many teams as stay resident, the parts each gate row's rows
+// are cut into so that the teams share them evenly, and the rows in flight per team.
 struct Plan {
-  int blocks, teams, splits;
+  int threads, blocks, teams, splits, slots, weights;
+  uint32_t row_bytes;
+  size_t smem;
   int64_t ws;  // floats of workspace
 };
 
-static Plan bwd_plan(int T, int H, int groups, bool gate) {
+constexpr size_t kSmemTeam = 200 * 1024;  // of an SM, shared by its teams
+
+static Plan bwd_plan(int T, int H, int dtype, int groups, bool gate) {
   Plan pl;
-  const int v = (H + 7) / 8, per = v <= 128 ? 8 : 1;
-  const int most = num_sms() * (v <= 128 ? 1 : (v <= 256 ? 6 : (v <= 512 ? 3 : (v <= 1024 ? 2 : 1))));
+  const bool warp = H <= 256;
+  const int nc = H <= 8192 ? 1 : (H <= 16384 ? 2 : 4);
+  const int per = warp ? 8 : 1;
+  pl.threads = warp ? 256 : team_threads(H, nc);
+  pl.row_bytes = (uint32_t)((H * dtype_size(dtype) + 15) / 16 * 16 + 16);
+  pl.weights = H <= 4096 ? W_REG : W_SMEM;
+  const size_t slot = (size_t)kArrays * pl.row_bytes;
+  const size_t fix = pl.weights == W_SMEM ? (size_t)8 * ((H + 3) / 4 * 4) : 0;
+  if (nc > 1 || slot + fix > kSmemTeam) pl.weights = W_MEM;
+  // teams of an SM: 512 threads of 128 registers
+  const int sm_blocks = pl.weights == W_REG ? 512 / pl.threads : 1;
+  pl.slots = 1;
+  pl.smem = 0;
+  if (pl.weights != W_MEM) {
+    const size_t fit = (kSmemTeam / sm_blocks - fix) / (slot * per);
+    pl.slots = (int)(fit < 1 ? 1 : (fit > kMaxSlots ? kMaxSlots : fit));
+    pl.smem = (size_t)pl.slots * slot * per + fix;
+  }
   int64_t blocks = ((int64_t)T + per - 1) / per;
+  const int64_t most = (int64_t)num_sms() * sm_blocks;
   if (blocks > most) blocks = most;
   pl.blocks = (int)blocks;
   pl.teams = pl.blocks * per;
+  // one part a team at most: a part more than there are teams would take a second turn
   const int rows = T / groups;
-  int s = (pl.teams + groups - 1) / groups;
-  if (s > rows) s = rows;
+  int s = pl.teams / groups;
+  s = s < 1 ? 1 : (s > rows ? rows : s);
   pl.splits = s;
   pl.ws = (int64_t)pl.teams * 2 * H + (gate && s > 1 ? (int64_t)groups * s * H : 0);
   return pl;
 }
 
-template <typename T, bool VEC>
-static int bwd_any(const Bwd& p, const Plan& pl, cudaStream_t st) {
-  const int v = (p.H + 7) / 8;
-  const unsigned g = (unsigned)pl.blocks;
-  if (v <= 32) bwd_kernel<T, VEC, 32, 1><<<g, 256, 0, st>>>(p);
-  else if (v <= 64) bwd_kernel<T, VEC, 32, 2><<<g, 256, 0, st>>>(p);
-  else if (v <= 128) bwd_kernel<T, VEC, 32, 4><<<g, 256, 0, st>>>(p);
-  else if (v <= 256) bwd_kernel<T, VEC, 128, 2><<<g, 128, 0, st>>>(p);
-  else if (v <= 512) bwd_kernel<T, VEC, 256, 2><<<g, 256, 0, st>>>(p);
-  else if (v <= 1024) bwd_kernel<T, VEC, 512, 2><<<g, 512, 0, st>>>(p);
-  else if (v <= 2048) bwd_kernel<T, VEC, 1024, 2><<<g, 1024, 0, st>>>(p);
-  else bwd_kernel<T, VEC, 1024, 4><<<g, 1024, 0, st>>>(p);
+template <typename T, bool VEC, bool WARP, int Q, int W, int THREADS>
+static int bwd_launch(const Bwd& p, const Plan& pl, cudaStream_t st) {
+  auto kern = bwd_kernel<T, VEC, WARP, Q, W, THREADS>;
+  if (pl.smem > 48 * 1024 &&
+      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pl.smem) !=
+          cudaSuccess)
+    return GSQ_ECUDA;
+  kern<<<pl.blocks, pl.threads, pl.smem, st>>>(p);
   GSQ_CHECK_LAUNCH();
   return GSQ_OK;
+}
+
+template <typename T, bool VEC>
+static int bwd_any(const Bwd& p, const Plan& pl, cudaStream_t st) {
+  if (p.H <= 256) return bwd_launch<T, VEC, true, 2, W_REG, 256>(p, pl, st);
+  if (pl.weights == W_REG) return bwd_launch<T, VEC, false, 2, W_REG, 512>(p, pl, st);
+  if (pl.weights == W_SMEM) return pl.threads <= 768
+                                       ? bwd_launch<T, VEC, false, 2, W_SMEM, 768>(p, pl, st)
+                                       : bwd_launch<T, VEC, false, 2, W_SMEM, 1024>(p, pl, st);
+  if (p.H <= 8192) return bwd_launch<T, VEC, false, 2, W_MEM, 1024>(p, pl, st);
+  if (p.H <= 16384) return bwd_launch<T, VEC, false, 4, W_MEM, 1024>(p, pl, st);
+  return bwd_launch<T, VEC, false, 8, W_MEM, 1024>(p, pl, st);
 }
 
 inline bool row_vec(const void* p, int64_t ld, size_t es) {
@@ -425,10 +772,11 @@ extern "C" int gsq_residual_norm(const void* h, int64_t ld_h, const void* y, int
   return vec ? norm::fwd_any<float, true>(p, st) : norm::fwd_any<float, false>(p, st);
 }
 
-extern "C" int gsq_residual_norm_bwd_workspace(int T, int H, int gate_rows, int64_t* bytes) {
-  if (T <= 0 || H <= 0 || gate_rows < 0 || (gate_rows && T % gate_rows) || !bytes)
+extern "C" int gsq_residual_norm_bwd_workspace(int T, int H, int dtype, int gate_rows,
+                                               int64_t* bytes) {
+  if (T <= 0 || H <= 0 || dtype < 0 || dtype > 2 || gate_rows < 0 || (gate_rows && T % gate_rows) || !bytes)
     return GSQ_EINVAL;
-  *bytes = norm::bwd_plan(T, H, gate_rows ? gate_rows : 1, gate_rows > 0).ws *
+  *bytes = norm::bwd_plan(T, H, dtype, gate_rows ? gate_rows : 1, gate_rows > 0).ws *
            (int64_t)sizeof(float);
   return GSQ_OK;
 }
@@ -440,8 +788,8 @@ extern "C" int gsq_residual_norm_bwd(const void* h, int64_t ld_h, const void* y,
                                      int dtype, float alpha, float offset, void* dh,
                                      int64_t ld_dh, void* dy, int64_t ld_dy, float* dw_post,
                                      float* dw_pre, float* dgate, float* workspace,
-                                     int64_t workspace_bytes, void* stream) {
-  if (T <= 0 || H <= 0 || dtype < 0 || dtype > 2 || !stats) return GSQ_EINVAL;
+                                     int64_t workspace_bytes, int* err, void* stream) {
+  if (T <= 0 || H <= 0 || dtype < 0 || dtype > 2 || !stats || !err) return GSQ_EINVAL;
   const size_t es = dtype_size(dtype);
   if (!norm::row_ok(h, ld_h, H, es) || !norm::row_ok(y, ld_y, H, es) ||
       !norm::row_ok(dh, ld_dh, H, es) || !norm::row_ok(dy, ld_dy, H, es))
@@ -452,17 +800,18 @@ extern "C" int gsq_residual_norm_bwd(const void* h, int64_t ld_h, const void* y,
     return GSQ_EINVAL;
   if (H > norm::kMaxH) return GSQ_ENOTSUP;
   const int groups = gate ? gate_rows : 1;
-  const norm::Plan pl = norm::bwd_plan(T, H, groups, gate != nullptr);
+  const norm::Plan pl = norm::bwd_plan(T, H, dtype, groups, gate != nullptr);
   if (!workspace || (uintptr_t)workspace % 4 || workspace_bytes < pl.ws * (int64_t)sizeof(float))
     return GSQ_EINVAL;
   norm::Bwd p;
-  p.h = h; p.y = y; p.w_post = w_post; p.w_pre = w_pre; p.gate = gate;
-  p.ld_h = ld_h; p.ld_y = ld_y; p.stats = stats;
-  p.dh2 = dh2; p.ld_dh2 = ld_dh2; p.dx = dx; p.ld_dx = ld_dx;
+  p.in[0] = y; p.in[1] = h; p.in[2] = dx; p.in[3] = dh2;
+  p.ld[0] = ld_y; p.ld[1] = ld_h; p.ld[2] = ld_dx; p.ld[3] = ld_dh2;
+  p.w_post = w_post; p.w_pre = w_pre; p.gate = gate; p.stats = stats;
   p.T = T; p.H = H; p.per_gate = T / groups;
   p.alpha = alpha; p.offset = offset;
   p.dh = dh; p.ld_dh = ld_dh; p.dy = dy; p.ld_dy = ld_dy;
-  p.groups = groups; p.splits = pl.splits;
+  p.groups = groups; p.splits = pl.splits; p.slots = pl.slots; p.row_bytes = pl.row_bytes;
+  p.err = err;
   p.part_w = workspace;
   p.part_g = !gate ? nullptr
                    : (pl.splits == 1 ? dgate : workspace + (int64_t)pl.teams * 2 * H);
@@ -484,8 +833,8 @@ extern "C" int gsq_residual_norm_bwd(const void* h, int64_t ld_h, const void* y,
   const norm::Reduce r1 = {workspace + H, w_pre ? dw_pre : nullptr, pl.teams, 0, 2 * (int64_t)H};
   const norm::Reduce r2 = {p.part_g, gsum ? dgate : nullptr, pl.splits, pl.splits, H};
   if (w_post || w_pre || gsum) {
-    norm::reduce_kernel<<<dim3((H + 31) / 32, 2 + (gsum ? groups : 0)), 256, 0, st>>>(r0, r1, r2,
-                                                                                      H, groups);
+    norm::reduce_kernel<<<dim3((H + 31) / 32, 2 + (gsum ? groups : 0)), 1024, 0, st>>>(r0, r1, r2,
+                                                                                       H);
     GSQ_CHECK_LAUNCH();
   }
   return GSQ_OK;

@@ -578,18 +578,19 @@ int gsq_residual_norm(const void *h, int64_t ld_h, const void *y, int64_t ld_y,
                       float *scales, int64_t ld_scales, float *stats, void *stream);
 
 /* Bytes of workspace of gsq_residual_norm_bwd (gate_rows 0: no gate), on the current device. */
-int gsq_residual_norm_bwd_workspace(int T, int H, int gate_rows, int64_t *bytes);
+int gsq_residual_norm_bwd_workspace(int T, int H, int dtype, int gate_rows, int64_t *bytes);
 
 /* Its vector-Jacobian product: dh, dy [T][H] in dtype and the float32 gradients dw_post [H],
  * dw_pre [H], dgate [gate_rows][H] of the parameters present, for the cotangents dh2 of h_out
- * (NULL: zero) and dx of x (with w_pre only), from the inputs and stats of the forward pass. */
+ * (NULL: zero) and dx of x (with w_pre only), from the inputs and stats of the forward pass.
+ * err: device word, nonzero after a bounded wait gave up. */
 int gsq_residual_norm_bwd(const void *h, int64_t ld_h, const void *y, int64_t ld_y,
                           const void *w_post, const void *w_pre, const void *gate, int gate_rows,
                           const float *stats, const void *dh2, int64_t ld_dh2, const void *dx,
                           int64_t ld_dx, int T, int H, int dtype, float alpha, float offset,
                           void *dh, int64_t ld_dh, void *dy, int64_t ld_dy, float *dw_post,
                           float *dw_pre, float *dgate, float *workspace, int64_t workspace_bytes,
-                          void *stream);
+                          int *err, void *stream);
 
 #ifdef __cplusplus
 }

@@ -221,15 +221,15 @@ def test_norm_entry_points_refuse_bad_arguments():
         wide[i] = 32769
     assert lib.gsq_residual_norm(*wide) == _lib.GSQ_ENOTSUP
     n = C.c_int64()
-    for bad in ((0, 64, 0), (4, 0, 0), (4, 64, 3), (4, 64, -1)):
+    for bad in ((0, 64, 0, 0), (4, 0, 0, 0), (4, 64, 0, 3), (4, 64, 0, -1), (4, 64, 3, 0)):
         assert lib.gsq_residual_norm_bwd_workspace(*bad, C.byref(n)) == _lib.GSQ_EINVAL
-    assert lib.gsq_residual_norm_bwd_workspace(4, 64, 0, None) == _lib.GSQ_EINVAL
+    assert lib.gsq_residual_norm_bwd_workspace(4, 64, 0, 0, None) == _lib.GSQ_EINVAL
     bwd = [P, 64, P, 64, P, P, P, 2, P, P, 64, P, 64, 4, 64, 0, 1.0, 0.0, P, 64, P, 64, P, P, P, P,
-           1 << 40, None]
+           1 << 40, P, None]
     _refused(lib.gsq_residual_norm_bwd, bwd,
              [(0, None), (1, 63), (2, None), (6, None), (7, 3), (8, None), (10, 63), (11, None),
               (12, 63), (13, 0), (14, 0), (15, 3), (18, None), (20, None), (22, None), (23, None),
-              (24, None), (25, None), (26, 16)])
+              (24, None), (25, None), (26, 16), (27, None)])
     none = list(bwd)
     none[5], none[9], none[11], none[23] = None, None, None, None   # neither cotangent
     assert lib.gsq_residual_norm_bwd(*none) == _lib.GSQ_EINVAL
