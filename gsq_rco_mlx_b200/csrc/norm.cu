@@ -77,172 +77,280 @@ __device__ __forceinline__ float team_sum(float v, float (*red)[32], int& turn) 
   return warp_sum(r[lane]);
 }
 
-// Column of value j of chunk c: eight neighbours (VEC), or dealt round the team.
+// Columns are dealt in fours: column j < 4 of a thread's chunk q is one of four neighbours (VEC:
+// chunks go round the team; a warp's chunk is 128 columns), or goes round the team by itself.
 template <bool VEC>
-__device__ __forceinline__ int column(int c, int j, int t, int tpr) {
-  return VEC ? (c * tpr + t) * 8 + j : (c * 8 + j) * tpr + t;
+__device__ __forceinline__ int column(int q, int j, int t, int tpr) {
+  return VEC ? (q * tpr + t) * 4 + j : (q * 4 + j) * tpr + t;
 }
 
-// The thread's eight values of chunk c of a row; columns from H on are zero.
-template <typename T, bool VEC>
-__device__ __forceinline__ void get8(const T* __restrict__ row, int c, int t, int tpr, int H,
-                                     float v[8]) {
-  if (VEC) {
-    load8<T, true>(row, (c * tpr + t) * 8, H, v);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int col = column<false>(c, j, t, tpr);
-      v[j] = col < H ? to_f32(row[col]) : 0.f;
+// Chunk q of a row as it lies in memory; columns from H on are zero. VEC: H is a multiple of 4
+// and the row starts on 8 (16-bit types) or 16 bytes. PAD: the row has room for the whole team's
+// columns, so it may be read past H.
+template <typename T>
+struct alignas(4 * sizeof(T)) Four {
+  T e[4];
+};
+
+template <typename T, bool VEC, bool PAD>
+__device__ __forceinline__ Four<T> raw4(const T* row, int q, int t, int tpr, int H) {
+  const int c0 = column<VEC>(q, 0, t, tpr);
+  Four<T> v;
+  if constexpr (VEC) {
+    if constexpr (sizeof(T) == 2) {
+      uint2 r = make_uint2(0u, 0u);
+      if (c0 < H) r = *reinterpret_cast<const uint2*>(row + c0);
+      *reinterpret_cast<uint2*>(&v) = r;
+    } else {
+      float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (c0 < H) r = *reinterpret_cast<const float4*>(row + c0);
+      *reinterpret_cast<float4*>(&v) = r;
     }
+  } else {
+    const T zero = from_f32<T>(0.f);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int col = c0 + j * tpr;
+      if (PAD) {
+        v.e[j] = row[col];
+        v.e[j] = col < H ? v.e[j] : zero;
+      } else {
+        v.e[j] = col < H ? row[col] : zero;
+      }
+    }
+  }
+  return v;
+}
+
+template <typename T>
+__device__ __forceinline__ void pairs(const Four<T>& r, F2 v[2]) {
+  v[0] = {to_f32(r.e[0]), to_f32(r.e[1])};
+  v[1] = {to_f32(r.e[2]), to_f32(r.e[3])};
+}
+
+template <typename T, bool VEC, bool PAD>
+__device__ __forceinline__ void get4(const T* row, int q, int t, int tpr, int H, F2 v[2]) {
+  pairs(raw4<T, VEC, PAD>(row, q, t, tpr, H), v);
+}
+
+template <typename T, bool VEC>
+__device__ __forceinline__ void put4(T* __restrict__ row, int q, int t, int tpr, int H,
+                                     const F2 v[2]) {
+  const int c0 = column<VEC>(q, 0, t, tpr);
+  if constexpr (VEC) {
+    if (c0 < H) {
+      if constexpr (sizeof(T) == 2)
+        *reinterpret_cast<uint2*>(row + c0) = make_uint2(f2_pack<T>(v[0]), f2_pack<T>(v[1]));
+      else
+        *reinterpret_cast<float4*>(row + c0) = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+    }
+  } else {
+    const float f[4] = {v[0].x, v[0].y, v[1].x, v[1].y};
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (c0 + j * tpr < H) row[c0 + j * tpr] = from_f32<T>(f[j]);
   }
 }
 
+__device__ __forceinline__ float f2_dot(const F2 a[2], const F2 b[2]) {
+  const F2 s = f2_fma(a[1], b[1], f2_mul(a[0], b[0]));
+  return s.x + s.y;
+}
+__device__ __forceinline__ float f2_at(const F2 v[2], int j) {
+  return j & 1 ? v[j >> 1].y : v[j >> 1].x;
+}
+
+// 1 / sqrt(m): the hardware's estimate (2 steps off at most) after one Newton iteration
+// r += r (1 - m r^2) / 2, whose residual is formed in one fused operation.
+__device__ __forceinline__ float inv_root(float m) {
+  const float r = rsqrtf(m);
+  const float n = fmaf(0.5f * r, fmaf(-m * r, r, 1.f), r);
+  return isfinite(n) ? n : r;   // (m = infinity or denormal: the estimate itself)
+}
+
+// A thread's columns of the parameters: alpha a g (from the gate row g) and b; 1 stands for a
+// missing w_post or gate, 0 for a missing w_pre.
+struct Params {
+  const void *w_post, *w_pre, *gate;
+  float alpha, offset;
+  int H;
+};
+
 template <typename T, bool VEC>
-__device__ __forceinline__ void put8(T* __restrict__ row, int c, int t, int tpr, int H,
-                                     const float v[8]) {
-  if (VEC) {
-    store8<T, true>(row, (c * tpr + t) * 8, H, v);
-  } else {
+struct Columns {
+  const Params& p;
+  int t, tpr;
+  __device__ __forceinline__ void a(int q, F2 v[2]) const {
+    if (p.w_post) get4<T, VEC, false>(reinterpret_cast<const T*>(p.w_post), q, t, tpr, p.H, v);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int col = column<false>(c, j, t, tpr);
-      if (col < H) row[col] = from_f32<T>(v[j]);
-    }
+    for (int j = 0; j < 2; ++j) v[j] = p.w_post ? f2_add(v[j], f2_same(p.offset)) : f2_same(1.f);
   }
-}
+  __device__ __forceinline__ void alpha_g(int g, int q, F2 v[2]) const {
+    if (p.gate)
+      get4<T, VEC, false>(reinterpret_cast<const T*>(p.gate) + (int64_t)g * p.H, q, t, tpr, p.H, v);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) v[j] = p.gate ? f2_mul(v[j], f2_same(p.alpha)) : f2_same(p.alpha);
+  }
+  __device__ __forceinline__ void alpha_ag(int g, int q, F2 v[2]) const {
+    F2 gv[2];
+    a(q, v);
+    alpha_g(g, q, gv);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) v[j] = f2_mul(v[j], gv[j]);
+  }
+  __device__ __forceinline__ void b(int q, F2 v[2]) const {
+    if (p.w_pre) get4<T, VEC, false>(reinterpret_cast<const T*>(p.w_pre), q, t, tpr, p.H, v);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) v[j] = p.w_pre ? f2_add(v[j], f2_same(p.offset)) : f2_same(0.f);
+  }
+};
 
-__device__ __forceinline__ float sumsq8(const float v[8]) {
-  const float a = fmaf(v[1], v[1], v[0] * v[0]), b = fmaf(v[3], v[3], v[2] * v[2]);
-  const float c = fmaf(v[5], v[5], v[4] * v[4]), d = fmaf(v[7], v[7], v[6] * v[6]);
-  return (a + b) + (c + d);
-}
-
-// One row per team (no loop over rows: enough blocks are resident to hide the loads). The
-// statistics are 1 / sqrt rounded once, so that x rounds no worse than its definition.
-template <typename T, bool VEC, bool WARP, int NC, bool FP8>
-__global__ void __launch_bounds__(WARP ? 256 : 1024, 1) fwd_kernel(const __grid_constant__ Fwd p) {
+// Persistent teams: team i takes rows i, i + teams, ...; the parameters' columns stay in
+// registers (HOLD) where the team leaves room for them, and the next row's loads are issued
+// before this row is worked on.
+template <typename T, bool VEC, bool WARP, int Q, bool HOLD, bool FP8, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) fwd_kernel(const __grid_constant__ Fwd p) {
   __shared__ __align__(16) float red[2][32];
-  __shared__ uint32_t amax_s[FP8 && !VEC ? 256 : 1];
+  __shared__ uint32_t amax_s[FP8 && !VEC ? 512 : 1];   // two rows' blocks, in turn
   int turn = 0;
   const int t = WARP ? threadIdx.x & 31 : threadIdx.x, tpr = WARP ? 32 : blockDim.x;
-  const int row = WARP ? blockIdx.x * 8 + (threadIdx.x >> 5) : blockIdx.x;
-  if (!WARP) {
-    if (threadIdx.x < 64) red[threadIdx.x >> 5][threadIdx.x & 31] = 0.f;
-    if (FP8 && !VEC)
-      for (int i = threadIdx.x; i < 256; i += blockDim.x) amax_s[i] = 0u;
-    __syncthreads();
-  } else if (FP8 && !VEC) {
-    for (int i = threadIdx.x; i < 256; i += blockDim.x) amax_s[i] = 0u;
-    __syncthreads();
-  }
-  if (row >= p.T) return;  // (a whole warp, or a whole block)
-  const T* hr = reinterpret_cast<const T*>(p.h) + (int64_t)row * p.ld_h;
-  const T* yr = reinterpret_cast<const T*>(p.y) + (int64_t)row * p.ld_y;
-  float y[NC][8], h[NC][8];
+  const int w = WARP ? threadIdx.x >> 5 : 0;
+  const int teams = WARP ? gridDim.x * 8 : gridDim.x;
+  if (!WARP && threadIdx.x < 64) red[threadIdx.x >> 5][threadIdx.x & 31] = 0.f;
+  if (FP8 && !VEC)
+    for (int i = threadIdx.x; i < 512; i += blockDim.x) amax_s[i] = 0u;
+  __syncthreads();
+  const Params pa = {p.w_post, p.w_pre, p.gate, p.alpha, p.offset, p.H};
+  const Columns<T, VEC> col{pa, t, tpr};
+  const float inv_H = 1.f / (float)p.H;
+  const T* h_in = reinterpret_cast<const T*>(p.h);
+  const T* y_in = reinterpret_cast<const T*>(p.y);
+  F2 ag[HOLD ? Q : 1][2], bw[HOLD ? Q : 1][2];
+  int held = -1;
+  int row = WARP ? blockIdx.x * 8 + w : blockIdx.x;
+  Four<T> yn[Q], hn[Q];   // the next row
+  auto load = [&](int r) {
 #pragma unroll
-  for (int c = 0; c < NC; ++c) get8<T, VEC>(yr, c, t, tpr, p.H, y[c]);
+    for (int q = 0; q < Q; ++q) yn[q] = raw4<T, VEC, false>(y_in + (int64_t)r * p.ld_y, q, t, tpr, p.H);
 #pragma unroll
-  for (int c = 0; c < NC; ++c) get8<T, VEC>(hr, c, t, tpr, p.H, h[c]);
-  const T* gr = p.gate ? reinterpret_cast<const T*>(p.gate) + (int64_t)(row / p.per_gate) * p.H
-                       : nullptr;
-  const float H = (float)p.H;
-  float r1 = 1.f;
-  if (p.w_post) {
+    for (int q = 0; q < Q; ++q) hn[q] = raw4<T, VEC, false>(h_in + (int64_t)r * p.ld_h, q, t, tpr, p.H);
+  };
+  int half = 0;
+  if (HOLD && row < p.T) load(row);
+  for (; row < p.T; row += teams, half ^= 256) {
+    F2 y[Q][2], h[Q][2];
+    if (!HOLD) load(row);
+#pragma unroll
+    for (int q = 0; q < Q; ++q) pairs(yn[q], y[q]), pairs(hn[q], h[q]);
+    if (HOLD && row + teams < p.T) load(row + teams);
+    const int g = p.gate ? row / p.per_gate : 0;
+    if (HOLD && g != held) {
+#pragma unroll
+      for (int q = 0; q < Q; ++q) {
+        col.alpha_ag(g, q, ag[HOLD ? q : 0]);
+        if (held < 0) col.b(q, bw[HOLD ? q : 0]);
+      }
+      held = g;
+    }
+    float r1 = 1.f, r2 = 1.f;
+    if (p.w_post) {
+      float s = 0.f;
+#pragma unroll
+      for (int q = 0; q < Q; ++q) s += f2_dot(y[q], y[q]);
+      r1 = inv_root(fmaf(team_sum<WARP>(s, red, turn), inv_H, p.eps));
+    }
     float s = 0.f;
 #pragma unroll
-    for (int c = 0; c < NC; ++c) s += sumsq8(y[c]);
-    r1 = __frsqrt_rn(__fdiv_rn(team_sum<WARP>(s, red, turn), H) + p.eps);
-  }
-  float s = 0.f;
+    for (int q = 0; q < Q; ++q) {
+      F2 v[2];
+      if (!HOLD) col.alpha_ag(g, q, v);
 #pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    if (p.w_post) {
-      float a[8];
-      get8<T, VEC>(reinterpret_cast<const T*>(p.w_post), c, t, tpr, p.H, a);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) y[c][j] = (y[c][j] * r1) * (a[j] + p.offset);
+      for (int j = 0; j < 2; ++j)
+        h[q][j] = f2_fma(HOLD ? ag[HOLD ? q : 0][j] : v[j], f2_mul(y[q][j], f2_same(r1)), h[q][j]);
+      s += f2_dot(h[q], h[q]);
+      if (p.h_out)
+        put4<T, VEC>(reinterpret_cast<T*>(p.h_out) + (int64_t)row * p.ld_ho, q, t, tpr, p.H, h[q]);
     }
-    if (gr) {
-      float g[8];
-      get8<T, VEC>(gr, c, t, tpr, p.H, g);
+    if (p.w_pre) {
+      r2 = inv_root(fmaf(team_sum<WARP>(s, red, turn), inv_H, p.eps));
 #pragma unroll
-      for (int j = 0; j < 8; ++j) y[c][j] *= g[j];
-    }
+      for (int q = 0; q < Q; ++q) {
+        F2 v[2];
+        if (!HOLD) col.b(q, v);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      // (columns from H on stay zero whatever the weights' pad would give)
-      h[c][j] = column<VEC>(c, j, t, tpr) < p.H ? fmaf(p.alpha, y[c][j], h[c][j]) : 0.f;
-    }
-    s += sumsq8(h[c]);
-    if (p.h_out)
-      put8<T, VEC>(reinterpret_cast<T*>(p.h_out) + (int64_t)row * p.ld_ho, c, t, tpr, p.H, h[c]);
-  }
-  float r2 = 1.f;
-  if (p.w_pre) {
-    r2 = __frsqrt_rn(__fdiv_rn(team_sum<WARP>(s, red, turn), H) + p.eps);
-#pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      float b[8];
-      get8<T, VEC>(reinterpret_cast<const T*>(p.w_pre), c, t, tpr, p.H, b);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        h[c][j] = (h[c][j] * r2) * (b[j] + p.offset);
-        if (FP8 && column<VEC>(c, j, t, tpr) >= p.H) h[c][j] = 0.f;
+        for (int j = 0; j < 2; ++j)
+          h[q][j] = f2_mul(f2_mul(h[q][j], f2_same(r2)), HOLD ? bw[HOLD ? q : 0][j] : v[j]);
+        if (!FP8)
+          put4<T, VEC>(reinterpret_cast<T*>(p.x) + (int64_t)row * p.ld_x, q, t, tpr, p.H, h[q]);
       }
-      if (!FP8)
-        put8<T, VEC>(reinterpret_cast<T*>(p.x) + (int64_t)row * p.ld_x, c, t, tpr, p.H, h[c]);
-    }
-    if (FP8 && VEC) {
-      // a 128-column block is the eight columns of each of 16 neighbouring lanes
+      if (FP8 && VEC) {
+        // a warp's chunk is one 128-column block; magnitudes compare as their bits (NaN is above
+        // infinity). Lane 2 q divides m / 448, lane 2 q + 1 448 / m.
+        const int lane = t & 31;
+        float num = 1.f, den = 1.f;
 #pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        const int col = (c * tpr + t) * 8;
-        float m = amax8(h[c]);
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-        m = max_nan(m, kFp8AmaxMin);
-        if (col < p.H) {
-          if ((t & 15) == 0)
-            p.scales[(int64_t)(col / kFp8Block) * p.ld_s + row] = __fdiv_rn(m, kFp8Max);
-          *reinterpret_cast<uint2*>(p.codes + (int64_t)row * p.ld_c + col) =
-              encode8(h[c], __fdiv_rn(kFp8Max, m));
+        for (int q = 0; q < Q; ++q) {
+          const uint32_t bits = max(max(__float_as_uint(fabsf(h[q][0].x)), __float_as_uint(fabsf(h[q][0].y))),
+                                    max(__float_as_uint(fabsf(h[q][1].x)), __float_as_uint(fabsf(h[q][1].y))));
+          const float m = max_nan(__uint_as_float(__reduce_max_sync(0xffffffffu, bits)),
+                                  kFp8AmaxMin);
+          if (lane == 2 * q) num = m, den = kFp8Max;
+          if (lane == 2 * q + 1) num = kFp8Max, den = m;
         }
-      }
-    }
-    if (FP8 && !VEC) {
-      // a warp's 32 columns of one j lie in one block: a warp maximum, then one shared-memory
-      // maximum per warp and block (magnitudes compare as their bits; NaN is above infinity)
-      uint32_t* am = amax_s + (WARP ? (threadIdx.x >> 5) * 2 : 0);
+        const float quot = __fdiv_rn(num, den);
 #pragma unroll
-      for (int c = 0; c < NC; ++c)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(h[c][j])));
-          const int col = column<false>(c, j, t, tpr);
-          if ((t & 31) == 0 && col < p.H) atomicMax(am + col / kFp8Block, m);
-        }
-      if (WARP) __syncwarp();
-      else __syncthreads();
-      for (int b = t; b < (p.H + kFp8Block - 1) / kFp8Block; b += tpr)
-        p.scales[(int64_t)b * p.ld_s + row] =
-            __fdiv_rn(max_nan(__uint_as_float(am[b]), kFp8AmaxMin), kFp8Max);
-#pragma unroll
-      for (int c = 0; c < NC; ++c)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int col = column<false>(c, j, t, tpr);
-          if (col < p.H) {
-            const float m = max_nan(__uint_as_float(am[col / kFp8Block]), kFp8AmaxMin);
-            p.codes[(int64_t)row * p.ld_c + col] =
-                (uint8_t)cvt4_e4m3(__fmul_rn(h[c][j], __fdiv_rn(kFp8Max, m)), 0.f, 0.f, 0.f);
+        for (int q = 0; q < Q; ++q) {
+          const float r = __shfl_sync(0xffffffffu, quot, 2 * q + 1);
+          const int c0 = column<true>(q, 0, t, tpr);
+          if (lane == 2 * q && c0 - 8 * q < p.H)   // (the warp's first column of the chunk)
+            p.scales[(int64_t)(c0 / kFp8Block) * p.ld_s + row] = quot;
+          if (c0 < p.H) {
+            const F2 u = f2_mul(h[q][0], f2_same(r)), v = f2_mul(h[q][1], f2_same(r));
+            *reinterpret_cast<uint32_t*>(p.codes + (int64_t)row * p.ld_c + c0) =
+                cvt4_e4m3(u.x, u.y, v.x, v.y);
           }
         }
+      }
+      if (FP8 && !VEC) {
+        // a warp's 32 columns of one j lie in one block: a warp maximum, then one shared-memory
+        // maximum per warp and block
+        const int nb = (p.H + kFp8Block - 1) / kFp8Block;
+        uint32_t* am = amax_s + half + (WARP ? w * 4 : 0);
+        uint32_t* other = amax_s + (half ^ 256) + (WARP ? w * 4 : 0);
+#pragma unroll
+        for (int q = 0; q < Q; ++q)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(f2_at(h[q], j))));
+            const int c = column<false>(q, j, t, tpr);
+            if ((t & 31) == 0 && c < p.H) atomicMax(am + c / kFp8Block, m);
+          }
+        if (WARP) __syncwarp();
+        else __syncthreads();
+        for (int b = t; b < nb; b += tpr) {
+          p.scales[(int64_t)b * p.ld_s + row] =
+              __fdiv_rn(max_nan(__uint_as_float(am[b]), kFp8AmaxMin), kFp8Max);
+          other[b] = 0u;   // for the next row
+        }
+#pragma unroll
+        for (int q = 0; q < Q; ++q)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int c = column<false>(q, j, t, tpr);
+            if (c < p.H) {
+              const float m = max_nan(__uint_as_float(am[c / kFp8Block]), kFp8AmaxMin);
+              p.codes[(int64_t)row * p.ld_c + c] = (uint8_t)cvt4_e4m3(
+                  __fmul_rn(f2_at(h[q], j), __fdiv_rn(kFp8Max, m)), 0.f, 0.f, 0.f);
+            }
+          }
+        // (a block's next row passes the barrier of its second sum before it adds to `other`)
+        if (WARP) __syncwarp();
+      }
     }
-  }
-  if (t == 0) {
-    p.stats[row] = r1;
-    p.stats[p.T + row] = r2;
+    if (t == 0) {
+      p.stats[row] = r1;
+      p.stats[p.T + row] = r2;
+    }
   }
 }
 
@@ -296,95 +404,6 @@ __device__ __forceinline__ void fetch_row(const Bwd& p, int row, uint8_t* slot, 
 
 constexpr int kMaxSlots = 4;
 
-// The backward pass deals columns in fours: column j < 4 of a thread's chunk q is one of four
-// neighbours (VEC: chunks go round the team), or goes round the team by itself.
-template <bool VEC>
-__device__ __forceinline__ int column4(int q, int j, int t, int tpr) {
-  return VEC ? (q * tpr + t) * 4 + j : (q * 4 + j) * tpr + t;
-}
-
-template <typename T>
-__device__ __forceinline__ float lds1(uint32_t a) {
-  if constexpr (sizeof(T) == 2) {
-    uint16_t v;
-    asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"(a));
-    return to_f32(*reinterpret_cast<const T*>(&v));
-  } else {
-    float v;
-    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a));
-    return v;
-  }
-}
-
-// Chunk q of a row, as two pairs: from shared memory (byte address `row`) or from memory;
-// columns from H on read as zero.
-template <typename T, bool VEC>
-__device__ __forceinline__ void sget4(uint32_t row, int q, int t, int tpr, int H, F2 v[2]) {
-  const int c0 = column4<VEC>(q, 0, t, tpr);
-  if (VEC && c0 + 4 <= H) {
-    if constexpr (sizeof(T) == 2) {
-      uint32_t x, y;
-      asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(x), "=r"(y) : "r"(row + c0 * 2));
-      v[0] = f2_unpack<T>(x);
-      v[1] = f2_unpack<T>(y);
-    } else {
-      asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
-                   : "=f"(v[0].x), "=f"(v[0].y), "=f"(v[1].x), "=f"(v[1].y)
-                   : "r"(row + c0 * 4));
-    }
-  } else {
-    const int step = VEC ? 1 : tpr;
-    uint32_t a = row + c0 * sizeof(T);
-    float f[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      f[j] = c0 + j * step < H ? lds1<T>(a) : 0.f;
-      a += step * sizeof(T);
-    }
-    v[0] = {f[0], f[1]};
-    v[1] = {f[2], f[3]};
-  }
-}
-
-template <typename T, bool VEC>
-__device__ __forceinline__ void get4(const T* __restrict__ row, int q, int t, int tpr, int H,
-                                     F2 v[2]) {
-  const int c0 = column4<VEC>(q, 0, t, tpr), step = VEC ? 1 : tpr;
-  float f[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) f[j] = c0 + j * step < H ? to_f32(row[c0 + j * step]) : 0.f;
-  v[0] = {f[0], f[1]};
-  v[1] = {f[2], f[3]};
-}
-
-template <typename T, bool VEC>
-__device__ __forceinline__ void put4(T* __restrict__ row, int q, int t, int tpr, int H,
-                                     const F2 v[2]) {
-  const int c0 = column4<VEC>(q, 0, t, tpr), step = VEC ? 1 : tpr;
-  if (VEC && c0 + 4 <= H) {
-    if constexpr (sizeof(T) == 2)
-      *reinterpret_cast<uint2*>(row + c0) = make_uint2(f2_pack<T>(v[0]), f2_pack<T>(v[1]));
-    else
-      *reinterpret_cast<float4*>(row + c0) = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
-  } else {
-    const float f[4] = {v[0].x, v[0].y, v[1].x, v[1].y};
-    T* o = row + c0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (c0 + j * step < H) *o = from_f32<T>(f[j]);
-      o += step;
-    }
-  }
-}
-
-__device__ __forceinline__ float f2_dot(const F2 a[2], const F2 b[2]) {
-  const F2 s = f2_fma(a[1], b[1], f2_mul(a[0], b[0]));
-  return s.x + s.y;
-}
-__device__ __forceinline__ float f2_at(const F2 v[2], int j) {
-  return j & 1 ? v[j >> 1].y : v[j >> 1].x;
-}
-
 // Where a thread's alpha a g and b are kept: in registers up to 512 threads a team, in shared
 // memory up to 1024, and read anew for every row where a row does not fit shared memory.
 enum Weights { W_REG, W_SMEM, W_MEM };
@@ -409,10 +428,8 @@ __global__ void __launch_bounds__(THREADS, 1) bwd_kernel(const __grid_constant__
   uint64_t* bar = bars[w];
   const uint32_t slot_bytes = kArrays * p.row_bytes;
   uint8_t* mine = dyn + (size_t)w * p.slots * slot_bytes;
-  const uint32_t mine_a = tc::smem_u32(mine);
   float* ag_s = reinterpret_cast<float*>(dyn + (size_t)(WARP ? 8 : 1) * p.slots * slot_bytes);
-  const int ldw = (p.H + 3) / 4 * 4;
-  const uint32_t ag_a = tc::smem_u32(ag_s), b_a = ag_a + ldw * 4;
+  float* b_s = ag_s + 4 * Q * tpr;
   if (!WARP && threadIdx.x < 64) red[threadIdx.x >> 5][threadIdx.x & 31] = 0.f;
   if (STAGED && t == 0) {
     for (int i = 0; i < p.slots; ++i) tc::mbar_init(&bar[i], 1);
@@ -427,30 +444,9 @@ __global__ void __launch_bounds__(THREADS, 1) bwd_kernel(const __grid_constant__
       fetch_row<T>(p, ahead.row, mine + i * slot_bytes, &bar[i]);
     ahead_s[w] = ahead;
   }
-  const T* wpost = reinterpret_cast<const T*>(p.w_post);
-  const T* wpre = reinterpret_cast<const T*>(p.w_pre);
-  auto a_at = [&](int q, F2 v[2]) {
-    if (wpost) get4<T, VEC>(wpost, q, t, tpr, p.H, v);
-#pragma unroll
-    for (int j = 0; j < 2; ++j) v[j] = wpost ? f2_add(v[j], f2_same(p.offset)) : f2_same(1.f);
-  };
-  auto g_at = [&](int g, int q, F2 v[2]) {   // alpha g
-    if (p.gate) get4<T, VEC>(reinterpret_cast<const T*>(p.gate) + (int64_t)g * p.H, q, t, tpr, p.H, v);
-#pragma unroll
-    for (int j = 0; j < 2; ++j) v[j] = p.gate ? f2_mul(v[j], f2_same(p.alpha)) : f2_same(p.alpha);
-  };
-  auto ag_of = [&](int g, int q, F2 v[2]) {   // alpha a g
-    F2 gv[2];
-    a_at(q, v);
-    g_at(g, q, gv);
-#pragma unroll
-    for (int j = 0; j < 2; ++j) v[j] = f2_mul(v[j], gv[j]);
-  };
-  auto b_of = [&](int q, F2 v[2]) {
-    if (wpre) get4<T, VEC>(wpre, q, t, tpr, p.H, v);
-#pragma unroll
-    for (int j = 0; j < 2; ++j) v[j] = wpre ? f2_add(v[j], f2_same(p.offset)) : f2_same(0.f);
-  };
+  const bool post = p.w_post != nullptr, pre = p.w_pre != nullptr;
+  const Params pa = {p.w_post, p.w_pre, p.gate, p.alpha, p.offset, p.H};
+  const Columns<T, VEC> cols{pa, t, tpr};
   F2 S[Q][2], sw[Q][2];     // sums of d y r1 and of dx h' r2
   F2 ag[QW][2], bw[QW][2];
 #pragma unroll
@@ -468,34 +464,29 @@ __global__ void __launch_bounds__(THREADS, 1) bwd_kernel(const __grid_constant__
 #pragma unroll
       for (int q = 0; q < Q; ++q) {
         F2 v[2], u[2];
-        ag_of(g, q, v);
-        if (held < 0) b_of(q, u);
+        cols.alpha_ag(g, q, v);
+        cols.b(q, u);
+        if (W == W_REG) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int col = column4<VEC>(q, j, t, tpr);
-          if (W == W_REG) {
-            if ((j & 1) == 0) {
-              ag[W == W_REG ? q : 0][j >> 1] = v[j >> 1];
-              if (held < 0) bw[W == W_REG ? q : 0][j >> 1] = u[j >> 1];
-            }
-          } else if (col < p.H) {   // (each thread reads only what it wrote)
-            ag_s[col] = f2_at(v, j);
-            if (held < 0) ag_s[ldw + col] = f2_at(u, j);
-          }
+          for (int j = 0; j < 2; ++j) ag[W == W_REG ? q : 0][j] = v[j], bw[W == W_REG ? q : 0][j] = u[j];
+        } else {   // (each thread reads only what it wrote)
+          put4<float, VEC>(ag_s, q, t, tpr, 4 * Q * tpr, v);
+          put4<float, VEC>(b_s, q, t, tpr, 4 * Q * tpr, u);
         }
       }
       held = it.item;
     }
-    const float r1 = wpost ? p.stats[row] : 1.f, r2 = wpre ? p.stats[p.T + row] : 1.f;
+    const float r1 = post ? p.stats[row] : 1.f, r2 = pre ? p.stats[p.T + row] : 1.f;
     // (after a timeout the rows run on unread, so that the block's barriers keep their count)
     if (STAGED && alive) alive = tc::mbar_wait(&bar[slot], phase, p.err, 6);
     auto read = [&](int i, int q, F2 v[2]) {
       const T* src = reinterpret_cast<const T*>(p.in[i]) + (int64_t)row * p.ld[i];
       if (STAGED)
-        sget4<T, VEC>(mine_a + slot * slot_bytes + i * p.row_bytes + ((uint32_t)(uintptr_t)src & 15u),
-                      q, t, tpr, p.H, v);
+        get4<T, VEC, true>(reinterpret_cast<const T*>(mine + slot * slot_bytes + i * p.row_bytes +
+                                                      ((uint32_t)(uintptr_t)src & 15u)),
+                           q, t, tpr, p.H, v);
       else
-        get4<T, VEC>(src, q, t, tpr, p.H, v);
+        get4<T, VEC, false>(src, q, t, tpr, p.H, v);
     };
     F2 y[Q][2], h[Q][2], u[Q][2];
     float s = 0.f;
@@ -504,24 +495,24 @@ __global__ void __launch_bounds__(THREADS, 1) bwd_kernel(const __grid_constant__
       F2 wv[2];
       read(0, q, y[q]);
       read(1, q, h[q]);
-      if (W == W_SMEM) sget4<float, VEC>(ag_a, q, t, tpr, p.H, wv);
-      if (W == W_MEM) ag_of(it.item / p.splits, q, wv);
+      if (W == W_SMEM) get4<float, VEC, true>(ag_s, q, t, tpr, 4 * Q * tpr, wv);
+      if (W == W_MEM) cols.alpha_ag(it.item / p.splits, q, wv);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         y[q][j] = f2_mul(y[q][j], f2_same(r1));
         h[q][j] = f2_mul(f2_fma(W == W_REG ? ag[W == W_REG ? q : 0][j] : wv[j], y[q][j], h[q][j]),
                          f2_same(r2));   // h' r2
       }
-      if (wpre) {
+      if (pre) {
         read(2, q, u[q]);
-        if (W == W_SMEM) sget4<float, VEC>(b_a, q, t, tpr, p.H, wv);
-        if (W == W_MEM) b_of(q, wv);
+        if (W == W_SMEM) get4<float, VEC, true>(b_s, q, t, tpr, 4 * Q * tpr, wv);
+        if (W == W_MEM) cols.b(q, wv);
       }
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        if (!wpre) u[q][j] = f2_same(0.f);
+        if (!pre) u[q][j] = f2_same(0.f);
         sw[q][j] = f2_fma(u[q][j], h[q][j], sw[q][j]);
-        if (wpre) u[q][j] = f2_mul(u[q][j], W == W_REG ? bw[W == W_REG ? q : 0][j] : wv[j]);
+        if (pre) u[q][j] = f2_mul(u[q][j], W == W_REG ? bw[W == W_REG ? q : 0][j] : wv[j]);
       }
       s += f2_dot(u[q], h[q]);
     }
@@ -531,12 +522,12 @@ __global__ void __launch_bounds__(THREADS, 1) bwd_kernel(const __grid_constant__
     for (int q = 0; q < Q; ++q) {
       F2 wv[2], d[2], e[2];
       if (p.in[3]) read(3, q, d);
-      if (W == W_SMEM) sget4<float, VEC>(ag_a, q, t, tpr, p.H, wv);
-      if (W == W_MEM) ag_of(it.item / p.splits, q, wv);
+      if (W == W_SMEM) get4<float, VEC, true>(ag_s, q, t, tpr, 4 * Q * tpr, wv);
+      if (W == W_MEM) cols.alpha_ag(it.item / p.splits, q, wv);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         if (!p.in[3]) d[j] = f2_same(0.f);
-        if (wpre) d[j] = f2_fma(f2_same(r2), f2_fma(f2_same(-mu), h[q][j], u[q][j]), d[j]);
+        if (pre) d[j] = f2_fma(f2_same(r2), f2_fma(f2_same(-mu), h[q][j], u[q][j]), d[j]);
         e[j] = f2_mul(d[j], y[q][j]);
         S[q][j] = f2_add(S[q][j], e[j]);
         u[q][j] = f2_mul(W == W_REG ? ag[W == W_REG ? q : 0][j] : wv[j], d[j]);   // v
@@ -545,7 +536,7 @@ __global__ void __launch_bounds__(THREADS, 1) bwd_kernel(const __grid_constant__
       put4<T, VEC>(reinterpret_cast<T*>(p.dh) + (int64_t)row * p.ld_dh, q, t, tpr, p.H, d);
     }
     float mv = team_sum<WARP>(s, red, turn) * inv_H;
-    if (!wpost) mv = 0.f;
+    if (!post) mv = 0.f;
     // every thread has read the slot (the sum's barrier; a warp's shuffles): the next row may land
     if (STAGED && t == 0 && alive && ahead_s[w].item >= 0) {
       fetch_row<T>(p, ahead_s[w].row, mine + slot * slot_bytes, &bar[slot]);
@@ -567,11 +558,11 @@ __global__ void __launch_bounds__(THREADS, 1) bwd_kernel(const __grid_constant__
 #pragma unroll
       for (int q = 0; q < Q; ++q) {
         F2 a[2], gv[2];
-        a_at(q, a);
-        g_at(g, q, gv);
+        cols.a(q, a);
+        cols.alpha_g(g, q, gv);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int col = column4<VEC>(q, j, t, tpr);
+          const int col = column<VEC>(q, j, t, tpr);
           if (col < p.H) {
             const float sj = f2_at(S[q], j);
             if (p.part_g) p.part_g[(int64_t)it.item * p.H + col] = p.alpha * f2_at(a, j) * sj;
@@ -589,7 +580,7 @@ __global__ void __launch_bounds__(THREADS, 1) bwd_kernel(const __grid_constant__
   for (int q = 0; q < Q; ++q)
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int col = column4<VEC>(q, j, t, tpr);
+      const int col = column<VEC>(q, j, t, tpr);
       if (col < p.H) {
         p.part_w[((int64_t)team * 2 + 1) * p.H + col] = f2_at(sw[q], j);
         if (!opened) p.part_w[(int64_t)team * 2 * p.H + col] = 0.f;
@@ -632,24 +623,29 @@ reduce_kernel(Reduce r0, Reduce r1, Reduce r2, int H) {
 
 constexpr int kMaxH = 32768;
 
-template <typename T, bool VEC, bool WARP, int NC>
+// Threads of a block team with Q chunks of four columns each.
+inline int team_threads(int H, int q) { return ((H + 4 * q - 1) / (4 * q) + 31) / 32 * 32; }
+
+template <typename T, bool VEC, bool WARP, int Q, bool HOLD, int THREADS>
 static int fwd_launch(const Fwd& p, int threads, cudaStream_t st) {
-  const unsigned g = (unsigned)(WARP ? (p.T + 7) / 8 : p.T);
-  if (p.codes) fwd_kernel<T, VEC, WARP, NC, true><<<g, threads, 0, st>>>(p);
-  else fwd_kernel<T, VEC, WARP, NC, false><<<g, threads, 0, st>>>(p);
+  int64_t blocks = WARP ? ((int64_t)p.T + 7) / 8 : p.T;
+  // the blocks that stay resident: 1024 threads of 64 registers an SM
+  const int64_t most = (int64_t)num_sms() * (1024 / threads);
+  if (blocks > most) blocks = most;
+  const unsigned g = (unsigned)blocks;
+  if (p.codes) fwd_kernel<T, VEC, WARP, Q, HOLD, true, THREADS><<<g, threads, 0, st>>>(p);
+  else fwd_kernel<T, VEC, WARP, Q, HOLD, false, THREADS><<<g, threads, 0, st>>>(p);
   GSQ_CHECK_LAUNCH();
   return GSQ_OK;
 }
 
-// Threads of a block team with NC chunks of eight columns each.
-inline int team_threads(int H, int nc) { return ((H + 8 * nc - 1) / (8 * nc) + 31) / 32 * 32; }
-
 template <typename T, bool VEC>
 static int fwd_any(const Fwd& p, cudaStream_t st) {
-  if (p.H <= 256) return fwd_launch<T, VEC, true, 1>(p, 256, st);
-  if (p.H <= 8192) return fwd_launch<T, VEC, false, 1>(p, team_threads(p.H, 1), st);
-  if (p.H <= 16384) return fwd_launch<T, VEC, false, 2>(p, team_threads(p.H, 2), st);
-  return fwd_launch<T, VEC, false, 4>(p, team_threads(p.H, 4), st);
+  if (p.H <= 256) return fwd_launch<T, VEC, true, 2, true, 256>(p, 256, st);
+  if (p.H <= 4096) return fwd_launch<T, VEC, false, 2, true, 512>(p, team_threads(p.H, 2), st);
+  if (p.H <= 8192) return fwd_launch<T, VEC, false, 2, false, 1024>(p, team_threads(p.H, 2), st);
+  if (p.H <= 16384) return fwd_launch<T, VEC, false, 4, false, 1024>(p, team_threads(p.H, 4), st);
+  return fwd_launch<T, VEC, false, 8, false, 1024>(p, team_threads(p.H, 8), st);
 }
 
 // How the backward pass runs: as many teams as stay resident, the parts each gate row's rows
@@ -666,14 +662,16 @@ constexpr size_t kSmemTeam = 200 * 1024;  // of an SM, shared by its teams
 static Plan bwd_plan(int T, int H, int dtype, int groups, bool gate) {
   Plan pl;
   const bool warp = H <= 256;
-  const int nc = H <= 8192 ? 1 : (H <= 16384 ? 2 : 4);
+  const int q = H <= 8192 ? 2 : (H <= 16384 ? 4 : 8);
   const int per = warp ? 8 : 1;
-  pl.threads = warp ? 256 : team_threads(H, nc);
-  pl.row_bytes = (uint32_t)((H * dtype_size(dtype) + 15) / 16 * 16 + 16);
+  pl.threads = warp ? 256 : team_threads(H, q);
+  // room for the whole team's columns (a row is read past H) and for an unaligned start
+  const int room = 4 * q * (warp ? 32 : pl.threads);
+  pl.row_bytes = (uint32_t)(room * dtype_size(dtype) + 32);
   pl.weights = H <= 4096 ? W_REG : W_SMEM;
   const size_t slot = (size_t)kArrays * pl.row_bytes;
-  const size_t fix = pl.weights == W_SMEM ? (size_t)8 * ((H + 3) / 4 * 4) : 0;
-  if (nc > 1 || slot + fix > kSmemTeam) pl.weights = W_MEM;
+  const size_t fix = pl.weights == W_SMEM ? (size_t)8 * room : 0;
+  if (q > 2 || slot + fix > kSmemTeam) pl.weights = W_MEM;
   // teams of an SM: 512 threads of 128 registers
   const int sm_blocks = pl.weights == W_REG ? 512 / pl.threads : 1;
   pl.slots = 1;
@@ -760,7 +758,7 @@ extern "C" int gsq_residual_norm(const void* h, int64_t ld_h, const void* y, int
   p.h_out = h_out; p.ld_ho = ld_ho; p.x = x; p.ld_x = ld_x;
   p.codes = (uint8_t*)codes; p.ld_c = ld_codes; p.scales = scales; p.ld_s = ld_scales;
   p.stats = stats;
-  const bool vec = norm::row_vec(h, ld_h, es) && norm::row_vec(y, ld_y, es) &&
+  const bool vec = H % 4 == 0 && norm::row_vec(h, ld_h, es) && norm::row_vec(y, ld_y, es) &&
                    norm::row_vec(w_post, 0, es) && norm::row_vec(w_pre, 0, es) &&
                    norm::row_vec(gate, H, es) && norm::row_vec(h_out, ld_ho, es) &&
                    norm::row_vec(x, ld_x, es);
@@ -815,7 +813,7 @@ extern "C" int gsq_residual_norm_bwd(const void* h, int64_t ld_h, const void* y,
   p.part_w = workspace;
   p.part_g = !gate ? nullptr
                    : (pl.splits == 1 ? dgate : workspace + (int64_t)pl.teams * 2 * H);
-  const bool vec = norm::row_vec(h, ld_h, es) && norm::row_vec(y, ld_y, es) &&
+  const bool vec = H % 4 == 0 && norm::row_vec(h, ld_h, es) && norm::row_vec(y, ld_y, es) &&
                    norm::row_vec(w_post, 0, es) && norm::row_vec(w_pre, 0, es) &&
                    norm::row_vec(gate, H, es) && norm::row_vec(dh2, ld_dh2, es) &&
                    norm::row_vec(dx, ld_dx, es) && norm::row_vec(dh, ld_dh, es) &&
