@@ -175,11 +175,12 @@ constexpr int kBM = 128;
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = 128 + 32 * kEpiWarps;
 constexpr int kMaxStages = 8;
-constexpr uint32_t kPipeBytes = 192 * 1024;
+constexpr uint32_t kPipeBytes = 144 * 1024;
+constexpr uint32_t kStageBytes = kEpiWarps * 2 * 4096;  // output boxes, two a warp
 constexpr uint32_t kTmemCols = 512;
 
 struct GemmArgs {
-  CUtensorMap a, b;
+  CUtensorMap a, b, o;
   int M, N, K, kb;
   int mt, nt;       // tiles along m and n
   int group;        // m tiles walked together (tile order)
@@ -189,7 +190,7 @@ struct GemmArgs {
   int64_t sb_n, sb_k;
   void* out;
   int64_t ld_o;
-  int accumulate, vec;  // vec: rows of out start on 16 bytes
+  int accumulate, boxes;  // boxes: out is written through the map o
   int* err;
 };
 
@@ -207,8 +208,35 @@ __device__ __forceinline__ void umma_e4m3(uint32_t d, uint64_t a, uint64_t b, ui
       "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
 }
 
+template <int N>
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t* r) {
+  if constexpr (N == 32) {
+    tc::tmem_ld32_nowait(taddr, r);
+  } else {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
+        "%11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+          "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+  }
+}
+
+__device__ __forceinline__ void copy4(float* to, const float* from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(tc::smem_u32(to)), "l"(from)
+               : "memory");
+}
+
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(tc::smem_u32(bar)) : "memory");
+}
+
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* src, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                   (uint64_t)map),
+               "r"(tc::smem_u32(src)), "r"(x), "r"(y)
+               : "memory");
 }
 
 // Tile t in groups of `group` row tiles: within a group the row tile runs fastest, so the CTAs
@@ -221,23 +249,54 @@ __device__ __forceinline__ void tile_at(const GemmArgs& p, int t, int& m, int& n
   m = g * p.group + (i - n * rows);
 }
 
+// An output row's values of one warp column range, element by element (rows that TMA cannot
+// write, and sums into what is there).
 template <typename T, int CW>
-__device__ __forceinline__ void store_row(const GemmArgs& p, int m, int n0, const float* acc) {
+__device__ __forceinline__ void store_row(const GemmArgs& p, int m, int n0, const F2* acc) {
   if (m >= p.M) return;
   T* o = reinterpret_cast<T*>(p.out) + (int64_t)m * p.ld_o + n0;
-  constexpr int V = 16 / sizeof(T);
 #pragma unroll
-  for (int c = 0; c < CW; c += V) {
-    if (p.vec && !p.accumulate && n0 + c + V <= p.N) {
-      __align__(16) T e[V];
+  for (int c = 0; c < CW; ++c) {
+    const float v = c & 1 ? acc[c >> 1].y : acc[c >> 1].x;
+    if (n0 + c < p.N) o[c] = from_f32<T>(p.accumulate ? v + to_f32(o[c]) : v);
+  }
+}
+
+// The tile's rows of one warp as boxes of 32 rows x 128 bytes, staged in shared memory in the
+// store's 128-byte swizzle (16-byte chunk c of row r at c ^ (r % 8): a lane writes its own row
+// without bank conflicts) and written by the TMA unit, which clips what lies outside the
+// output. Two buffers a warp: a box is written while the last one is still being read.
+template <typename T, int CW>
+__device__ __forceinline__ void store_boxes(const GemmArgs& p, uint8_t* stage, int& buf, int lane,
+                                            int m0, int n0, const F2* acc) {
+  constexpr int BW = 128 / sizeof(T);  // columns of a box
+  if (m0 >= p.M) return;
 #pragma unroll
-      for (int j = 0; j < V; ++j) e[j] = from_f32<T>(acc[c + j]);
-      *reinterpret_cast<uint4*>(o + c) = *reinterpret_cast<const uint4*>(e);
-    } else {
+  for (int c0 = 0; c0 < CW; c0 += BW) {
+    if (n0 + c0 < p.N) {
+      uint8_t* b = stage + buf * 4096;
+      if (lane == 0) tc::bulk_wait_read<1>();
+      __syncwarp();
 #pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (n0 + c + j < p.N)
-          o[c + j] = from_f32<T>(p.accumulate ? acc[c + j] + to_f32(o[c + j]) : acc[c + j]);
+      for (int c = 0; c < 8; ++c) {
+        uint4 v;
+        if constexpr (sizeof(T) == 2) {
+          const F2* a = acc + (c0 + c * 8) / 2;
+          v = make_uint4(f2_pack<T>(a[0]), f2_pack<T>(a[1]), f2_pack<T>(a[2]), f2_pack<T>(a[3]));
+        } else {
+          const F2* a = acc + (c0 + c * 4) / 2;
+          v = make_uint4(__float_as_uint(a[0].x), __float_as_uint(a[0].y),
+                         __float_as_uint(a[1].x), __float_as_uint(a[1].y));
+        }
+        *reinterpret_cast<uint4*>(b + lane * 128 + ((c ^ (lane & 7)) << 4)) = v;
+      }
+      tc::fence_proxy_async_shared();
+      __syncwarp();
+      if (lane == 0) {
+        tma_store_2d(&p.o, b, n0 + c0, m0);
+        tc::bulk_commit();
+      }
+      buf ^= 1;
     }
   }
 }
@@ -270,7 +329,12 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
   uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages], tfull[4], tempty[4], last;
   __shared__ uint32_t tmem_base;
-  __shared__ __align__(16) float sb_s[BROWS ? kEpiWarps : 1][BROWS ? 2 : 1][BROWS ? CW : 4];
+  constexpr int CH = BN == 256 ? 16 : 32;
+  // k-blocks whose scales are on their way, and the ring's entries
+  constexpr int kAhead = BROWS && BN == 256 ? 2 : 4, kRing = kAhead + 1;
+  constexpr int kRow = 32 + (BROWS ? CW : 4);   // a k-block's scales of a warp: rows, columns
+  __shared__ __align__(16) float ring_s[kEpiWarps][kRing * kRow];
+  uint8_t* stage = smem + kStages * kStage;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
@@ -345,73 +409,107 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
     if (BN == 256) regs_inc<216>();
     const int q = warp & 3, half = (warp - 4) >> 2;
     const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16) + half * CW;
+    // The scales of the k-block kAhead ahead (of the next tile's, at a tile's end) are copied to
+    // the warp's ring while this one is folded: a load from L2 takes longer than a k-block.
+    float* ring = ring_s[warp - 4];
+    int pt = blockIdx.x, pk = 0, pslot = 0, pn = 0;
+    const float *psa = nullptr, *psb = nullptr;
+    auto prefetch = [&]() {
+      if (pt < tiles) {
+        if (pk == 0) {
+          int mi, ni;
+          tile_at(p, pt, mi, ni);
+          const int m = mi * kBM + q * 32 + lane;
+          psa = p.sa + (m < p.M ? m : 0);
+          pn = ni * BN + half * CW;
+          // CW is 64 or 128 and pn a multiple of it: a warp's columns lie in one weight block
+          psb = BROWS ? p.sb + lane : p.sb + min(pn, p.N - 1) / kBlk * p.sb_n;
+        }
+        float* to = ring + pslot * kRow;
+        copy4(to + lane, psa);
+        if (BROWS) {
+#pragma unroll
+          for (int i = 0; i < CW / 32; ++i)
+            copy4(to + 32 + 32 * i + lane, psb + (pn + 32 * i + lane < p.N ? pn + 32 * i : -lane));
+        } else if (lane == 0) {
+          copy4(to + 32, psb);
+        }
+        psa += p.ld_sa;
+        psb += p.sb_k;
+        if (++pk == p.kb) {
+          pk = 0;
+          pt += gridDim.x;
+        }
+        pslot = pslot + 1 == kRing ? 0 : pslot + 1;
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) prefetch();
     uint32_t it = 0;
+    int buf = 0, islot = 0;
     bool ok = true;
     for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
       int mi, ni;
       tile_at(p, t, mi, ni);
       const int m = mi * kBM + q * 32 + lane, n0 = ni * BN + half * CW;
-      const float* sa = p.sa + (m < p.M ? m : 0);
-      // CW is 64 or 128 and n0 a multiple of it: a warp's columns lie in one weight block
-      const float* sb = BROWS ? p.sb : p.sb + min(n0, p.N - 1) / kBlk * p.sb_n;
-      float acc[CW];
+      F2 acc[CW / 2];
 #pragma unroll
-      for (int c = 0; c < CW; ++c) acc[c] = 0.f;
-      // the scales of the next k-block are on their way while this one is folded
-      float sa_n = sa[0], sb_n = BROWS ? 1.f : sb[0];
-      float sbr[BROWS ? CW / 32 : 1];
-      if (BROWS) {
-#pragma unroll
-        for (int i = 0; i < CW / 32; ++i)
-          sbr[BROWS ? i : 0] = n0 + 32 * i + lane < p.N ? sb[n0 + 32 * i + lane] : 0.f;
-      }
+      for (int c = 0; c < CW / 2; ++c) acc[c] = f2_same(0.f);
       for (int k = 0; k < p.kb; ++k, ++it) {
         const int sl = it % kSlots;
-        const float s = sa_n * sb_n;
-        if (BROWS) {
-#pragma unroll
-          for (int i = 0; i < CW / 32; ++i)
-            sb_s[warp - 4][k & 1][32 * i + lane] = sbr[BROWS ? i : 0];
-        }
-        if (k + 1 < p.kb) {
-          sa_n = sa[(int64_t)(k + 1) * p.ld_sa];
-          if (!BROWS) {
-            sb_n = sb[(int64_t)(k + 1) * p.sb_k];
-          } else {
-#pragma unroll
-            for (int i = 0; i < CW / 32; ++i)
-              sbr[BROWS ? i : 0] =
-                  n0 + 32 * i + lane < p.N ? sb[(int64_t)(k + 1) * p.sb_k + n0 + 32 * i + lane]
-                                           : 0.f;
-          }
-        }
+        asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
         ok = tc::mbar_wait(&tfull[sl], (it / kSlots) & 1, p.err, 5);
-        ok = __all_sync(0xffffffffu, ok);  // (also orders sb_s between the lanes)
+        ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
+        __syncwarp();   // the other lanes' copies
         tc::fence_after_sync();
-        const float* sbw = sb_s[BROWS ? warp - 4 : 0][BROWS ? k & 1 : 0];
+        const float* sc = ring + islot * kRow;
+        islot = islot + 1 == kRing ? 0 : islot + 1;
+        const float s = BROWS ? sc[lane] : sc[lane] * sc[32];
+        const float* sbw = sc + 32;
+        // CH columns are folded while the next are on their way from TMEM; the accumulator is
+        // given back before the last ones are folded
+        uint32_t r[2][CH];
+        tmem_ld<CH>(lanes + sl * BN, r[0]);
 #pragma unroll
-        for (int c = 0; c < CW; c += 32) {
-          uint32_t r[32];
-          tc::tmem_ld32_nowait(lanes + sl * BN + c, r);
+        for (int c = 0; c < CW / CH; ++c) {
           tc::tmem_wait_ld();
+          if (c + 1 < CW / CH) {
+            tmem_ld<CH>(lanes + sl * BN + CH * (c + 1), r[(c + 1) & 1]);
+          } else {
+            tc::fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&tempty[sl]);
+          }
+          const uint32_t* d = r[c & 1];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            const float d = __uint_as_float(r[j]);
-            acc[c + j] = __fmaf_rn(BROWS ? __fmul_rn(d, sbw[BROWS ? c + j : 0]) : d, s,
-                                   acc[c + j]);
+          for (int j = 0; j < CH / 2; ++j) {
+            F2 v = {__uint_as_float(d[2 * j]), __uint_as_float(d[2 * j + 1])};
+            if (BROWS) v = f2_mul(v, *reinterpret_cast<const F2*>(sbw + (BROWS ? CH * c + 2 * j : 0)));
+            F2& to = acc[CH / 2 * c + j];
+            to = f2_fma(v, f2_same(s), to);
           }
         }
-        tc::fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&tempty[sl]);
+        __syncwarp();   // (BROWS: every lane has read the ring's entry)
+        prefetch();
       }
       if (ok) {
-        if (dtype == BF16) store_row<__nv_bfloat16, CW>(p, m, n0, acc);
-        else if (dtype == F16) store_row<__half, CW>(p, m, n0, acc);
-        else store_row<float, CW>(p, m, n0, acc);
+        uint8_t* st = stage + (warp - 4) * 8192;
+        const int m0 = m - lane;
+        if (p.boxes) {
+          if (dtype == BF16) store_boxes<__nv_bfloat16, CW>(p, st, buf, lane, m0, n0, acc);
+          else if (dtype == F16) store_boxes<__half, CW>(p, st, buf, lane, m0, n0, acc);
+          else store_boxes<float, CW>(p, st, buf, lane, m0, n0, acc);
+        } else {
+          if (dtype == BF16) store_row<__nv_bfloat16, CW>(p, m, n0, acc);
+          else if (dtype == F16) store_row<__half, CW>(p, m, n0, acc);
+          else store_row<float, CW>(p, m, n0, acc);
+        }
       }
     }
+    if (lane == 0) tc::bulk_wait_all();
+    asm volatile("cp.async.wait_all;" ::: "memory");
   }
   tc::fence_before_sync();
   __syncthreads();
@@ -452,10 +550,27 @@ static bool codes_map(CUtensorMap* m, const void* base, int64_t rows, int cols, 
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// out [M][ld] in boxes of 32 rows x 128 bytes.
+static bool out_map(CUtensorMap* m, void* base, int dtype, int M, int N, int64_t ld) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t es = dtype_size(dtype);
+  cuuint64_t dims[2] = {(cuuint64_t)N, (cuuint64_t)M};
+  cuuint64_t strides[1] = {(cuuint64_t)ld * es};
+  cuuint32_t box[2] = {(cuuint32_t)(128 / es), 32};
+  cuuint32_t estr[2] = {1, 1};
+  const CUtensorMapDataType t = dtype == BF16  ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                : dtype == F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                               : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
+  return fn(m, t, 2, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int BN, bool BROWS>
 static int launch_gemm(GemmArgs& p, int dtype, cudaStream_t st) {
   constexpr uint32_t kStage = (kBM + BN) * kBlk;
-  constexpr uint32_t smem = kPipeBytes / kStage * kStage + 1024;
+  constexpr uint32_t smem = kPipeBytes / kStage * kStage + kStageBytes + 1024;
   auto kern = gemm_kernel<BN, BROWS>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) !=
       cudaSuccess)
@@ -606,8 +721,13 @@ extern "C" int gsq_fp8_gemm(int M, int N, int K, const void* a, int64_t lda, con
                     accumulate, err))
     return GSQ_EINVAL;
   fp8::GemmArgs p;
-  const int64_t tiles256 = (int64_t)((M + 127) / 128) * ((N + 255) / 256);
-  const bool wide = tiles256 >= num_sms();
+  // Tile width by the rounds that the busiest CTA walks: a 256-wide tile costs two 128-wide ones
+  // but loads its A rows once (4094 x 896 x 4864: 128 wide tiles are one round of 148 SMs, 224
+  // narrow ones two halves; 4864 x 896 x 4094: 152 wide tiles are two rounds, 266 narrow ones two
+  // halves).
+  const int64_t mt = (M + 127) / 128;
+  const auto rounds = [&](int bn) { return (mt * ((N + bn - 1) / bn) + num_sms() - 1) / num_sms(); };
+  const bool wide = 2 * rounds(256) <= rounds(128) + (rounds(128) >= 8 ? 1 : 0);
   if (!fp8::codes_map(&p.a, a, M, K, lda, fp8::kBM) ||
       !fp8::codes_map(&p.b, b, N, K, ldb, wide ? 256 : 128))
     return GSQ_ECUDA;
@@ -623,7 +743,8 @@ extern "C" int gsq_fp8_gemm(int M, int N, int K, const void* a, int64_t lda, con
   p.out = out;
   p.ld_o = ld_out;
   p.accumulate = accumulate;
-  p.vec = (uintptr_t)out % 16 == 0 && ld_out * dtype_size(dtype) % 16 == 0;
+  p.boxes = !accumulate && (uintptr_t)out % 16 == 0 && ld_out * dtype_size(dtype) % 16 == 0;
+  if (p.boxes && !fp8::out_map(&p.o, out, dtype, M, N, ld_out)) return GSQ_ECUDA;
   p.err = err;
   cudaStream_t st = (cudaStream_t)stream;
   if (sb_rows) return wide ? fp8::launch_gemm<256, true>(p, dtype, st)
