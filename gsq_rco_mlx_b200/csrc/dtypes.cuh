@@ -26,41 +26,6 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
 template <>
 __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 
-// Eight values of a row from column c on; columns past `cols` are zero. VEC: the row starts on
-// 16 bytes and c is a multiple of 8.
-template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* __restrict__ row, int c, int cols, float v[8]) {
-  if (VEC && c + 8 <= cols) {
-    constexpr int N4 = sizeof(T) * 8 / 16;
-    uint4 raw[N4];
-#pragma unroll
-    for (int i = 0; i < N4; ++i) raw[i] = reinterpret_cast<const uint4*>(row + c)[i];
-    const T* e = reinterpret_cast<const T*>(raw);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = to_f32(e[j]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = c + j < cols ? to_f32(row[c + j]) : 0.f;
-  }
-}
-
-template <typename T, bool VEC>
-__device__ __forceinline__ void store8(T* __restrict__ row, int c, int cols, const float v[8]) {
-  if (VEC && c + 8 <= cols) {
-    constexpr int N4 = sizeof(T) * 8 / 16;
-    __align__(16) T e[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) e[j] = from_f32<T>(v[j]);
-#pragma unroll
-    for (int i = 0; i < N4; ++i)
-      reinterpret_cast<uint4*>(row + c)[i] = reinterpret_cast<const uint4*>(e)[i];
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (c + j < cols) row[c + j] = from_f32<T>(v[j]);
-  }
-}
-
 // Pairs of float32 in one instruction (each half rounds as the scalar operation does): the fused
 // multiply-add of a pair issues as fast as a single one.
 struct F2 {
@@ -118,6 +83,58 @@ __device__ __forceinline__ uint32_t f2_pack<__half>(F2 v) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// A row's columns are dealt to a team of tpr threads in fours: column j < 4 of a thread's chunk q
+// is one of four neighbours (VEC: chunks go round the team; a warp's chunk is 128 columns), or
+// goes round the team by itself, which keeps every access of a warp to a row one segment.
+template <bool VEC>
+__device__ __forceinline__ int column(int q, int j, int t, int tpr) {
+  return VEC ? (q * tpr + t) * 4 + j : (q * 4 + j) * tpr + t;
+}
+
+// Chunk q of a row as it lies in memory; columns from H on are zero. VEC: H is a multiple of 4
+// and the row starts on 8 (16-bit types) or 16 bytes. PAD: the row has room for the whole team's
+// columns, so it may be read past H.
+template <typename T>
+struct alignas(4 * sizeof(T)) Four {
+  T e[4];
+};
+
+template <typename T, bool VEC, bool PAD>
+__device__ __forceinline__ Four<T> raw4(const T* row, int q, int t, int tpr, int H) {
+  const int c0 = column<VEC>(q, 0, t, tpr);
+  Four<T> v;
+  if constexpr (VEC) {
+    if constexpr (sizeof(T) == 2) {
+      uint2 r = make_uint2(0u, 0u);
+      if (c0 < H) r = *reinterpret_cast<const uint2*>(row + c0);
+      *reinterpret_cast<uint2*>(&v) = r;
+    } else {
+      float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (c0 < H) r = *reinterpret_cast<const float4*>(row + c0);
+      *reinterpret_cast<float4*>(&v) = r;
+    }
+  } else {
+    const T zero = from_f32<T>(0.f);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int col = c0 + j * tpr;
+      if (PAD) {
+        v.e[j] = row[col];
+        v.e[j] = col < H ? v.e[j] : zero;
+      } else {
+        v.e[j] = col < H ? row[col] : zero;
+      }
+    }
+  }
+  return v;
+}
+
+template <typename T>
+__device__ __forceinline__ void pairs(const Four<T>& r, F2 v[2]) {
+  v[0] = {to_f32(r.e[0]), to_f32(r.e[1])};
+  v[1] = {to_f32(r.e[2]), to_f32(r.e[3])};
+}
+
 // maximum that keeps NaN (fmaxf drops it)
 __device__ __forceinline__ float max_nan(float a, float b) {
   float d;
@@ -131,11 +148,10 @@ constexpr int kFp8Block = 128;
 constexpr float kFp8Max = 448.f;
 constexpr float kFp8AmaxMin = 7.8886090522101181e-31f;  // 2^-100
 
-__device__ __forceinline__ float amax8(const float v[8]) {
-  float a = fabsf(v[0]);
-#pragma unroll
-  for (int j = 1; j < 8; ++j) a = max_nan(a, fabsf(v[j]));
-  return a;
+// Bits of the largest magnitude of four (magnitudes compare as their bits, NaN above infinity).
+__device__ __forceinline__ uint32_t amax4(const F2 v[2]) {
+  return max(max(__float_as_uint(fabsf(v[0].x)), __float_as_uint(fabsf(v[0].y))),
+             max(__float_as_uint(fabsf(v[1].x)), __float_as_uint(fabsf(v[1].y))));
 }
 
 __device__ __forceinline__ uint32_t cvt4_e4m3(float a, float b, float c, float d) {
@@ -145,11 +161,22 @@ __device__ __forceinline__ uint32_t cvt4_e4m3(float a, float b, float c, float d
   return (uint32_t)lo | ((uint32_t)hi << 16);
 }
 
-__device__ __forceinline__ uint2 encode8(const float v[8], float r) {
-  float q[8];
+__device__ __forceinline__ uint32_t encode4(const F2 v[2], float r) {
+  const F2 a = f2_mul(v[0], f2_same(r)), b = f2_mul(v[1], f2_same(r));
+  return cvt4_e4m3(a.x, a.y, b.x, b.y);
+}
+
+// Writes a chunk's codes (as raw4 deals columns): one word, or a byte each.
+template <bool VEC>
+__device__ __forceinline__ void put_codes(uint8_t* row, int q, int t, int tpr, int H, uint32_t c) {
+  const int c0 = column<VEC>(q, 0, t, tpr);
+  if (VEC) {
+    if (c0 < H) *reinterpret_cast<uint32_t*>(row + c0) = c;
+  } else {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) q[j] = __fmul_rn(v[j], r);
-  return make_uint2(cvt4_e4m3(q[0], q[1], q[2], q[3]), cvt4_e4m3(q[4], q[5], q[6], q[7]));
+    for (int j = 0; j < 4; ++j)
+      if (c0 + j * tpr < H) row[c0 + j * tpr] = (uint8_t)(c >> (8 * j));
+  }
 }
 
 }  // namespace gsq

@@ -27,124 +27,164 @@ namespace fp8 {
 constexpr int kBlk = kFp8Block;
 
 // ---------------------------------------------------------------------- quantization ---
-// Rows: a half-warp per (row, block), eight values a lane, so a block's amax is four shuffles.
-// One pass over x: bound by its bytes.
+// The quotients m / 448 (scale) and 448 / m of N <= 16 blocks with maxima `m[i]` (bits), in one
+// division by the warp: lane 2 i holds the scale of block i, lane 2 i + 1 its reciprocal.
+template <int N>
+__device__ __forceinline__ float quotients(const uint32_t m[N], int lane) {
+  float v = 1.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (lane >> 1 == i) v = max_nan(__uint_as_float(m[i]), kFp8AmaxMin);
+  return lane & 1 ? __fdiv_rn(kFp8Max, v) : __fdiv_rn(v, kFp8Max);
+}
+
+// Rows: a warp takes eight rows of one 128-column block, four columns a lane (a row's maximum is
+// one warp reduction, the eight scales are neighbours). One pass over x, eight rows' loads in
+// flight: bound by its bytes.
+constexpr int kRowsWarp = 8;
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256)
 quant_rows_kernel(const T* __restrict__ x, int64_t ld_x, int rows, int cols, int nblk,
                   uint8_t* __restrict__ codes, int64_t ld_c, float* __restrict__ scales,
                   int64_t ld_s) {
-  const int sub = threadIdx.x & 15;
-  const int64_t items = (int64_t)rows * nblk;
-  const int64_t step = (int64_t)gridDim.x * 16;
-  // both halves of a warp take the same number of turns (the shuffles are warp-wide)
-  const int64_t first = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
-  const int64_t base = (int64_t)blockIdx.x * 16 + ((threadIdx.x >> 5) << 1);
-  for (int64_t o = 0; base + o < items; o += step) {
-    const int64_t it = first + o;
-    const bool on = it < items;
-    const int r = on ? (int)(it / nblk) : 0;
-    const int b = on ? (int)(it - (int64_t)r * nblk) : 0;
-    const int c = b * kBlk + sub * 8;
-    float v[8];
-    load8<T, VEC>(x + (int64_t)r * ld_x, c, on ? cols : 0, v);
-    float a = amax8(v);
+  const int lane = threadIdx.x & 31;
+  const int64_t items = (int64_t)((rows + kRowsWarp - 1) / kRowsWarp) * nblk;
+  const int64_t warps = (int64_t)gridDim.x * 8;
+  for (int64_t it = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); it < items; it += warps) {
+    const int rg = (int)(it / nblk), b = (int)(it - (int64_t)rg * nblk);
+    const int r0 = rg * kRowsWarp, H = cols - b * kBlk;
+    const T* src = x + (int64_t)r0 * ld_x + b * kBlk;
+    Four<T> raw[kRowsWarp];
 #pragma unroll
-    for (int s = 8; s > 0; s >>= 1) a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, s));
-    a = max_nan(a, kFp8AmaxMin);
-    if (!on) continue;
-    if (sub == 0) scales[(int64_t)b * ld_s + r] = __fdiv_rn(a, kFp8Max);
-    const uint2 q = encode8(v, __fdiv_rn(kFp8Max, a));
-    // the row pitch is a multiple of 16 bytes: the last vector of a row may run into its pad
-    if (c < cols) *reinterpret_cast<uint2*>(codes + (int64_t)r * ld_c + c) = q;
+    for (int i = 0; i < kRowsWarp; ++i)
+      raw[i] = raw4<T, VEC, false>(src + (r0 + i < rows ? i * ld_x : 0), 0, lane, 32,
+                                   r0 + i < rows ? H : 0);
+    uint32_t m[kRowsWarp];
+#pragma unroll
+    for (int i = 0; i < kRowsWarp; ++i) {
+      F2 v[2];
+      pairs(raw[i], v);
+      m[i] = __reduce_max_sync(0xffffffffu, amax4(v));
+    }
+    const float quot = quotients<kRowsWarp>(m, lane);
+    if ((lane & 1) == 0 && lane < 2 * kRowsWarp && r0 + (lane >> 1) < rows)
+      scales[(int64_t)b * ld_s + r0 + (lane >> 1)] = quot;
+    uint8_t* dst = codes + (int64_t)r0 * ld_c + b * kBlk;
+#pragma unroll
+    for (int i = 0; i < kRowsWarp; ++i) {
+      F2 v[2];
+      pairs(raw[i], v);
+      const float r = __shfl_sync(0xffffffffu, quot, 2 * i + 1);
+      if (r0 + i < rows) put_codes<VEC>(dst + i * ld_c, 0, lane, 32, H, encode4(v, r));
+    }
   }
 }
 
-// A 128 x 128 tile per CTA, an 8 x 8 piece per thread (rows 8 (tid / 16).., columns
-// 8 (tid % 16)..), in any of three forms from one read of the tile:
+// A 128 x 128 tile per CTA, sixteen rows a warp and four columns a lane, in any of three forms
+// from one read of the tile:
 //   ROWS    a scale per row          -> codes [rows][ld_c], scales [cols / 128][ld_s]
-//   COLS    a scale per column       -> codes_t [cols][ld_ct] (transposed through shared memory,
-//                                       8 bytes a write), scales_t [rows / 128][ld_st]
+//   COLS    a scale per column       -> codes_t [cols][ld_ct], scales_t [rows / 128][ld_st]: a
+//           lane's sixteen rows of a column are one 16-byte chunk of the transposed row, swizzled
+//           in shared memory so that neither the writes nor the reads of chunks conflict
 //   BLOCKS  one scale for the tile   -> codes, scales [rows / 128][ld_s]
 template <typename T, bool VEC, bool ROWS, bool COLS, bool BLOCKS>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 2)
 quant_tile_kernel(const T* __restrict__ x, int64_t ld_x, int rows, int cols,
                   uint8_t* __restrict__ codes, int64_t ld_c, float* __restrict__ scales,
                   int64_t ld_s, uint8_t* __restrict__ codes_t, int64_t ld_ct,
                   float* __restrict__ scales_t, int64_t ld_st) {
-  __shared__ float red[8][kBlk];
-  __shared__ __align__(16) uint8_t tile[COLS ? kBlk : 1][kBlk + 8];
-  const int sub = threadIdx.x & 15, rg = threadIdx.x >> 4, warp = threadIdx.x >> 5;
+  constexpr int R = 16;
+  __shared__ __align__(16) uint32_t red[8][kBlk];
+  __shared__ __align__(16) float inv[kBlk];
+  __shared__ __align__(16) uint8_t tile[COLS ? kBlk : 1][kBlk];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int cb = blockIdx.x, rb = blockIdx.y;
-  const int c = cb * kBlk + sub * 8, r0 = rb * kBlk + rg * 8;
-  float v[8][8];
+  const int r0 = rb * kBlk + w * R, H = cols - cb * kBlk;
+  const T* src = x + (int64_t)(r0 < rows ? r0 : 0) * ld_x + cb * kBlk;
+  Four<T> raw[R];
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    load8<T, VEC>(x + (int64_t)(r0 + i < rows ? r0 + i : 0) * ld_x, c, r0 + i < rows ? cols : 0,
-                  v[i]);
+  for (int i = 0; i < R; ++i)
+    raw[i] = raw4<T, VEC, false>(src + (r0 + i < rows ? i * ld_x : 0), 0, lane, 32,
+                                 r0 + i < rows ? H : 0);
+  uint32_t top[4] = {0u, 0u, 0u, 0u};   // the columns' maxima over the warp's rows
+  uint32_t m[ROWS ? R : 1];
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    F2 v[2];
+    pairs(raw[i], v);
+    if (ROWS) m[ROWS ? i : 0] = __reduce_max_sync(0xffffffffu, amax4(v));
+    top[0] = max(top[0], __float_as_uint(fabsf(v[0].x)));
+    top[1] = max(top[1], __float_as_uint(fabsf(v[0].y)));
+    top[2] = max(top[2], __float_as_uint(fabsf(v[1].x)));
+    top[3] = max(top[3], __float_as_uint(fabsf(v[1].y)));
+  }
+  uint8_t* dst = codes + (int64_t)r0 * ld_c + cb * kBlk;
   if (ROWS) {
+    const float quot = quotients<ROWS ? R : 1>(m, lane);
+    if ((lane & 1) == 0 && r0 + (lane >> 1) < rows)
+      scales[(int64_t)cb * ld_s + r0 + (lane >> 1)] = quot;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      float a = amax8(v[i]);
-#pragma unroll
-      for (int s = 8; s > 0; s >>= 1) a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, s));
-      a = max_nan(a, kFp8AmaxMin);
-      if (r0 + i < rows) {
-        if (sub == 0) scales[(int64_t)cb * ld_s + r0 + i] = __fdiv_rn(a, kFp8Max);
-        if (c < cols)
-          *reinterpret_cast<uint2*>(codes + (int64_t)(r0 + i) * ld_c + c) =
-              encode8(v[i], __fdiv_rn(kFp8Max, a));
-      }
+    for (int i = 0; i < R; ++i) {
+      F2 v[2];
+      pairs(raw[i], v);
+      const float r = __shfl_sync(0xffffffffu, quot, 2 * i + 1);
+      if (r0 + i < rows) put_codes<VEC>(dst + i * ld_c, 0, lane, 32, H, encode4(v, r));
     }
   }
-  if (COLS || BLOCKS) {
-    float a[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      a[j] = fabsf(v[0][j]);
+  for (int j = 0; j < 4; ++j) red[w][column<VEC>(0, j, lane, 32)] = top[j];
+  __syncthreads();
+  if (COLS) {
+    if (threadIdx.x < kBlk) {
+      uint32_t a = 0u;
 #pragma unroll
-      for (int i = 1; i < 8; ++i) a[j] = max_nan(a[j], fabsf(v[i][j]));
-      a[j] = max_nan(a[j], __shfl_xor_sync(0xffffffffu, a[j], 16));
-    }
-    if ((threadIdx.x & 16) == 0) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) red[warp][sub * 8 + j] = a[j];
+      for (int i = 0; i < 8; ++i) a = max(a, red[i][threadIdx.x]);
+      const float v = max_nan(__uint_as_float(a), kFp8AmaxMin);
+      inv[threadIdx.x] = __fdiv_rn(kFp8Max, v);
+      if ((int)threadIdx.x < H)
+        scales_t[(int64_t)rb * ld_st + cb * kBlk + threadIdx.x] = __fdiv_rn(v, kFp8Max);
     }
     __syncthreads();
-    if (COLS) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        float m = kFp8AmaxMin;
+    for (int j = 0; j < 4; ++j) {
+      const int c = column<VEC>(0, j, lane, 32);
+      const float r = inv[c];
+      uint32_t q[4];
 #pragma unroll
-        for (int w = 0; w < 8; ++w) m = max_nan(m, red[w][sub * 8 + j]);
-        if (rg == 0 && c + j < cols) scales_t[(int64_t)rb * ld_st + c + j] = __fdiv_rn(m, kFp8Max);
-        float col[8];
+      for (int g = 0; g < 4; ++g) {
+        float f[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) col[i] = v[i][j];
-        *reinterpret_cast<uint2*>(&tile[sub * 8 + j][rg * 8]) = encode8(col, __fdiv_rn(kFp8Max, m));
+        for (int i = 0; i < 4; ++i) f[i] = __fmul_rn(to_f32(raw[4 * g + i].e[j]), r);
+        q[g] = cvt4_e4m3(f[0], f[1], f[2], f[3]);
       }
-      __syncthreads();
-      for (int e = threadIdx.x; e < kBlk * 16; e += 256) {
-        const int cc = e >> 4, rr = (e & 15) * 8;
-        if (cb * kBlk + cc < cols && rb * kBlk + rr < rows)
-          *reinterpret_cast<uint2*>(codes_t + (int64_t)(cb * kBlk + cc) * ld_ct + rb * kBlk + rr) =
-              *reinterpret_cast<const uint2*>(&tile[cc][rr]);
-      }
+      const int at = w ^ ((VEC ? c >> 2 : c) & 7);
+      *reinterpret_cast<uint4*>(&tile[COLS ? c : 0][at * 16]) = make_uint4(q[0], q[1], q[2], q[3]);
     }
-    if (BLOCKS) {
-      float m = kFp8AmaxMin;
+    __syncthreads();
 #pragma unroll
-      for (int w = 0; w < 8; ++w)
+    for (int e = threadIdx.x; e < kBlk * 8; e += 256) {
+      const int c = e >> 3, k = e & 7, at = k ^ ((VEC ? c >> 2 : c) & 7);
+      // (the pitch is a multiple of 16: a chunk that holds a row lies inside it)
+      if (c < H && rb * kBlk + k * 16 < rows)
+        *reinterpret_cast<uint4*>(codes_t + (int64_t)(cb * kBlk + c) * ld_ct + rb * kBlk + k * 16) =
+            *reinterpret_cast<const uint4*>(&tile[COLS ? c : 0][at * 16]);
+    }
+  }
+  if (BLOCKS) {
+    uint32_t a = 0u;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) m = max_nan(m, red[w][sub * 8 + j]);
+    for (int i = 0; i < 8; ++i)
 #pragma unroll
-      for (int s = 8; s > 0; s >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, s));
-      if (threadIdx.x == 0) scales[(int64_t)rb * ld_s + cb] = __fdiv_rn(m, kFp8Max);
-      const float r = __fdiv_rn(kFp8Max, m);
+      for (int j = 0; j < 4; ++j) a = max(a, red[i][32 * j + lane]);
+    a = __reduce_max_sync(0xffffffffu, a);
+    const float v = max_nan(__uint_as_float(a), kFp8AmaxMin);
+    if (threadIdx.x == 0) scales[(int64_t)rb * ld_s + cb] = __fdiv_rn(v, kFp8Max);
+    const float r = __fdiv_rn(kFp8Max, v);
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (r0 + i < rows && c < cols)
-          *reinterpret_cast<uint2*>(codes + (int64_t)(r0 + i) * ld_c + c) = encode8(v[i], r);
+    for (int i = 0; i < R; ++i) {
+      F2 u[2];
+      pairs(raw[i], u);
+      if (r0 + i < rows) put_codes<VEC>(dst + i * ld_c, 0, lane, 32, H, encode4(u, r));
     }
   }
 }
@@ -199,34 +239,166 @@ constexpr uint32_t idesc_e4m3(int M, int N) {
   return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
 
+template <bool PAIR>
 __device__ __forceinline__ void umma_e4m3(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
                                           uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
+  if constexpr (PAIR)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
 }
 
-template <int N>
-__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t* r) {
-  if constexpr (N == 32) {
-    tc::tmem_ld32_nowait(taddr, r);
-  } else {
+// Arrive on `bar` (PAIR: on the barrier at this address in both CTAs) once the MMAs issued so far
+// have completed.
+template <bool PAIR>
+__device__ __forceinline__ void umma_commit(uint64_t* bar) {
+  if constexpr (PAIR)
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
-        "%11, %12, %13, %14, %15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-          "=r"(r[14]), "=r"(r[15])
-        : "r"(taddr));
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
+        " [%0], %1;" ::"r"(tc::smem_u32(bar)),
+        "h"((uint16_t)3)
+        : "memory");
+  else
+    tc::umma_commit(bar);
+}
+
+template <bool PAIR>
+__device__ __forceinline__ void tmem_alloc(uint32_t* dst, uint32_t ncols) {
+  if constexpr (PAIR) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     tc::smem_u32(dst)),
+                 "r"(ncols));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+  } else {
+    tc::tmem_alloc(dst, ncols);
   }
 }
 
-__device__ __forceinline__ void copy4(float* to, const float* from) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(tc::smem_u32(to)), "l"(from)
+template <bool PAIR>
+__device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t ncols) {
+  if constexpr (PAIR)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols));
+  else
+    tc::tmem_dealloc(taddr, ncols);
+}
+
+// This shared-memory address in the pair's first CTA.
+__device__ __forceinline__ uint32_t leader_u32(const void* ptr) {
+  uint32_t a;
+  asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(tc::smem_u32(ptr)));
+  return a;
+}
+
+// (What it orders is the reads of TMEM before it, which tcgen05.wait::ld and the fence have
+// completed; release.cluster would add a memory barrier of some thousand cycles.)
+__device__ __forceinline__ void arrive_leader(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(leader_u32(bar))
                : "memory");
 }
+
+// A box into this CTA's shared memory, its bytes counted on the first CTA's barrier.
+__device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, uint32_t bar,
+                                                 int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2"
+      " [%0], [%1, {%3, %4}], [%2];" ::"r"(tc::smem_u32(dst)),
+      "l"((uint64_t)map), "r"(bar), "r"(x), "r"(y)
+      : "memory");
+}
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
+                   : "memory");
+}
+
+// acc += (d0, d1) s, and acc += ((d0, d1) b) s, on pairs
+__device__ __forceinline__ void fold(uint64_t& acc, uint32_t d0, uint32_t d1, uint64_t s) {
+  asm("{\n\t.reg .b64 d;\n\tmov.b64 d, {%1, %2};\n\tfma.rn.f32x2 %0, d, %3, %0;\n\t}"
+      : "+l"(acc)
+      : "r"(d0), "r"(d1), "l"(s));
+}
+__device__ __forceinline__ void fold2(uint64_t& acc, uint32_t d0, uint32_t d1, uint64_t b,
+                                      uint64_t s) {
+  asm("{\n\t.reg .b64 d;\n\tmov.b64 d, {%1, %2};\n\tmul.rn.f32x2 d, d, %3;\n\t"
+      "fma.rn.f32x2 %0, d, %4, %0;\n\t}"
+      : "+l"(acc)
+      : "r"(d0), "r"(d1), "l"(b), "l"(s));
+}
+
+// Four bytes to shared memory, or zero.
+__device__ __forceinline__ void copy4(float* to, const float* from, bool on) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(tc::smem_u32(to)),
+               "l"(from), "r"(on ? 4 : 0)
+               : "memory");
+}
+
+// 64 columns of this thread's lane; no wait.
+__device__ __forceinline__ void tmem_ld64(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
+      "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, "
+      "%18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, "
+      "%34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, "
+      "%50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63 "
+      "}, [%64];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+        "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]), "=r"(r[33]), "=r"(r[34]),
+        "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]), "=r"(r[41]),
+        "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]),
+        "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
+        "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]),
+        "=r"(r[63])
+      : "r"(taddr));
+}
+
+// The warp's wait for a phase: one poll by all lanes where the phase is there already (control
+// stays uniform over the warp, so what follows is issued from uniform registers); bounded as
+// tc::mbar_wait.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* err, int code) {
+  if (__all_sync(0xffffffffu, tc::mbar_try_wait(bar, parity))) return true;
+  const long long t0 = clock64();
+  for (uint32_t i = 1;; ++i) {
+    if (__all_sync(0xffffffffu, tc::mbar_try_wait(bar, parity))) return true;
+    if ((i & 255u) == 0) {
+      const bool late = clock64() - t0 > tc::kWaitCycles;
+      if (late) atomicCAS(err, 0, code);
+      if (__any_sync(0xffffffffu, late || *(volatile int*)err != 0)) return false;
+    }
+  }
+}
+
+__device__ __forceinline__ bool elect_one() {
+  uint32_t on;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(on));
+  return on != 0;
+}
+
+// A place in a ring of N barriers and the parity of its current phase.
+template <int N>
+struct Turn {
+  uint32_t i = 0, phase = 0;
+  __device__ __forceinline__ void next() {
+    if (++i == N) {
+      i = 0;
+      phase ^= 1;
+    }
+  }
+};
+
+constexpr int kRing = 8;   // k-blocks whose scales are in shared memory
 
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(tc::smem_u32(bar)) : "memory");
@@ -252,12 +424,14 @@ __device__ __forceinline__ void tile_at(const GemmArgs& p, int t, int& m, int& n
 // An output row's values of one warp column range, element by element (rows that TMA cannot
 // write, and sums into what is there).
 template <typename T, int CW>
-__device__ __forceinline__ void store_row(const GemmArgs& p, int m, int n0, const F2* acc) {
+__device__ __forceinline__ void store_row(const GemmArgs& p, int m, int n0,
+                                          const uint64_t* acc) {
   if (m >= p.M) return;
   T* o = reinterpret_cast<T*>(p.out) + (int64_t)m * p.ld_o + n0;
 #pragma unroll
   for (int c = 0; c < CW; ++c) {
-    const float v = c & 1 ? acc[c >> 1].y : acc[c >> 1].x;
+    const F2 a = f2_of(acc[c >> 1]);
+    const float v = c & 1 ? a.y : a.x;
     if (n0 + c < p.N) o[c] = from_f32<T>(p.accumulate ? v + to_f32(o[c]) : v);
   }
 }
@@ -268,32 +442,33 @@ __device__ __forceinline__ void store_row(const GemmArgs& p, int m, int n0, cons
 // output. Two buffers a warp: a box is written while the last one is still being read.
 template <typename T, int CW>
 __device__ __forceinline__ void store_boxes(const GemmArgs& p, uint8_t* stage, int& buf, int lane,
-                                            int m0, int n0, const F2* acc) {
+                                            int m0, int n0, const uint64_t* acc) {
   constexpr int BW = 128 / sizeof(T);  // columns of a box
   if (m0 >= p.M) return;
 #pragma unroll
   for (int c0 = 0; c0 < CW; c0 += BW) {
     if (n0 + c0 < p.N) {
-      uint8_t* b = stage + buf * 4096;
+      uint8_t* box = stage + buf * 4096;
       if (lane == 0) tc::bulk_wait_read<1>();
       __syncwarp();
 #pragma unroll
       for (int c = 0; c < 8; ++c) {
         uint4 v;
         if constexpr (sizeof(T) == 2) {
-          const F2* a = acc + (c0 + c * 8) / 2;
-          v = make_uint4(f2_pack<T>(a[0]), f2_pack<T>(a[1]), f2_pack<T>(a[2]), f2_pack<T>(a[3]));
+          const uint64_t* a = acc + (c0 + c * 8) / 2;
+          v = make_uint4(f2_pack<T>(f2_of(a[0])), f2_pack<T>(f2_of(a[1])), f2_pack<T>(f2_of(a[2])),
+                         f2_pack<T>(f2_of(a[3])));
         } else {
-          const F2* a = acc + (c0 + c * 4) / 2;
-          v = make_uint4(__float_as_uint(a[0].x), __float_as_uint(a[0].y),
-                         __float_as_uint(a[1].x), __float_as_uint(a[1].y));
+          const F2 a = f2_of(acc[(c0 + c * 4) / 2]), b = f2_of(acc[(c0 + c * 4) / 2 + 1]);
+          v = make_uint4(__float_as_uint(a.x), __float_as_uint(a.y), __float_as_uint(b.x),
+                         __float_as_uint(b.y));
         }
-        *reinterpret_cast<uint4*>(b + lane * 128 + ((c ^ (lane & 7)) << 4)) = v;
+        *reinterpret_cast<uint4*>(box + lane * 128 + ((c ^ (lane & 7)) << 4)) = v;
       }
       tc::fence_proxy_async_shared();
       __syncwarp();
       if (lane == 0) {
-        tma_store_2d(&p.o, b, n0 + c0, m0);
+        tma_store_2d(&p.o, box, n0 + c0, m0);
         tc::bulk_commit();
       }
       buf ^= 1;
@@ -318,22 +493,27 @@ __device__ __forceinline__ void regs_inc() {
 // issues the MMAs of a k-block into the next accumulator of the ring, warps 4-11 fold it: warp
 // w reads TMEM lanes 32 (w % 4).. (its rows) and half of the columns.
 // BROWS: B has a scale per row and k-block instead of one per 128 x 128.
-template <int BN, bool BROWS>
+// PAIR: two CTAs of a cluster share a tile of 256 rows. Each loads its 128 rows of A and half of
+// B's columns, the first one issues MMAs over both (cta_group::2: each SM multiplies its rows by
+// all columns), and each folds its own rows: half the bytes of B from L2 and in shared memory.
+template <int BN, bool BROWS, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant__ GemmArgs p,
                                                            int dtype) {
   constexpr int kSlots = kTmemCols / BN;
-  constexpr uint32_t kStage = (kBM + BN) * kBlk;
+  constexpr int kBRows = PAIR ? BN / 2 : BN;  // rows of B this CTA loads
+  constexpr uint32_t kStage = (kBM + kBRows) * kBlk;
+  uint32_t rank = 0;
+  if (PAIR) asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  const int first = PAIR ? blockIdx.x >> 1 : blockIdx.x, step = PAIR ? gridDim.x >> 1 : gridDim.x;
   constexpr int kStages = kPipeBytes / kStage;
   constexpr int CW = BN / 2;  // columns per epilogue warp
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages], tfull[4], tempty[4], last;
   __shared__ uint32_t tmem_base;
-  constexpr int CH = BN == 256 ? 16 : 32;
-  // k-blocks whose scales are on their way, and the ring's entries
-  constexpr int kAhead = BROWS && BN == 256 ? 2 : 4, kRing = kAhead + 1;
-  constexpr int kRow = 32 + (BROWS ? CW : 4);   // a k-block's scales of a warp: rows, columns
-  __shared__ __align__(16) float ring_s[kEpiWarps][kRing * kRow];
+  // a k-block's scales: the rows', and the weight blocks' or the columns'
+  __shared__ __align__(16) float ring_s[kRing][kBM + (BROWS ? BN : 4)];
+  __shared__ __align__(8) uint64_t sfull[kRing], sempty[kRing];
   uint8_t* stage = smem + kStages * kStage;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -343,159 +523,203 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
     }
     for (int i = 0; i < kSlots; ++i) {
       tc::mbar_init(&tfull[i], 1);
-      tc::mbar_init(&tempty[i], kEpiWarps);
+      tc::mbar_init(&tempty[i], (PAIR ? 2 : 1) * kEpiWarps);
+    }
+    for (int i = 0; i < kRing; ++i) {
+      tc::mbar_init(&sfull[i], 32);
+      tc::mbar_init(&sempty[i], kEpiWarps);
     }
     tc::mbar_init(&last, 1);
     tc::fence_barrier_init();
   }
-  if (warp == 1) tc::tmem_alloc(&tmem_base, kTmemCols);
+  if (warp == 1) tmem_alloc<PAIR>(&tmem_base, kTmemCols);
   tc::fence_before_sync();
   __syncthreads();
+  if (PAIR) cluster_sync();
   tc::fence_after_sync();
   const uint32_t tmem = tmem_base;
   const int tiles = p.mt * p.nt;
 
   if (warp < 4) {
     if (BN == 256) regs_dec<72>();
-    if (warp == 0 && lane == 0) {
-      uint32_t it = 0;
+    if (warp == 0) {
+      const bool one = elect_one();
+      Turn<kStages> at;
+      uint32_t issued = 0;
       bool ok = true;
-      for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
+      for (int t = first; ok && t < tiles; t += step) {
         int m, n;
         tile_at(p, t, m, n);
-        for (int k = 0; k < p.kb; ++k, ++it) {
-          const int s = it % kStages;
-          if (it >= kStages && !tc::mbar_wait(&empty[s], (it / kStages - 1) & 1, p.err, 1)) {
+        for (int k = 0; k < p.kb; ++k) {
+          const uint32_t s = at.i;
+          // (a fresh barrier passes for the phase before its first)
+          if (!warp_wait(&empty[s], at.phase ^ 1, p.err, 1)) {
             ok = false;
             break;
           }
-          uint8_t* st = smem + s * kStage;
-          tc::mbar_arrive_expect_tx(&full[s], kStage);
-          tc::tma_load_2d(st, &p.a, &full[s], k * kBlk, m * kBM);
-          tc::tma_load_2d(st + kBM * kBlk, &p.b, &full[s], k * kBlk, n * BN);
+          if (one) {
+            uint8_t* st = smem + s * kStage;
+            if (!PAIR || rank == 0)
+              tc::mbar_arrive_expect_tx(&full[s], (PAIR ? 2 : 1) * kStage);
+            if (PAIR) {
+              const uint32_t bar = leader_u32(&full[s]);
+              tma_load_2d_pair(st, &p.a, bar, k * kBlk, (2 * m + rank) * kBM);
+              tma_load_2d_pair(st + kBM * kBlk, &p.b, bar, k * kBlk, n * BN + rank * kBRows);
+            } else {
+              tc::tma_load_2d(st, &p.a, &full[s], k * kBlk, m * kBM);
+              tc::tma_load_2d(st + kBM * kBlk, &p.b, &full[s], k * kBlk, n * BN);
+            }
+          }
+          __syncwarp();
+          at.next();
+          ++issued;
         }
       }
-      // a copy still in flight after a timeout must land before the CTA's memory goes
-      if (!ok)
-        for (uint32_t i = it > kStages ? it - kStages : 0; i < it; ++i)
-          tc::mbar_wait(&full[i % kStages], (i / kStages) & 1, nullptr, 0);
-    } else if (warp == 1 && lane == 0) {
-      constexpr uint32_t id = idesc_e4m3(kBM, BN);
-      uint32_t it = 0;
+      // a copy still in flight after a timeout must land before the CTA's memory goes (a pair's
+      // second CTA cannot see its own land: it waits far longer than a copy takes)
+      if (!ok && one) {
+        if (PAIR) {
+          const long long t0 = clock64();
+          while (clock64() - t0 < 20000000ll) {}
+        } else {
+          for (uint32_t i = issued > kStages ? issued - kStages : 0; i < issued; ++i)
+            tc::mbar_wait(&full[i % kStages], (i / kStages) & 1, nullptr, 0);
+        }
+      }
+    } else if (warp == 1 && rank == 0) {
+      // The tensor core takes 256 or 512 cycles for a k-block: the loop that feeds it has to be
+      // shorter, so its control and operands are uniform over the warp and one lane issues.
+      constexpr uint32_t id = idesc_e4m3(PAIR ? 2 * kBM : kBM, BN);
+      const bool one = elect_one();
+      const uint32_t base = tc::smem_u32(smem);
+      const uint64_t da0 = tc::umma_desc_k_sw128(base),
+                     db0 = tc::umma_desc_k_sw128(base + kBM * kBlk);
+      Turn<kStages> at;
+      Turn<kSlots> acc;
       bool ok = true;
-      for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
-        for (int k = 0; k < p.kb; ++k, ++it) {
-          const int s = it % kStages, sl = it % kSlots;
-          if ((it >= kSlots && !tc::mbar_wait(&tempty[sl], (it / kSlots - 1) & 1, p.err, 2)) ||
-              !tc::mbar_wait(&full[s], (it / kStages) & 1, p.err, 3)) {
+      for (int t = first; ok && t < tiles; t += step) {
+        for (int k = 0; k < p.kb; ++k) {
+          if (!warp_wait(&tempty[acc.i], acc.phase ^ 1, p.err, 2) ||
+              !warp_wait(&full[at.i], at.phase, p.err, 3)) {
             ok = false;
             break;
           }
           tc::fence_after_sync();
-          const uint32_t a = tc::smem_u32(smem + s * kStage);
-          const uint64_t da = tc::umma_desc_k_sw128(a),
-                         db = tc::umma_desc_k_sw128(a + kBM * kBlk);
+          const uint64_t off = at.i * (kStage >> 4);
+          const uint32_t d = tmem + acc.i * BN;
+          if (one) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j)  // 32 values (32 bytes) of k per instruction
-            umma_e4m3(tmem + sl * BN, da + 2 * j, db + 2 * j, id, j > 0);
-          tc::umma_commit(&empty[s]);
-          tc::umma_commit(&tfull[sl]);
+            for (int j = 0; j < 4; ++j)  // 32 values (32 bytes) of k per instruction
+              umma_e4m3<PAIR>(d, da0 + off + 2 * j, db0 + off + 2 * j, id, j > 0);
+            umma_commit<PAIR>(&empty[at.i]);
+            umma_commit<PAIR>(&tfull[acc.i]);
+          }
+          __syncwarp();
+          at.next();
+          acc.next();
         }
       }
-      tc::umma_commit(&last);
-      tc::mbar_wait(&last, 0, p.err, 4);
+      if (one) {
+        umma_commit<PAIR>(&last);
+        tc::mbar_wait(&last, 0, p.err, 4);
+      }
+    } else if (warp == 2) {
+      // Scales: copied to the ring up to kRing k-blocks ahead of the fold (a load from L2 takes
+      // longer than the MMAs of a k-block); each lane's arrival on sfull follows its copies.
+      Turn<kRing> at;
+      bool ok = true;
+      for (int t = first; ok && t < tiles; t += step) {
+        int mi, ni;
+        tile_at(p, t, mi, ni);
+        const int m = (PAIR ? 2 * mi + rank : mi) * kBM + lane;
+        const float* sa = p.sa + m;
+        const float* sb = p.sb;
+        int n = ni * BN;
+        if (BROWS) {
+          n += lane;
+          sb += n;
+        } else {   // lane i: the weight block of columns 128 i .. of the tile
+          n += kBlk * lane;
+          sb += n / kBlk * p.sb_n;
+        }
+        for (int k = 0; k < p.kb; ++k, at.next()) {
+          const uint32_t e = at.i;
+          ok = warp_wait(&sempty[e], at.phase ^ 1, p.err, 8);
+          if (!ok) break;
+          float* to = ring_s[e];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) copy4(to + 32 * i + lane, sa + 32 * i, m + 32 * i < p.M);
+          if (BROWS) {
+#pragma unroll
+            for (int i = 0; i < BN / 32; ++i)
+              copy4(to + kBM + 32 * i + lane, sb + 32 * i, n + 32 * i < p.N);
+          } else if (lane < BN / kBlk) {
+            copy4(to + kBM + lane, sb, n < p.N);
+          }
+          asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(
+                           tc::smem_u32(&sfull[e]))
+                       : "memory");
+          sa += p.ld_sa;
+          sb += p.sb_k;
+        }
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
     }
   } else {
     if (BN == 256) regs_inc<216>();
-    const int q = warp & 3, half = (warp - 4) >> 2;
-    const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16) + half * CW;
-    // The scales of the k-block kAhead ahead (of the next tile's, at a tile's end) are copied to
-    // the warp's ring while this one is folded: a load from L2 takes longer than a k-block.
-    float* ring = ring_s[warp - 4];
-    int pt = blockIdx.x, pk = 0, pslot = 0, pn = 0;
-    const float *psa = nullptr, *psb = nullptr;
-    auto prefetch = [&]() {
-      if (pt < tiles) {
-        if (pk == 0) {
-          int mi, ni;
-          tile_at(p, pt, mi, ni);
-          const int m = mi * kBM + q * 32 + lane;
-          psa = p.sa + (m < p.M ? m : 0);
-          pn = ni * BN + half * CW;
-          // CW is 64 or 128 and pn a multiple of it: a warp's columns lie in one weight block
-          psb = BROWS ? p.sb + lane : p.sb + min(pn, p.N - 1) / kBlk * p.sb_n;
-        }
-        float* to = ring + pslot * kRow;
-        copy4(to + lane, psa);
-        if (BROWS) {
-#pragma unroll
-          for (int i = 0; i < CW / 32; ++i)
-            copy4(to + 32 + 32 * i + lane, psb + (pn + 32 * i + lane < p.N ? pn + 32 * i : -lane));
-        } else if (lane == 0) {
-          copy4(to + 32, psb);
-        }
-        psa += p.ld_sa;
-        psb += p.sb_k;
-        if (++pk == p.kb) {
-          pk = 0;
-          pt += gridDim.x;
-        }
-        pslot = pslot + 1 == kRing ? 0 : pslot + 1;
-      }
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    };
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) prefetch();
-    uint32_t it = 0;
-    int buf = 0, islot = 0;
+    const int q = warp & 3, part = (warp - 4) >> 2;
+    const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16) + part * CW;
+    Turn<kSlots> slot;
+    Turn<kRing> at;
+    int buf = 0;
     bool ok = true;
-    for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
+    for (int t = first; ok && t < tiles; t += step) {
       int mi, ni;
       tile_at(p, t, mi, ni);
-      const int m = mi * kBM + q * 32 + lane, n0 = ni * BN + half * CW;
-      F2 acc[CW / 2];
+      const int m = (PAIR ? 2 * mi + rank : mi) * kBM + q * 32 + lane, n0 = ni * BN + part * CW;
+      uint64_t acc[CW / 2];   // pairs of float32, in registers as the packed operations take them
 #pragma unroll
-      for (int c = 0; c < CW / 2; ++c) acc[c] = f2_same(0.f);
-      for (int k = 0; k < p.kb; ++k, ++it) {
-        const int sl = it % kSlots;
-        asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
-        ok = tc::mbar_wait(&tfull[sl], (it / kSlots) & 1, p.err, 5);
-        ok = __all_sync(0xffffffffu, ok);
+      for (int c = 0; c < CW / 2; ++c) acc[c] = 0;
+      for (int k = 0; k < p.kb; ++k) {
+        const uint32_t sl = slot.i, e = at.i;
+        ok = warp_wait(&sfull[e], at.phase, p.err, 7) &&
+             warp_wait(&tfull[sl], slot.phase, p.err, 5);
         if (!ok) break;
-        __syncwarp();   // the other lanes' copies
         tc::fence_after_sync();
-        const float* sc = ring + islot * kRow;
-        islot = islot + 1 == kRing ? 0 : islot + 1;
-        const float s = BROWS ? sc[lane] : sc[lane] * sc[32];
-        const float* sbw = sc + 32;
-        // CH columns are folded while the next are on their way from TMEM; the accumulator is
-        // given back before the last ones are folded
-        uint32_t r[2][CH];
-        tmem_ld<CH>(lanes + sl * BN, r[0]);
+        slot.next();
+        at.next();
+        float s = ring_s[e][q * 32 + lane];
+        if (!BROWS) s *= ring_s[e][kBM + part * CW / kBlk];
+        const uint64_t s2 = f2_bits(f2_same(s));
+        const float* sbw = ring_s[e] + kBM + part * CW;
+        uint32_t r[64];
 #pragma unroll
-        for (int c = 0; c < CW / CH; ++c) {
+        for (int c = 0; c < CW / 64; ++c) {
+          tmem_ld64(lanes + sl * BN + 64 * c, r);
           tc::tmem_wait_ld();
-          if (c + 1 < CW / CH) {
-            tmem_ld<CH>(lanes + sl * BN + CH * (c + 1), r[(c + 1) & 1]);
-          } else {
+          if (c + 1 == CW / 64) {
+            // the accumulator is given back before its last columns are folded
             tc::fence_before_sync();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&tempty[sl]);
+            if (lane == 0) {
+              if (PAIR) arrive_leader(&tempty[sl]);
+              else mbar_arrive(&tempty[sl]);
+            }
           }
-          const uint32_t* d = r[c & 1];
 #pragma unroll
-          for (int j = 0; j < CH / 2; ++j) {
-            F2 v = {__uint_as_float(d[2 * j]), __uint_as_float(d[2 * j + 1])};
-            if (BROWS) v = f2_mul(v, *reinterpret_cast<const F2*>(sbw + (BROWS ? CH * c + 2 * j : 0)));
-            F2& to = acc[CH / 2 * c + j];
-            to = f2_fma(v, f2_same(s), to);
+          for (int j = 0; j < 32; ++j) {
+            if (BROWS)
+              fold2(acc[32 * c + j], r[2 * j], r[2 * j + 1],
+                    *reinterpret_cast<const uint64_t*>(sbw + (BROWS ? 64 * c + 2 * j : 0)), s2);
+            else
+              fold(acc[32 * c + j], r[2 * j], r[2 * j + 1], s2);
           }
         }
-        __syncwarp();   // (BROWS: every lane has read the ring's entry)
-        prefetch();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sempty[e]);
       }
       if (ok) {
-        uint8_t* st = stage + (warp - 4) * 8192;
+        uint8_t* st = stage + (warp - 4) * 2 * 4096;
         const int m0 = m - lane;
         if (p.boxes) {
           if (dtype == BF16) store_boxes<__nv_bfloat16, CW>(p, st, buf, lane, m0, n0, acc);
@@ -509,12 +733,17 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
       }
     }
     if (lane == 0) tc::bulk_wait_all();
-    asm volatile("cp.async.wait_all;" ::: "memory");
   }
   tc::fence_before_sync();
   __syncthreads();
+  if (PAIR) {
+    // the second CTA stays until the pair's last commit has arrived here too
+    if (rank == 1 && threadIdx.x == 0) tc::mbar_wait(&last, 0, p.err, 9);
+    __syncwarp();
+    cluster_sync();   // (the other CTA's MMAs, commits and arrivals are over)
+  }
   tc::fence_after_sync();
-  if (warp == 1) tc::tmem_dealloc(tmem, kTmemCols);
+  if (warp == 1) tmem_dealloc<PAIR>(tmem, kTmemCols);
 }
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
@@ -567,27 +796,46 @@ static bool out_map(CUtensorMap* m, void* base, int dtype, int M, int N, int64_t
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int BN, bool BROWS>
-static int launch_gemm(GemmArgs& p, int dtype, cudaStream_t st) {
-  constexpr uint32_t kStage = (kBM + BN) * kBlk;
+template <int BN, bool BROWS, bool PAIR>
+static int launch_gemm(GemmArgs& p, const void* b, int64_t ldb, int dtype, cudaStream_t st) {
+  constexpr int kBRows = PAIR ? BN / 2 : BN;
+  constexpr uint32_t kStage = (kBM + kBRows) * kBlk;
   constexpr uint32_t smem = kPipeBytes / kStage * kStage + kStageBytes + 1024;
-  auto kern = gemm_kernel<BN, BROWS>;
+  auto kern = gemm_kernel<BN, BROWS, PAIR>;
+  if (!codes_map(&p.b, b, p.N, p.K, ldb, kBRows)) return GSQ_ECUDA;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) !=
       cudaSuccess)
     return GSQ_ECUDA;
   if (BN == 256) {
-    // the split above is only right for the register count it was made for
+    // the register split is only right for the register count it was made for
     cudaFuncAttributes at;
     if (cudaFuncGetAttributes(&at, kern) != cudaSuccess) return GSQ_ECUDA;
     if (at.numRegs != kLaunchRegs) return GSQ_ENOTSUP;
   }
-  p.mt = (p.M + kBM - 1) / kBM;
+  constexpr int rows = PAIR ? 2 * kBM : kBM;
+  p.mt = (p.M + rows - 1) / rows;
   p.nt = (p.N + BN - 1) / BN;
-  p.group = 16;
+  p.group = 16 / (PAIR ? 2 : 1);
   const int64_t tiles = (int64_t)p.mt * p.nt;
   if (tiles > INT32_MAX / 2) return GSQ_EINVAL;
-  const int grid = (int)(tiles < num_sms() ? tiles : num_sms());
-  kern<<<grid, kThreads, smem, st>>>(p, dtype);
+  const int most = num_sms() / (PAIR ? 2 : 1);
+  const int n = (int)(tiles < most ? tiles : most);
+  if (!PAIR) {
+    kern<<<n, kThreads, smem, st>>>(p, dtype);
+  } else {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2 * n);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = 2;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, kern, p, dtype) != cudaSuccess) return GSQ_ECUDA;
+  }
   GSQ_CHECK_LAUNCH();
   return GSQ_OK;
 }
@@ -596,11 +844,11 @@ template <typename T>
 static int quant_launch(const T* x, int rows, int cols, int64_t ld_x, uint8_t* codes, int64_t ld_c,
                         float* scales, int64_t ld_s, uint8_t* codes_t, int64_t ld_ct,
                         float* scales_t, int64_t ld_st, bool blocks, cudaStream_t st) {
-  const bool vec = (uintptr_t)x % 16 == 0 && ld_x * sizeof(T) % 16 == 0;
+  const bool vec = (uintptr_t)x % 16 == 0 && ld_x * sizeof(T) % 16 == 0 && cols % 4 == 0;
   const int cb = (cols + kBlk - 1) / kBlk, rb = (rows + kBlk - 1) / kBlk;
   if (!blocks && !codes_t) {
-    const int64_t items = (int64_t)rows * cb;
-    int64_t g = (items + 15) / 16;
+    const int64_t items = (int64_t)((rows + kRowsWarp - 1) / kRowsWarp) * cb;
+    int64_t g = (items + 7) / 8;
     const int64_t cap = (int64_t)num_sms() * 32;
     if (g > cap) g = cap;
     if (vec) quant_rows_kernel<T, true><<<(unsigned)g, 256, 0, st>>>(x, ld_x, rows, cols, cb, codes, ld_c, scales, ld_s);
@@ -721,16 +969,7 @@ extern "C" int gsq_fp8_gemm(int M, int N, int K, const void* a, int64_t lda, con
                     accumulate, err))
     return GSQ_EINVAL;
   fp8::GemmArgs p;
-  // Tile width by the rounds that the busiest CTA walks: a 256-wide tile costs two 128-wide ones
-  // but loads its A rows once (4094 x 896 x 4864: 128 wide tiles are one round of 148 SMs, 224
-  // narrow ones two halves; 4864 x 896 x 4094: 152 wide tiles are two rounds, 266 narrow ones two
-  // halves).
-  const int64_t mt = (M + 127) / 128;
-  const auto rounds = [&](int bn) { return (mt * ((N + bn - 1) / bn) + num_sms() - 1) / num_sms(); };
-  const bool wide = 2 * rounds(256) <= rounds(128) + (rounds(128) >= 8 ? 1 : 0);
-  if (!fp8::codes_map(&p.a, a, M, K, lda, fp8::kBM) ||
-      !fp8::codes_map(&p.b, b, N, K, ldb, wide ? 256 : 128))
-    return GSQ_ECUDA;
+  if (!fp8::codes_map(&p.a, a, M, K, lda, fp8::kBM)) return GSQ_ECUDA;
   p.M = M;
   p.N = N;
   p.K = K;
@@ -747,10 +986,25 @@ extern "C" int gsq_fp8_gemm(int M, int N, int K, const void* a, int64_t lda, con
   if (p.boxes && !fp8::out_map(&p.o, out, dtype, M, N, ld_out)) return GSQ_ECUDA;
   p.err = err;
   cudaStream_t st = (cudaStream_t)stream;
-  if (sb_rows) return wide ? fp8::launch_gemm<256, true>(p, dtype, st)
-                           : fp8::launch_gemm<128, true>(p, dtype, st);
-  return wide ? fp8::launch_gemm<256, false>(p, dtype, st)
-              : fp8::launch_gemm<128, false>(p, dtype, st);
+  // Tile by the time of the rounds that the busiest SM walks: 256 x 256 of a pair, 256 x 128 of a
+  // pair, or 128 x 128 of one SM. A k-block of the narrow tiles takes 0.64 and 0.7 of the wide
+  // one's time (8191 x 8192 x 4096: 251, 330 and 365 us), so they are taken where they need
+  // fewer rounds (4864 x 896 x 4094: 76 wide tiles are two rounds of 74 pairs, 133 narrow ones
+  // two of 0.64).
+  const auto rounds = [&](int rows, int bn, int sms) {
+    return (double)(((int64_t)((M + rows - 1) / rows) * ((N + bn - 1) / bn) * sms + num_sms() - 1) /
+                    num_sms());
+  };
+  const double r256 = rounds(256, 256, 2), r128 = 0.64 * rounds(256, 128, 2),
+               r1 = 0.7 * rounds(128, 128, 1);
+  const int pick = r256 <= r128 && r256 <= r1 ? 0 : (r128 <= r1 ? 1 : 2);
+  if (sb_rows)
+    return pick == 0   ? fp8::launch_gemm<256, true, true>(p, b, ldb, dtype, st)
+           : pick == 1 ? fp8::launch_gemm<128, true, true>(p, b, ldb, dtype, st)
+                       : fp8::launch_gemm<128, true, false>(p, b, ldb, dtype, st);
+  return pick == 0   ? fp8::launch_gemm<256, false, true>(p, b, ldb, dtype, st)
+         : pick == 1 ? fp8::launch_gemm<128, false, true>(p, b, ldb, dtype, st)
+                     : fp8::launch_gemm<128, false, false>(p, b, ldb, dtype, st);
 }
 
 extern "C" int gsq_fp8_linear(const void* x, int dtype, int M, int K, int64_t ld_x,

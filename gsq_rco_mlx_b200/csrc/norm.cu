@@ -77,57 +77,6 @@ __device__ __forceinline__ float team_sum(float v, float (*red)[32], int& turn) 
   return warp_sum(r[lane]);
 }
 
-// Columns are dealt in fours: column j < 4 of a thread's chunk q is one of four neighbours (VEC:
-// chunks go round the team; a warp's chunk is 128 columns), or goes round the team by itself.
-template <bool VEC>
-__device__ __forceinline__ int column(int q, int j, int t, int tpr) {
-  return VEC ? (q * tpr + t) * 4 + j : (q * 4 + j) * tpr + t;
-}
-
-// Chunk q of a row as it lies in memory; columns from H on are zero. VEC: H is a multiple of 4
-// and the row starts on 8 (16-bit types) or 16 bytes. PAD: the row has room for the whole team's
-// columns, so it may be read past H.
-template <typename T>
-struct alignas(4 * sizeof(T)) Four {
-  T e[4];
-};
-
-template <typename T, bool VEC, bool PAD>
-__device__ __forceinline__ Four<T> raw4(const T* row, int q, int t, int tpr, int H) {
-  const int c0 = column<VEC>(q, 0, t, tpr);
-  Four<T> v;
-  if constexpr (VEC) {
-    if constexpr (sizeof(T) == 2) {
-      uint2 r = make_uint2(0u, 0u);
-      if (c0 < H) r = *reinterpret_cast<const uint2*>(row + c0);
-      *reinterpret_cast<uint2*>(&v) = r;
-    } else {
-      float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (c0 < H) r = *reinterpret_cast<const float4*>(row + c0);
-      *reinterpret_cast<float4*>(&v) = r;
-    }
-  } else {
-    const T zero = from_f32<T>(0.f);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int col = c0 + j * tpr;
-      if (PAD) {
-        v.e[j] = row[col];
-        v.e[j] = col < H ? v.e[j] : zero;
-      } else {
-        v.e[j] = col < H ? row[col] : zero;
-      }
-    }
-  }
-  return v;
-}
-
-template <typename T>
-__device__ __forceinline__ void pairs(const Four<T>& r, F2 v[2]) {
-  v[0] = {to_f32(r.e[0]), to_f32(r.e[1])};
-  v[1] = {to_f32(r.e[2]), to_f32(r.e[3])};
-}
-
 template <typename T, bool VEC, bool PAD>
 __device__ __forceinline__ void get4(const T* row, int q, int t, int tpr, int H, F2 v[2]) {
   pairs(raw4<T, VEC, PAD>(row, q, t, tpr, H), v);
@@ -290,8 +239,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) fwd_kernel(const __gr
         float num = 1.f, den = 1.f;
 #pragma unroll
         for (int q = 0; q < Q; ++q) {
-          const uint32_t bits = max(max(__float_as_uint(fabsf(h[q][0].x)), __float_as_uint(fabsf(h[q][0].y))),
-                                    max(__float_as_uint(fabsf(h[q][1].x)), __float_as_uint(fabsf(h[q][1].y))));
+          const uint32_t bits = amax4(h[q]);
           const float m = max_nan(__uint_as_float(__reduce_max_sync(0xffffffffu, bits)),
                                   kFp8AmaxMin);
           if (lane == 2 * q) num = m, den = kFp8Max;
@@ -304,11 +252,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) fwd_kernel(const __gr
           const int c0 = column<true>(q, 0, t, tpr);
           if (lane == 2 * q && c0 - 8 * q < p.H)   // (the warp's first column of the chunk)
             p.scales[(int64_t)(c0 / kFp8Block) * p.ld_s + row] = quot;
-          if (c0 < p.H) {
-            const F2 u = f2_mul(h[q][0], f2_same(r)), v = f2_mul(h[q][1], f2_same(r));
-            *reinterpret_cast<uint32_t*>(p.codes + (int64_t)row * p.ld_c + c0) =
-                cvt4_e4m3(u.x, u.y, v.x, v.y);
-          }
+          put_codes<true>(p.codes + (int64_t)row * p.ld_c, q, t, tpr, p.H, encode4(h[q], r));
         }
       }
       if (FP8 && !VEC) {
