@@ -18,6 +18,8 @@
 // accumulator is free to go on: two of 256 columns (or four of 128) fill TMEM.
 #include <cuda_fp8.h>
 
+#include <type_traits>
+
 #include "dtypes.cuh"
 #include "tc_common.cuh"
 
@@ -27,15 +29,95 @@ namespace fp8 {
 constexpr int kBlk = kFp8Block;
 
 // ---------------------------------------------------------------------- quantization ---
-// The quotients m / 448 (scale) and 448 / m of N <= 16 blocks with maxima `m[i]` (bits), in one
+// Magnitudes of a chunk as bits that compare as they do: 16-bit types two to a word.
+template <typename T>
+struct Mags {
+  static constexpr int N = sizeof(T) == 2 ? 2 : 4;
+  uint32_t w[N];
+};
+
+template <typename T>
+__device__ __forceinline__ Mags<T> mags(const Four<T>& r) {
+  Mags<T> m;
+  if constexpr (sizeof(T) == 2) {
+    const uint2 u = *reinterpret_cast<const uint2*>(&r);
+    m.w[0] = u.x & 0x7fff7fffu;
+    m.w[1] = u.y & 0x7fff7fffu;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) m.w[j] = __float_as_uint(r.e[j]) & 0x7fffffffu;
+  }
+  return m;
+}
+
+template <typename T>
+__device__ __forceinline__ void mags_max(Mags<T>& a, const Mags<T>& b) {
+#pragma unroll
+  for (int i = 0; i < Mags<T>::N; ++i)
+    a.w[i] = sizeof(T) == 2 ? __vmaxu2(a.w[i], b.w[i]) : max(a.w[i], b.w[i]);
+}
+
+// The float32 value of the bits of one magnitude.
+template <typename T>
+__device__ __forceinline__ float mag_value(uint32_t m) {
+  if constexpr (sizeof(T) == 2) {
+    const uint16_t h = (uint16_t)m;
+    return to_f32(*reinterpret_cast<const T*>(&h));
+  } else {
+    return __uint_as_float(m);
+  }
+}
+
+// The warp's largest magnitude (bits).
+template <typename T>
+__device__ __forceinline__ uint32_t warp_top(const Mags<T>& m) {
+  uint32_t v;
+  if constexpr (sizeof(T) == 2) {
+    const uint32_t w = __vmaxu2(m.w[0], m.w[1]);
+    v = max(w & 0xffffu, w >> 16);
+  } else {
+    v = max(max(m.w[0], m.w[1]), max(m.w[2], m.w[3]));
+  }
+  return __reduce_max_sync(0xffffffffu, v);
+}
+
+// The quotients m / 448 (scale) and 448 / m of N <= 16 blocks with maxima m[i] (bits), in one
 // division by the warp: lane 2 i holds the scale of block i, lane 2 i + 1 its reciprocal.
-template <int N>
+template <typename T, int N>
 __device__ __forceinline__ float quotients(const uint32_t m[N], int lane) {
-  float v = 1.f;
+  uint32_t b = 0u;
 #pragma unroll
   for (int i = 0; i < N; ++i)
-    if (lane >> 1 == i) v = max_nan(__uint_as_float(m[i]), kFp8AmaxMin);
-  return lane & 1 ? __fdiv_rn(kFp8Max, v) : __fdiv_rn(v, kFp8Max);
+    if (lane >> 1 == i) b = m[i];
+  const float v = max_nan(mag_value<T>(b), kFp8AmaxMin);
+  return __fdiv_rn(lane & 1 ? kFp8Max : v, lane & 1 ? v : kFp8Max);
+}
+
+// Eight rows' loads of one 128-column block, or R of them. FULL: the block is whole.
+template <typename T, bool VEC, bool FULL, int R>
+__device__ __forceinline__ void load_rows(const T* src, int64_t ld, int rows, int H, int lane,
+                                          Four<T> raw[R]) {
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    raw[i] = raw4<T, VEC, false>(src, 0, lane, 32, FULL ? kBlk : (i < rows ? H : 0));
+    if (FULL || i + 1 < rows) src += ld;
+  }
+}
+
+// R rows' codes in row form, and their scales (lanes 2 i).
+template <typename T, bool VEC, bool FULL, int R>
+__device__ __forceinline__ void put_rows(const Four<T> raw[R], const uint32_t m[R], int rows, int H,
+                                         int lane, uint8_t* dst, int64_t ld_c, float* scales) {
+  const float quot = quotients<T, R>(m, lane);
+  if ((lane & 1) == 0 && lane < 2 * R && (FULL || (lane >> 1) < rows)) scales[lane >> 1] = quot;
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    F2 v[2];
+    pairs(raw[i], v);
+    const float r = __shfl_sync(0xffffffffu, quot, 2 * i + 1);
+    if (FULL || i < rows) put_codes<VEC>(dst, 0, lane, 32, FULL ? kBlk : H, encode4(v, r));
+    dst += ld_c;
+  }
 }
 
 // Rows: a warp takes eight rows of one 128-column block, four columns a lane (a row's maximum is
@@ -43,40 +125,32 @@ __device__ __forceinline__ float quotients(const uint32_t m[N], int lane) {
 // flight: bound by its bytes.
 constexpr int kRowsWarp = 8;
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 4)
 quant_rows_kernel(const T* __restrict__ x, int64_t ld_x, int rows, int cols, int nblk,
                   uint8_t* __restrict__ codes, int64_t ld_c, float* __restrict__ scales,
                   int64_t ld_s) {
+  // (a product launched on these rows may set itself up while they are made)
+  asm volatile("griddepcontrol.launch_dependents;");
   const int lane = threadIdx.x & 31;
   const int64_t items = (int64_t)((rows + kRowsWarp - 1) / kRowsWarp) * nblk;
   const int64_t warps = (int64_t)gridDim.x * 8;
   for (int64_t it = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); it < items; it += warps) {
     const int rg = (int)(it / nblk), b = (int)(it - (int64_t)rg * nblk);
-    const int r0 = rg * kRowsWarp, H = cols - b * kBlk;
+    const int r0 = rg * kRowsWarp, H = cols - b * kBlk, left = rows - r0;
     const T* src = x + (int64_t)r0 * ld_x + b * kBlk;
-    Four<T> raw[kRowsWarp];
-#pragma unroll
-    for (int i = 0; i < kRowsWarp; ++i)
-      raw[i] = raw4<T, VEC, false>(src + (r0 + i < rows ? i * ld_x : 0), 0, lane, 32,
-                                   r0 + i < rows ? H : 0);
-    uint32_t m[kRowsWarp];
-#pragma unroll
-    for (int i = 0; i < kRowsWarp; ++i) {
-      F2 v[2];
-      pairs(raw[i], v);
-      m[i] = __reduce_max_sync(0xffffffffu, amax4(v));
-    }
-    const float quot = quotients<kRowsWarp>(m, lane);
-    if ((lane & 1) == 0 && lane < 2 * kRowsWarp && r0 + (lane >> 1) < rows)
-      scales[(int64_t)b * ld_s + r0 + (lane >> 1)] = quot;
     uint8_t* dst = codes + (int64_t)r0 * ld_c + b * kBlk;
+    float* sc = scales + (int64_t)b * ld_s + r0;
+    auto work = [&](auto full) {
+      constexpr bool FULL = decltype(full)::value;
+      Four<T> raw[kRowsWarp];
+      load_rows<T, VEC, FULL, kRowsWarp>(src, ld_x, left, H, lane, raw);
+      uint32_t m[kRowsWarp];
 #pragma unroll
-    for (int i = 0; i < kRowsWarp; ++i) {
-      F2 v[2];
-      pairs(raw[i], v);
-      const float r = __shfl_sync(0xffffffffu, quot, 2 * i + 1);
-      if (r0 + i < rows) put_codes<VEC>(dst + i * ld_c, 0, lane, 32, H, encode4(v, r));
-    }
+      for (int i = 0; i < kRowsWarp; ++i) m[i] = warp_top<T>(mags(raw[i]));
+      put_rows<T, VEC, FULL, kRowsWarp>(raw, m, left, H, lane, dst, ld_c, sc);
+    };
+    if (H >= kBlk && left >= kRowsWarp) work(std::true_type());
+    else work(std::false_type());
   }
 }
 
@@ -88,7 +162,7 @@ quant_rows_kernel(const T* __restrict__ x, int64_t ld_x, int rows, int cols, int
 //           in shared memory so that neither the writes nor the reads of chunks conflict
 //   BLOCKS  one scale for the tile   -> codes, scales [rows / 128][ld_s]
 template <typename T, bool VEC, bool ROWS, bool COLS, bool BLOCKS>
-__global__ void __launch_bounds__(256, 2)
+__global__ void __launch_bounds__(256, sizeof(T) == 2 && (VEC || !ROWS) ? 3 : 2)
 quant_tile_kernel(const T* __restrict__ x, int64_t ld_x, int rows, int cols,
                   uint8_t* __restrict__ codes, int64_t ld_c, float* __restrict__ scales,
                   int64_t ld_s, uint8_t* __restrict__ codes_t, int64_t ld_ct,
@@ -99,47 +173,38 @@ quant_tile_kernel(const T* __restrict__ x, int64_t ld_x, int rows, int cols,
   __shared__ __align__(16) uint8_t tile[COLS ? kBlk : 1][kBlk];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int cb = blockIdx.x, rb = blockIdx.y;
-  const int r0 = rb * kBlk + w * R, H = cols - cb * kBlk;
-  const T* src = x + (int64_t)(r0 < rows ? r0 : 0) * ld_x + cb * kBlk;
-  Four<T> raw[R];
-#pragma unroll
-  for (int i = 0; i < R; ++i)
-    raw[i] = raw4<T, VEC, false>(src + (r0 + i < rows ? i * ld_x : 0), 0, lane, 32,
-                                 r0 + i < rows ? H : 0);
-  uint32_t top[4] = {0u, 0u, 0u, 0u};   // the columns' maxima over the warp's rows
-  uint32_t m[ROWS ? R : 1];
-#pragma unroll
-  for (int i = 0; i < R; ++i) {
-    F2 v[2];
-    pairs(raw[i], v);
-    if (ROWS) m[ROWS ? i : 0] = __reduce_max_sync(0xffffffffu, amax4(v));
-    top[0] = max(top[0], __float_as_uint(fabsf(v[0].x)));
-    top[1] = max(top[1], __float_as_uint(fabsf(v[0].y)));
-    top[2] = max(top[2], __float_as_uint(fabsf(v[1].x)));
-    top[3] = max(top[3], __float_as_uint(fabsf(v[1].y)));
-  }
+  const int r0 = rb * kBlk + w * R, H = cols - cb * kBlk, left = rows - r0;
+  const T* src = x + (int64_t)(left > 0 ? r0 : 0) * ld_x + cb * kBlk;
   uint8_t* dst = codes + (int64_t)r0 * ld_c + cb * kBlk;
-  if (ROWS) {
-    const float quot = quotients<ROWS ? R : 1>(m, lane);
-    if ((lane & 1) == 0 && r0 + (lane >> 1) < rows)
-      scales[(int64_t)cb * ld_s + r0 + (lane >> 1)] = quot;
+  Four<T> raw[R];
+  auto work = [&](auto full) {
+    constexpr bool FULL = decltype(full)::value;
+    load_rows<T, VEC, FULL, R>(src, ld_x, left, H, lane, raw);
+    Mags<T> top = mags(raw[0]);   // the columns' maxima over the warp's rows
+    uint32_t m[ROWS ? R : 1];
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-      F2 v[2];
-      pairs(raw[i], v);
-      const float r = __shfl_sync(0xffffffffu, quot, 2 * i + 1);
-      if (r0 + i < rows) put_codes<VEC>(dst + i * ld_c, 0, lane, 32, H, encode4(v, r));
+      const Mags<T> a = mags(raw[i]);
+      if (ROWS) m[ROWS ? i : 0] = warp_top<T>(a);
+      if (i) mags_max(top, a);
     }
-  }
 #pragma unroll
-  for (int j = 0; j < 4; ++j) red[w][column<VEC>(0, j, lane, 32)] = top[j];
+    for (int j = 0; j < 4; ++j)
+      red[w][column<VEC>(0, j, lane, 32)] =
+          sizeof(T) == 2 ? (top.w[j >> 1] >> (16 * (j & 1))) & 0xffffu : top.w[sizeof(T) == 2 ? 0 : j];
+    if (ROWS)
+      put_rows<T, VEC, FULL, ROWS ? R : 1>(raw, m, left, H, lane, dst, ld_c,
+                                           scales + (int64_t)cb * ld_s + r0);
+  };
+  if (H >= kBlk && left >= R) work(std::true_type());
+  else work(std::false_type());
   __syncthreads();
   if (COLS) {
     if (threadIdx.x < kBlk) {
       uint32_t a = 0u;
 #pragma unroll
       for (int i = 0; i < 8; ++i) a = max(a, red[i][threadIdx.x]);
-      const float v = max_nan(__uint_as_float(a), kFp8AmaxMin);
+      const float v = max_nan(mag_value<T>(a), kFp8AmaxMin);
       inv[threadIdx.x] = __fdiv_rn(kFp8Max, v);
       if ((int)threadIdx.x < H)
         scales_t[(int64_t)rb * ld_st + cb * kBlk + threadIdx.x] = __fdiv_rn(v, kFp8Max);
@@ -148,14 +213,14 @@ quant_tile_kernel(const T* __restrict__ x, int64_t ld_x, int rows, int cols,
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int c = column<VEC>(0, j, lane, 32);
-      const float r = inv[c];
+      const F2 r = f2_same(inv[c]);
       uint32_t q[4];
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        float f[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) f[i] = __fmul_rn(to_f32(raw[4 * g + i].e[j]), r);
-        q[g] = cvt4_e4m3(f[0], f[1], f[2], f[3]);
+        const Four<T>* f = raw + 4 * g;
+        const F2 a = f2_mul({to_f32(f[0].e[j]), to_f32(f[1].e[j])}, r),
+                 b = f2_mul({to_f32(f[2].e[j]), to_f32(f[3].e[j])}, r);
+        q[g] = cvt4_e4m3(a.x, a.y, b.x, b.y);
       }
       const int at = w ^ ((VEC ? c >> 2 : c) & 7);
       *reinterpret_cast<uint4*>(&tile[COLS ? c : 0][at * 16]) = make_uint4(q[0], q[1], q[2], q[3]);
@@ -177,14 +242,14 @@ quant_tile_kernel(const T* __restrict__ x, int64_t ld_x, int rows, int cols,
 #pragma unroll
       for (int j = 0; j < 4; ++j) a = max(a, red[i][32 * j + lane]);
     a = __reduce_max_sync(0xffffffffu, a);
-    const float v = max_nan(__uint_as_float(a), kFp8AmaxMin);
+    const float v = max_nan(mag_value<T>(a), kFp8AmaxMin);
     if (threadIdx.x == 0) scales[(int64_t)rb * ld_s + cb] = __fdiv_rn(v, kFp8Max);
     const float r = __fdiv_rn(kFp8Max, v);
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       F2 u[2];
       pairs(raw[i], u);
-      if (r0 + i < rows) put_codes<VEC>(dst + i * ld_c, 0, lane, 32, H, encode4(u, r));
+      if (i < left) put_codes<VEC>(dst + i * ld_c, 0, lane, 32, H, encode4(u, r));
     }
   }
 }
@@ -312,6 +377,11 @@ __device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* m
       " [%0], [%1, {%3, %4}], [%2];" ::"r"(tc::smem_u32(dst)),
       "l"((uint64_t)map), "r"(bar), "r"(x), "r"(y)
       : "memory");
+}
+
+// Until the kernels that this one was launched to follow are complete (no wait otherwise).
+__device__ __forceinline__ void grid_wait() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 __device__ __forceinline__ void cluster_sync() {
@@ -539,6 +609,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
   tc::fence_after_sync();
   const uint32_t tmem = tmem_base;
   const int tiles = p.mt * p.nt;
+  grid_wait();   // what comes before reads nothing that the quantization writes
 
   if (warp < 4) {
     if (BN == 256) regs_dec<72>();
@@ -796,8 +867,39 @@ static bool out_map(CUtensorMap* m, void* base, int dtype, int M, int N, int64_t
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// A launch in clusters of `cluster` CTAs; follows: it may begin while the kernel before it on the
+// stream, whose output it reads only after grid_wait, still runs.
+template <typename K, typename... A>
+static int launch_cluster(K kern, int blocks, int threads, uint32_t smem, int cluster, bool follows,
+                          cudaStream_t st, const A&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  int n = 0;
+  if (cluster > 1) {
+    at[n].id = cudaLaunchAttributeClusterDimension;
+    at[n].val.clusterDim.x = cluster;
+    at[n].val.clusterDim.y = at[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (follows) {
+    at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
+  cfg.attrs = at;
+  cfg.numAttrs = n;
+  if (cudaLaunchKernelEx(&cfg, kern, args...) != cudaSuccess) return GSQ_ECUDA;
+  GSQ_CHECK_LAUNCH();
+  return GSQ_OK;
+}
+
 template <int BN, bool BROWS, bool PAIR>
-static int launch_gemm(GemmArgs& p, const void* b, int64_t ldb, int dtype, cudaStream_t st) {
+static int launch_gemm(GemmArgs& p, const void* b, int64_t ldb, int dtype, bool follows,
+                       cudaStream_t st) {
   constexpr int kBRows = PAIR ? BN / 2 : BN;
   constexpr uint32_t kStage = (kBM + kBRows) * kBlk;
   constexpr uint32_t smem = kPipeBytes / kStage * kStage + kStageBytes + 1024;
@@ -820,24 +922,220 @@ static int launch_gemm(GemmArgs& p, const void* b, int64_t ldb, int dtype, cudaS
   if (tiles > INT32_MAX / 2) return GSQ_EINVAL;
   const int most = num_sms() / (PAIR ? 2 : 1);
   const int n = (int)(tiles < most ? tiles : most);
-  if (!PAIR) {
-    kern<<<n, kThreads, smem, st>>>(p, dtype);
-  } else {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(2 * n);
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = 2;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    if (cudaLaunchKernelEx(&cfg, kern, p, dtype) != cudaSuccess) return GSQ_ECUDA;
+  return launch_cluster(kern, PAIR ? 2 * n : n, kThreads, smem, PAIR ? 2 : 1, follows, st, p, dtype);
+}
+
+// ------------------------------------------------------------------------ few rows (decode) ---
+// Up to 64 rows of A: the weight's bytes bound the product, so its rows are the 128 of an MMA
+// tile and the activations its NT columns, and the k-blocks of a row tile are shared out over a
+// cluster of CTAs (a 8192 x 8192 weight has 64 row tiles for 148 SMs). Each CTA streams its
+// k-blocks through kSkStages stages and folds each with the scales of its 128 x 128 block and of
+// the columns; the partial sums meet in the first CTAs' shared memory in the order of the ranks.
+// The weight's first stages are loaded before the activations are quantized (grid_wait).
+constexpr int kSkStages = 5;
+constexpr int kSkThreads = 256;
+
+struct SkinnyArgs {
+  CUtensorMap w, x;
+  int M, N, kb, splits;
+  const float* sx;
+  int64_t ld_sx;
+  const float* sw;
+  int64_t sw_n, sw_k;
+  void* out;
+  int64_t ld_o;
+  int* err;
+};
+
+template <int NT>
+__global__ void __launch_bounds__(kSkThreads) skinny_kernel(const __grid_constant__ SkinnyArgs p,
+                                                            int dtype) {
+  constexpr int kSlots = 4;
+  constexpr uint32_t kCols = kSlots * NT < 32 ? 32 : kSlots * NT;
+  constexpr uint32_t kW = kBM * kBlk, kStage = kW + NT * kBlk;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  __shared__ __align__(8) uint64_t full[kSkStages], empty[kSkStages], tfull[kSlots], tempty[kSlots];
+  __shared__ __align__(8) uint64_t last;
+  __shared__ uint32_t tmem_base;
+  __shared__ __align__(16) float part[NT][kBM];   // this CTA's sums
+  __shared__ __align__(16) float sx_s[16][NT];    // scales of 16 k-blocks, of their columns
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = blockIdx.x % p.splits, tile = blockIdx.x / p.splits;
+  const int k0 = (int)((int64_t)p.kb * rank / p.splits),
+            k1 = (int)((int64_t)p.kb * (rank + 1) / p.splits);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kSkStages; ++i) {
+      tc::mbar_init(&full[i], 1);
+      tc::mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < kSlots; ++i) {
+      tc::mbar_init(&tfull[i], 1);
+      tc::mbar_init(&tempty[i], 4);
+    }
+    tc::mbar_init(&last, 1);
+    tc::fence_barrier_init();
   }
-  GSQ_CHECK_LAUNCH();
-  return GSQ_OK;
+  if (warp == 1) tc::tmem_alloc(&tmem_base, kCols);
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tmem = tmem_base;
+  if (warp == 0) {
+    const bool one = elect_one();
+    const int first = min(k1 - k0, kSkStages);
+    if (one)
+      for (int i = 0; i < first; ++i) {
+        tc::mbar_arrive_expect_tx(&full[i], kStage);
+        tc::tma_load_2d(smem + i * kStage, &p.w, &full[i], (k0 + i) * kBlk, tile * kBM);
+      }
+    grid_wait();
+    if (one)
+      for (int i = 0; i < first; ++i)
+        tc::tma_load_2d(smem + i * kStage + kW, &p.x, &full[i], (k0 + i) * kBlk, 0);
+    __syncwarp();
+    Turn<kSkStages> at;
+    bool ok = true;
+    int issued = first;
+    for (int k = k0 + first; k < k1; ++k, at.next()) {
+      if (!warp_wait(&empty[at.i], at.phase, p.err, 11)) {
+        ok = false;
+        break;
+      }
+      if (one) {
+        uint8_t* st = smem + at.i * kStage;
+        tc::mbar_arrive_expect_tx(&full[at.i], kStage);
+        tc::tma_load_2d(st, &p.w, &full[at.i], k * kBlk, tile * kBM);
+        tc::tma_load_2d(st + kW, &p.x, &full[at.i], k * kBlk, 0);
+      }
+      __syncwarp();
+      ++issued;
+    }
+    // a copy still in flight after a timeout must land before the CTA's memory goes
+    if (!ok && one)
+      for (int i = issued > kSkStages ? issued - kSkStages : 0; i < issued; ++i)
+        tc::mbar_wait(&full[i % kSkStages], (i / kSkStages) & 1, nullptr, 0);
+  } else if (warp == 1) {
+    constexpr uint32_t id = idesc_e4m3(kBM, NT);
+    const bool one = elect_one();
+    const uint32_t base = tc::smem_u32(smem);
+    const uint64_t da0 = tc::umma_desc_k_sw128(base), db0 = tc::umma_desc_k_sw128(base + kW);
+    Turn<kSkStages> at;
+    Turn<kSlots> acc;
+    for (int k = k0; k < k1; ++k, at.next(), acc.next()) {
+      if (!warp_wait(&tempty[acc.i], acc.phase ^ 1, p.err, 12) ||
+          !warp_wait(&full[at.i], at.phase, p.err, 13))
+        break;
+      tc::fence_after_sync();
+      if (one) {
+        const uint64_t off = at.i * (kStage >> 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          umma_e4m3<false>(tmem + acc.i * NT, da0 + off + 2 * j, db0 + off + 2 * j, id, j > 0);
+        tc::umma_commit(&empty[at.i]);
+        tc::umma_commit(&tfull[acc.i]);
+      }
+      __syncwarp();
+    }
+    if (one) {
+      tc::umma_commit(&last);
+      tc::mbar_wait(&last, 0, p.err, 14);
+    }
+  } else if (warp >= 4) {
+    grid_wait();
+    const int q = warp & 3, row = q * 32 + lane, tid = threadIdx.x - 128;
+    const float* sw = p.sw + min(tile * kBM, p.N - 1) / kBlk * p.sw_n;
+    float acc[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) acc[j] = 0.f;
+    Turn<kSlots> slot;
+    bool ok = true;
+    for (int kc = k0; kc < k1; kc += 16) {
+      // the scales of up to 16 k-blocks, times the weight block's
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      for (int i = tid; i < 16 * NT; i += 128) {
+        const int k = kc + i / NT, m = i % NT;
+        sx_s[i / NT][m] = k < k1 && m < p.M ? p.sx[k * p.ld_sx + m] * sw[k * p.sw_k] : 0.f;
+      }
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      for (int k = kc; k < min(k1, kc + 16); ++k) {
+        // (after a timeout the loop runs on, unread: the four warps' barriers keep their count)
+        if (ok) ok = warp_wait(&tfull[slot.i], slot.phase, p.err, 15);
+        if (!ok) continue;
+        tc::fence_after_sync();
+        const float* sx = sx_s[k - kc];
+#pragma unroll
+        for (int c = 0; c < NT; c += 16) {
+          float v[16];
+          tc::tmem_ld16(tmem + ((uint32_t)(q * 32) << 16) + slot.i * NT + c, v);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) acc[c + j] = fmaf(v[j], sx[c + j], acc[c + j]);
+        }
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&tempty[slot.i]);
+        slot.next();
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < NT; ++j) part[j][row] = acc[j];
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  if (warp == 1) tc::tmem_dealloc(tmem, kCols);
+  if (p.splits > 1) cluster_sync();
+  // rows of the output (tokens) rank, rank + splits, ...: 128 columns each, summed over the ranks
+  const int n = threadIdx.x & 127, col = tile * kBM + n;
+  for (int m = rank + p.splits * (threadIdx.x >> 7); m < p.M; m += 2 * p.splits) {
+    float v = 0.f;
+    for (int r = 0; r < p.splits; ++r) {
+      float x;
+      uint32_t a;
+      asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(tc::smem_u32(&part[m][n])), "r"(r));
+      asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(a) : "memory");
+      v += x;
+    }
+    if (col < p.N) {
+      const int64_t o = m * p.ld_o + col;
+      if (dtype == BF16) reinterpret_cast<__nv_bfloat16*>(p.out)[o] = from_f32<__nv_bfloat16>(v);
+      else if (dtype == F16) reinterpret_cast<__half*>(p.out)[o] = from_f32<__half>(v);
+      else reinterpret_cast<float*>(p.out)[o] = v;
+    }
+  }
+  if (p.splits > 1) cluster_sync();   // (the other CTAs have read this one's sums)
+}
+
+constexpr int kSkRows = 64;
+
+template <int NT>
+static int launch_skinny(const GemmArgs& g, const void* x, int64_t ld_x, const void* w, int64_t ldw,
+                         int dtype, bool follows, cudaStream_t st) {
+  constexpr uint32_t kStage = (kBM + NT) * kBlk, smem = kSkStages * kStage + 1024;
+  SkinnyArgs p;
+  if (!codes_map(&p.w, w, g.N, g.K, ldw, kBM) || !codes_map(&p.x, x, g.M, g.K, ld_x, NT))
+    return GSQ_ECUDA;
+  auto kern = skinny_kernel<NT>;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) !=
+      cudaSuccess)
+    return GSQ_ECUDA;
+  p.M = g.M;
+  p.N = g.N;
+  p.kb = g.kb;
+  p.sx = g.sa;
+  p.ld_sx = g.ld_sa;
+  p.sw = g.sb;
+  p.sw_n = g.sb_n;
+  p.sw_k = g.sb_k;
+  p.out = g.out;
+  p.ld_o = g.ld_o;
+  p.err = g.err;
+  const int tiles = (g.N + kBM - 1) / kBM;
+  // as many parts of k as give every SM a CTA, and no more than there are k-blocks
+  int s = 1;
+  while (s < 8 && tiles * s < num_sms() && 2 * s <= g.kb) s *= 2;
+  p.splits = s;
+  return launch_cluster(kern, tiles * s, kSkThreads, smem, s, follows, st, p, dtype);
 }
 
 template <typename T>
@@ -961,10 +1259,11 @@ extern "C" int gsq_fp8_dequant(const void* codes, int64_t ld_codes, const float*
   return GSQ_OK;
 }
 
-extern "C" int gsq_fp8_gemm(int M, int N, int K, const void* a, int64_t lda, const float* sa,
-                            int64_t ld_sa, const void* b, int64_t ldb, const float* sb,
-                            int sb_rows, int64_t sb_n, int64_t sb_k, void* out,
-                            int dtype, int64_t ld_out, int accumulate, int* err, void* stream) {
+static int fp8_gemm(int M, int N, int K, const void* a, int64_t lda, const float* sa,
+                    int64_t ld_sa, const void* b, int64_t ldb, const float* sb,
+                    int sb_rows, int64_t sb_n, int64_t sb_k, void* out,
+                    int dtype, int64_t ld_out, int accumulate, int* err, bool follows,
+                    void* stream) {
   if (!fp8::gemm_ok(M, N, K, a, lda, sa, ld_sa, b, ldb, sb, sb_rows, sb_n, sb_k, out, dtype, ld_out,
                     accumulate, err))
     return GSQ_EINVAL;
@@ -986,6 +1285,12 @@ extern "C" int gsq_fp8_gemm(int M, int N, int K, const void* a, int64_t lda, con
   if (p.boxes && !fp8::out_map(&p.o, out, dtype, M, N, ld_out)) return GSQ_ECUDA;
   p.err = err;
   cudaStream_t st = (cudaStream_t)stream;
+  // Few rows: bound by the weight's bytes (16 x 8192 x 8192: 31 us on 128-row tiles of A, half of
+  // the SMs idle; see skinny_kernel for its figure).
+  if (M <= fp8::kSkRows && !sb_rows && !accumulate)
+    return M <= 16   ? fp8::launch_skinny<16>(p, a, lda, b, ldb, dtype, follows, st)
+           : M <= 32 ? fp8::launch_skinny<32>(p, a, lda, b, ldb, dtype, follows, st)
+                     : fp8::launch_skinny<64>(p, a, lda, b, ldb, dtype, follows, st);
   // Tile by the time of the rounds that the busiest SM walks: 256 x 256 of a pair, 256 x 128 of a
   // pair, or 128 x 128 of one SM. A k-block of the narrow tiles takes 0.64 and 0.7 of the wide
   // one's time (8191 x 8192 x 4096: 251, 330 and 365 us), so they are taken where they need
@@ -999,12 +1304,20 @@ extern "C" int gsq_fp8_gemm(int M, int N, int K, const void* a, int64_t lda, con
                r1 = 0.7 * rounds(128, 128, 1);
   const int pick = r256 <= r128 && r256 <= r1 ? 0 : (r128 <= r1 ? 1 : 2);
   if (sb_rows)
-    return pick == 0   ? fp8::launch_gemm<256, true, true>(p, b, ldb, dtype, st)
-           : pick == 1 ? fp8::launch_gemm<128, true, true>(p, b, ldb, dtype, st)
-                       : fp8::launch_gemm<128, true, false>(p, b, ldb, dtype, st);
-  return pick == 0   ? fp8::launch_gemm<256, false, true>(p, b, ldb, dtype, st)
-         : pick == 1 ? fp8::launch_gemm<128, false, true>(p, b, ldb, dtype, st)
-                     : fp8::launch_gemm<128, false, false>(p, b, ldb, dtype, st);
+    return pick == 0   ? fp8::launch_gemm<256, true, true>(p, b, ldb, dtype, follows, st)
+           : pick == 1 ? fp8::launch_gemm<128, true, true>(p, b, ldb, dtype, follows, st)
+                       : fp8::launch_gemm<128, true, false>(p, b, ldb, dtype, follows, st);
+  return pick == 0   ? fp8::launch_gemm<256, false, true>(p, b, ldb, dtype, follows, st)
+         : pick == 1 ? fp8::launch_gemm<128, false, true>(p, b, ldb, dtype, follows, st)
+                     : fp8::launch_gemm<128, false, false>(p, b, ldb, dtype, follows, st);
+}
+
+extern "C" int gsq_fp8_gemm(int M, int N, int K, const void* a, int64_t lda, const float* sa,
+                            int64_t ld_sa, const void* b, int64_t ldb, const float* sb,
+                            int sb_rows, int64_t sb_n, int64_t sb_k, void* out, int dtype,
+                            int64_t ld_out, int accumulate, int* err, void* stream) {
+  return fp8_gemm(M, N, K, a, lda, sa, ld_sa, b, ldb, sb, sb_rows, sb_n, sb_k, out, dtype, ld_out,
+                  accumulate, err, false, stream);
 }
 
 extern "C" int gsq_fp8_linear(const void* x, int dtype, int M, int K, int64_t ld_x,
@@ -1023,6 +1336,6 @@ extern "C" int gsq_fp8_linear(const void* x, int dtype, int M, int K, int64_t ld
     return GSQ_EINVAL;
   const int s = gsq_fp8_quant(x, dtype, M, K, ld_x, q, ld_q, sq, M, nullptr, 0, nullptr, 0, stream);
   if (s != GSQ_OK) return s;
-  return gsq_fp8_gemm(M, N, K, q, ld_q, sq, M, codes, ld_codes, scales, 0, ld_scales, 1, y,
-                      y_dtype, ld_y, 0, err, stream);
+  return fp8_gemm(M, N, K, q, ld_q, sq, M, codes, ld_codes, scales, 0, ld_scales, 1, y, y_dtype,
+                  ld_y, 0, err, true, stream);
 }
