@@ -168,10 +168,18 @@ class Launches:
     n = 0
 
 
+_entry = {}   # name -> entry point, once the library is loaded on a GPU machine
+
+
 def call(name: str, *args):
     """Call an entry point and raise on a nonzero status."""
     Launches.n += 1
-    check(getattr(lib(), name)(*args), name)
+    fn = _entry.get(name)
+    if fn is None:
+        fn = _entry[name] = getattr(lib(), name)
+    status = fn(*args)
+    if status != GSQ_OK:
+        check(status, name)
 
 
 def device():

@@ -19,7 +19,7 @@ import torch
 
 from .. import _lib
 from ..gemm import err_flag
-from .operands import DTYPES, matrix, on_device, output, pitch
+from .operands import DTYPES, matrix, on_device, output, same_device, stream_of
 
 BLOCK = 128
 E4M3 = torch.float8_e4m3fn
@@ -44,9 +44,9 @@ class Fp8Tensor:
             raise ValueError("codes must be float8_e4m3fn and scales float32")
         if tuple(scales.shape) != (R, _blocks(C)):
             raise ValueError(f"scales must be [{R}, {_blocks(C)}], got {tuple(scales.shape)}")
-        on_device(codes, "codes")
-        on_device(scales, "scales")
-        if R and (codes.stride(1) != 1 or pitch(codes) % 16 or codes.data_ptr() % 16):
+        same_device(scales, "scales", on_device(codes, "codes"))
+        if R and (C > 1 and codes.stride(1) != 1 or R > 1 and codes.stride(0) < C or
+                  codes.stride(0) % 16 or codes.data_ptr() % 16):
             raise ValueError("codes rows must be contiguous with a pitch of a multiple of 16")
         if R > 1 and scales.stride(0) != 1 or scales.shape[1] > 1 and scales.stride(1) < R:
             raise ValueError("scales must be stored block-major ([blocks, rows] transposed)")
@@ -55,8 +55,13 @@ class Fp8Tensor:
 
     @classmethod
     def empty(cls, R, C, dev):
+        """Room for [R, C] (built by its own layout: nothing to check)."""
+        q = cls.__new__(cls)
         codes = torch.empty(R, pad16(C), device=dev, dtype=E4M3)
-        return cls(codes[:, :C], torch.empty(_blocks(C), R, device=dev, dtype=torch.float32).t())
+        q.codes = codes if C == codes.shape[1] else codes[:, :C]
+        q.scales = torch.empty(_blocks(C), R, device=dev, dtype=torch.float32).t()
+        q.shape = (R, C)
+        return q
 
     def float(self):
         """The float32 values that the codes stand for."""
@@ -66,13 +71,13 @@ class Fp8Tensor:
 
 def quantize_rows(x) -> Fp8Tensor:
     """x [R, C] (bf16, float16 or float32) in e4m3 with a scale per row and 128 columns."""
-    x = matrix(x, "x")
+    x, ld = matrix(x, "x")
+    dev = on_device(x, "x")
     R, C = x.shape
     q = Fp8Tensor.empty(R, C, x.device)
     if R and C:
-        _lib.call("gsq_fp8_quant", x.data_ptr(), DTYPES[x.dtype], R, C, pitch(x),
-                  q.codes.data_ptr(), pad16(C), q.scales.data_ptr(), R, None, 0, None, 0,
-                  _lib.stream_ptr())
+        _lib.call("gsq_fp8_quant", x.data_ptr(), DTYPES[x.dtype], R, C, ld, q.codes.data_ptr(),
+                  pad16(C), q.scales.data_ptr(), R, None, 0, None, 0, stream_of(dev))
     return q
 
 
@@ -101,29 +106,33 @@ class Fp8Linear:
                 tuple(scales.shape) != (_blocks(self.N), _blocks(self.K)):
             raise ValueError(f"scales must be float32 [{_blocks(self.N)}, {_blocks(self.K)}], "
                              f"got {scales.dtype} {tuple(scales.shape)}")
-        on_device(codes, "codes")
-        on_device(scales, "scales")
+        self.dev = on_device(codes, "codes")
+        same_device(scales, "scales", self.dev)
         self.codes, self.scales = _padded(codes), scales.contiguous()
         self._t = None
         if codes_t is not None:
             if codes_t.dtype != E4M3 or tuple(codes_t.shape) != (self.K, self.N):
                 raise ValueError(f"codes_t must be float8_e4m3fn [{self.K}, {self.N}]")
-            on_device(codes_t, "codes_t")
+            same_device(codes_t, "codes_t", self.dev)
             self._t = _padded(codes_t)
         self._err = err_flag(codes.device)
+        self._weight = (self.codes.data_ptr(), self.codes.stride(0), self.scales.data_ptr(),
+                        self.scales.shape[1], self.N)
+        self._width = pad16(self.K) + 4 * _blocks(self.K)   # workspace bytes of a row
 
     @classmethod
     def from_weight(cls, W, transposed=False):
         """Quantize a dense weight [N, K] (bf16, float16 or float32); transposed: also keep the
         codes transposed, for vjp."""
-        W = matrix(W, "W")
+        W, ld = matrix(W, "W")
+        dev = on_device(W, "W")
         N, K = W.shape
         if not N or not K:
             raise ValueError("W must not be empty")
         codes = torch.empty(N, pad16(K), device=W.device, dtype=E4M3)
         scales = torch.empty(_blocks(N), _blocks(K), device=W.device, dtype=torch.float32)
-        _lib.call("gsq_fp8_quant_blocks", W.data_ptr(), DTYPES[W.dtype], N, K, pitch(W),
-                  codes.data_ptr(), pad16(K), scales.data_ptr(), _blocks(K), _lib.stream_ptr())
+        _lib.call("gsq_fp8_quant_blocks", W.data_ptr(), DTYPES[W.dtype], N, K, ld,
+                  codes.data_ptr(), pad16(K), scales.data_ptr(), _blocks(K), stream_of(dev))
         lin = cls(codes[:, :K], scales)
         if transposed:
             lin.codes_t()
@@ -141,44 +150,45 @@ class Fp8Linear:
         """out [N, K] (bf16, float16 or float32; rows may be strided) = the dense weight."""
         if out.dtype not in DTYPES:
             raise ValueError(f"unsupported out dtype {out.dtype}")
-        output(out, self.N, self.K, out.dtype, out.device, "out")
-        _lib.call("gsq_fp8_dequant", self.codes.data_ptr(), self.codes.stride(0),
-                  self.scales.data_ptr(), self.scales.shape[1], self.N, self.K, out.data_ptr(),
-                  DTYPES[out.dtype], pitch(out), _lib.stream_ptr())
+        dev = on_device(self.codes, "the weight")
+        _, ld = output(out, self.N, self.K, out.dtype, self.codes, "out")
+        _lib.call("gsq_fp8_dequant", *self._weight[:4], self.N, self.K, out.data_ptr(),
+                  DTYPES[out.dtype], ld, stream_of(dev))
         return out
 
-    def _gemm(self, M, N, K, a, sa, b, sb, sb_rows, sb_n, sb_k, out, accumulate=False):
+    def _gemm(self, M, N, K, a, sa, b, sb, sb_rows, sb_n, sb_k, out, ld, accumulate=False):
         _lib.call("gsq_fp8_gemm", M, N, K, a.data_ptr(), a.stride(0), sa.data_ptr(), M,
                   b.data_ptr(), b.stride(0), sb.data_ptr(), sb_rows, sb_n, sb_k, out.data_ptr(),
-                  DTYPES[out.dtype], pitch(out), int(accumulate), self._err.data_ptr(),
-                  _lib.stream_ptr())
+                  DTYPES[out.dtype], ld, int(accumulate), self._err.data_ptr(),
+                  stream_of(self.dev))
 
     def __call__(self, x, out=None, y_f32=False):
         """y = x W^T [M, N] in x's type (or float32): x [M, K] (bf16, float16 or float32),
         quantized per row and 128 columns on the way; or x an Fp8Tensor (y in bf16)."""
-        on_device(self.codes, "the weight")
+        dev = on_device(self.codes, "the weight")
         if isinstance(x, Fp8Tensor):
             M = x.shape[0]
             if x.shape[1] != self.K:
                 raise ValueError(f"x must be [M, {self.K}], got {x.shape}")
-            y = output(out, M, self.N, torch.float32 if y_f32 else torch.bfloat16,
-                     self.codes.device, "out")
+            same_device(x.codes, "x", dev)
+            y, ld = output(out, M, self.N, torch.float32 if y_f32 else torch.bfloat16,
+                           self.codes, "out")
             if M:
                 self._gemm(M, self.N, self.K, x.codes, x.scales, self.codes, self.scales, 0,
-                           self.scales.shape[1], 1, y)
+                           self.scales.shape[1], 1, y, ld)
             return y
-        x = matrix(x, "x", cols=self.K)
+        x, ld_x = matrix(x, "x", cols=self.K)
+        same_device(x, "x", dev)
         M = x.shape[0]
-        y = output(out, M, self.N, torch.float32 if y_f32 else x.dtype, x.device, "out")
+        y, ld = output(out, M, self.N, torch.float32 if y_f32 else x.dtype, x, "out")
         if not M:
             return y
         # allocated per call on the calling stream: nothing is shared between calls
-        ws = torch.empty(M * (pad16(self.K) + 4 * _blocks(self.K)), device=x.device,
-                         dtype=torch.uint8)
-        _lib.call("gsq_fp8_linear", x.data_ptr(), DTYPES[x.dtype], M, self.K, pitch(x),
-                  self.codes.data_ptr(), self.codes.stride(0), self.scales.data_ptr(),
-                  self.scales.shape[1], self.N, y.data_ptr(), DTYPES[y.dtype], pitch(y),
-                  ws.data_ptr(), ws.numel(), self._err.data_ptr(), _lib.stream_ptr())
+        nbytes = M * self._width
+        ws = x.new_empty((nbytes,), dtype=torch.uint8)
+        _lib.call("gsq_fp8_linear", x.data_ptr(), DTYPES[x.dtype], M, self.K, ld_x, *self._weight,
+                  y.data_ptr(), DTYPES[y.dtype], ld, ws.data_ptr(), nbytes, self._err.data_ptr(),
+                  stream_of(dev))
         return y
 
     def vjp(self, x, dy, dx=None, dw=None, accumulate=False):
@@ -186,32 +196,34 @@ class Fp8Linear:
         dx = dy W [M, K] in x's type, dy quantized per row and 128 columns, W the weight's own
         codes. dw = dy^T x float32 [N, K] (added to dw when accumulate), both quantized per
         column and 128 rows; rounding counts as the identity (straight through)."""
-        x = matrix(x, "x", cols=self.K)
+        dev = on_device(self.codes, "the weight")
+        x, ld_x = matrix(x, "x", cols=self.K)
         M, N, K = x.shape[0], self.N, self.K
-        dy = matrix(dy, "dy", rows=M, cols=N)
-        dev = x.device
-        on_device(self.codes, "the weight")
+        dy, ld_dy = matrix(dy, "dy", rows=M, cols=N)
+        same_device(x, "x", dev)
+        same_device(dy, "dy", dev)
         if accumulate and dw is None:
             raise ValueError("accumulate needs dw")
-        dx = output(dx, M, K, x.dtype, dev, "dx")
-        dw = output(dw, N, K, torch.float32, dev, "dw")
+        dx, ld_dx = output(dx, M, K, x.dtype, x, "dx")
+        dw, ld_dw = output(dw, N, K, torch.float32, x, "dw")
         if not M:
             if not accumulate:
                 dw.zero_()
             return dx, dw
         wt, sw = self.codes_t(), self.scales
-        st = _lib.stream_ptr()
+        st = stream_of(dev)
         lm, ln, mb = pad16(M), pad16(N), _blocks(M)
-        q = torch.empty(M * ln + (N + K) * lm, device=dev, dtype=torch.uint8)
-        s = torch.empty(_blocks(N) * M + mb * (N + K), device=dev, dtype=torch.float32)
+        # allocated per call on the calling stream: nothing is shared between calls
+        q = x.new_empty((M * ln + (N + K) * lm,), dtype=torch.uint8)
+        s = x.new_empty((_blocks(N) * M + mb * (N + K),), dtype=torch.float32)
         dyq, dyt, xt = q[:M * ln].view(M, ln), q[M * ln:M * ln + N * lm].view(N, lm), \
             q[M * ln + N * lm:].view(K, lm)
         s0, s1 = _blocks(N) * M, _blocks(N) * M + mb * N
-        _lib.call("gsq_fp8_quant", dy.data_ptr(), DTYPES[dy.dtype], M, N, pitch(dy),
+        _lib.call("gsq_fp8_quant", dy.data_ptr(), DTYPES[dy.dtype], M, N, ld_dy,
                   dyq.data_ptr(), ln, s.data_ptr(), M, dyt.data_ptr(), lm, s[s0:].data_ptr(), N,
                   st)
-        _lib.call("gsq_fp8_quant", x.data_ptr(), DTYPES[x.dtype], M, K, pitch(x), None, 0, None, 0,
+        _lib.call("gsq_fp8_quant", x.data_ptr(), DTYPES[x.dtype], M, K, ld_x, None, 0, None, 0,
                   xt.data_ptr(), lm, s[s1:].data_ptr(), K, st)
-        self._gemm(M, K, N, dyq, s, wt, sw, 0, 1, sw.shape[1], dx)
-        self._gemm(N, K, M, dyt, s[s0:], xt, s[s1:], 1, 0, K, dw, accumulate)
+        self._gemm(M, K, N, dyq, s, wt, sw, 0, 1, sw.shape[1], dx, ld_dx)
+        self._gemm(N, K, M, dyt, s[s0:], xt, s[s1:], 1, 0, K, dw, ld_dw, accumulate)
         return dx, dw

@@ -1,4 +1,6 @@
-"""Checks of tensor arguments shared by the operators that take bf16, float16 and float32."""
+"""Checks of tensor arguments shared by the operators that take bf16, float16 and float32. They run
+on every call of operators that take a few microseconds on the GPU, so they ask each tensor once
+and build messages only to raise them."""
 from __future__ import annotations
 
 import torch
@@ -7,43 +9,55 @@ DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
 def on_device(t, what):
-    """t is on the current CUDA device (where the launch and its stream are)."""
-    if not t.is_cuda:
+    """The index of the current CUDA device, where t has to be (there are the launch and its
+    stream)."""
+    d = t.get_device()
+    if d < 0:
         raise ValueError(f"{what} must be a CUDA tensor")
-    if t.get_device() != torch.cuda.current_device():
+    if d != torch._C._cuda_getDevice():
         raise ValueError(f"{what} is on {t.device}, the current device is "
                          f"cuda:{torch.cuda.current_device()}")
+    return d
+
+
+def same_device(t, what, dev):
+    """t is on device `dev` (of on_device)."""
+    if t.get_device() != dev:
+        raise ValueError(f"{what} must be on cuda:{dev}, got {t.device}")
+
+
+def stream_of(dev):
+    """The current stream's handle on device `dev`."""
+    return torch._C._cuda_getCurrentRawStream(dev)
 
 
 def matrix(t, what, rows=None, cols=None, dtype=None):
     """t as a matrix whose rows are contiguous (strided rows are taken as they are, any other
-    layout is copied)."""
+    layout is copied), and the elements between its rows. The caller checks its device."""
     if t.dim() != 2 or t.dtype not in DTYPES:
         raise ValueError(f"{what} must be a bf16, float16 or float32 matrix, got {t.dtype} "
                          f"{tuple(t.shape)}")
     if dtype is not None and t.dtype != dtype:
         raise ValueError(f"{what} must be {dtype}, got {t.dtype}")
-    if (rows is not None and t.shape[0] != rows) or (cols is not None and t.shape[1] != cols):
+    r, c = t.shape
+    if rows is not None and r != rows or cols is not None and c != cols:
         raise ValueError(f"{what} must be [{'any' if rows is None else rows}, "
                          f"{'any' if cols is None else cols}], got {tuple(t.shape)}")
-    on_device(t, what)
-    if t.stride(1) != 1 and t.shape[1] > 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+    s0, s1 = t.stride()
+    if s1 != 1 and c > 1 or s0 < c and r > 1:
         t = t.contiguous()
-    return t
+        s0 = c
+    return t, s0 if s0 > c else c
 
 
-def pitch(t):
-    """Elements between the rows of a matrix (one row: any number that holds it)."""
-    return max(t.stride(0), t.shape[1])
-
-
-def output(out, rows, cols, dtype, dev, what):
-    """out, checked, or a new matrix."""
+def output(out, rows, cols, dtype, like, what):
+    """out, checked, or a new matrix beside `like`; and the elements between its rows."""
     if out is None:
-        return torch.empty(rows, cols, device=dev, dtype=dtype)
+        return like.new_empty((rows, cols), dtype=dtype), cols
     if out.dtype != dtype or tuple(out.shape) != (rows, cols):
         raise ValueError(f"{what} must be {dtype} [{rows}, {cols}]")
-    on_device(out, what)
-    if cols > 1 and out.stride(1) != 1 or rows > 1 and out.stride(0) < cols:
+    same_device(out, what, like.get_device())
+    s0, s1 = out.stride()
+    if s1 != 1 and cols > 1 or s0 < cols and rows > 1:
         raise ValueError(f"{what} must have contiguous rows that do not overlap")
-    return out
+    return out, s0 if s0 > cols else cols

@@ -26,7 +26,7 @@ import numpy as np
 import torch
 
 from .. import _lib
-from .operands import DTYPES, on_device
+from .operands import DTYPES, on_device, same_device, stream_of
 
 _KEYS = {"linear": set(), "ntk": set(), "yarn": {"original", "slow", "fast", "attention"},
          "bands": {"original", "low", "high"}}
@@ -90,24 +90,22 @@ class Rotary:
         self.layout = layout
         self.freqs, self.factor = frequencies(self.rotary_dim, theta, scaling)
         self.turns = torch.from_numpy(self.freqs / (2 * math.pi)).to(device or _lib.device())
+        self._turns, self._pairs = self.turns.data_ptr(), int(layout == "interleaved")
 
-    def _side(self, x, T, dtype, what):
+    def _side(self, x, T, dtype, dev, what):
         """Strides of tokens and heads, and the heads, of x [T, heads, head_dim]."""
-        if x.dim() != 3 or x.dtype != dtype:
+        shape = x.shape
+        if len(shape) != 3 or x.dtype != dtype or shape[2] != self.head_dim or shape[0] != T:
             raise ValueError(f"{what} must be {dtype} [{T}, heads, {self.head_dim}], got "
-                             f"{x.dtype} {tuple(x.shape)}")
-        t, n, hd = x.shape
-        if hd != self.head_dim or t != T:
-            raise ValueError(f"{what} must be {dtype} [{T}, heads, {self.head_dim}], got "
-                             f"{x.dtype} {tuple(x.shape)}")
-        on_device(x, what)
+                             f"{x.dtype} {tuple(shape)}")
+        same_device(x, what, dev)
         st, sh, se = x.stride()
-        if se != 1 and hd > 1:
+        if se != 1 and self.head_dim > 1:
             raise ValueError(f"{what}: the elements of a head must be contiguous")
-        return st, sh, n
+        return st, sh, shape[1]
 
-    def _out_side(self, o, x, T, dtype, what):
-        st, sh, n = self._side(o, T, dtype, what)
+    def _out_side(self, o, x, T, dtype, dev, what):
+        st, sh, n = self._side(o, T, dtype, dev, what)
         if n != x.shape[1]:
             raise ValueError(f"{what} must be {tuple(x.shape)}, got {tuple(o.shape)}")
         if st == 0 and T > 1 or sh == 0 and n > 1:
@@ -121,36 +119,34 @@ class Rotary:
         if q.dim() != 3 or code is None:
             raise ValueError(f"q must be a bf16, float16 or float32 [T, heads, {self.head_dim}] "
                              f"tensor, got {q.dtype} {tuple(q.shape)}")
-        T, dt = q.shape[0], q.dtype
-        q_t, q_h, nq = self._side(q, T, dt, "q")
+        dev = on_device(q, "q")
+        T, dt, hd = q.shape[0], q.dtype, self.head_dim
+        q_t, q_h, nq = self._side(q, T, dt, dev, "q")
         if not nq and T:
             raise ValueError("q must have at least one head")
-        k_t, k_h, nk = (0, 0, 0) if k is None else self._side(k, T, dt, "k")
+        k_t, k_h, nk = (0, 0, 0) if k is None else self._side(k, T, dt, dev, "k")
         wide = positions.dtype is torch.int64
         if not wide and positions.dtype is not torch.int32 or positions.shape != (T,):
             raise ValueError(f"positions must be int32 or int64 [{T}], got {positions.dtype} "
                              f"{tuple(positions.shape)}")
-        on_device(positions, "positions")
-        on_device(self.turns, "the plan")
-        positions = positions.contiguous()
-        hd = self.head_dim
+        same_device(positions, "positions", dev)
+        same_device(self.turns, "the plan", dev)
+        if not positions.is_contiguous():
+            positions = positions.contiguous()
         if out is None:
-            qo, qo_t, qo_h = torch.empty((T, nq, hd), device=q.device, dtype=dt), nq * hd, hd
-            ko, ko_t, ko_h = None, nk * hd, hd
-            if k is not None:
-                ko = torch.empty((T, nk, hd), device=q.device, dtype=dt)
+            qo, qo_t, qo_h = q.new_empty((T, nq, hd)), nq * hd, hd
+            ko, ko_t, ko_h = None if k is None else k.new_empty((T, nk, hd)), nk * hd, hd
         else:
             qo, ko = out
             if qo is None or (ko is None) != (k is None):
                 raise ValueError("out must be (q_out, k_out), k_out None without k")
-            qo_t, qo_h = self._out_side(qo, q, T, dt, "q_out")
-            ko_t, ko_h = (0, 0) if k is None else self._out_side(ko, k, T, dt, "k_out")
+            qo_t, qo_h = self._out_side(qo, q, T, dt, dev, "q_out")
+            ko_t, ko_h = (0, 0) if k is None else self._out_side(ko, k, T, dt, dev, "k_out")
         if T:
             _lib.call("gsq_rope", q.data_ptr(), q_t, q_h, nq, k.data_ptr() if nk else None, k_t,
-                      k_h, nk, T, hd, self.rotary_dim, int(self.layout == "interleaved"), code,
-                      positions.data_ptr(), int(wide), self.turns.data_ptr(), self.factor,
-                      int(inverse), qo.data_ptr(), qo_t, qo_h, ko.data_ptr() if nk else None, ko_t,
-                      ko_h, _lib.stream_ptr())
+                      k_h, nk, T, hd, self.rotary_dim, self._pairs, code, positions.data_ptr(),
+                      wide, self._turns, self.factor, inverse, qo.data_ptr(), qo_t, qo_h,
+                      ko.data_ptr() if nk else None, ko_t, ko_h, stream_of(dev))
         return qo, ko
 
     def __call__(self, q, k, positions, out=None):

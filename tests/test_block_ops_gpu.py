@@ -126,6 +126,24 @@ def test_fp8_vjp(M, K, N, dtype):
          + U * np.abs(rw + f64(base)), "dw added")
 
 
+def test_fp8_long_and_wide():
+    """More k-blocks than a CTA of the few-row product stages scales for at a time, with no split
+    of k; and the widest tiles with a scale per row of both sides (dW of a square weight)."""
+    from gsq_rco_mlx_b200.common.fp8 import Fp8Linear
+    lin = Fp8Linear.from_weight(rnd((19000, 2600), 1, torch.bfloat16, 0.05))
+    x = rnd((4, 2600), 2, torch.bfloat16)
+    y = lin(x, y_f32=True)
+    ref, mag = of.linear(f32(x), f32(lin.codes), f32(lin.scales))
+    near(f64(y), ref, _tol_gemm(mag, 2600, torch.float32, ref))
+    lin = Fp8Linear.from_weight(rnd((4864, 4864), 3, torch.bfloat16, 0.05))
+    x, dy = rnd((130, 4864), 4, torch.bfloat16), rnd((130, 4864), 5, torch.bfloat16)
+    dx, dw = lin.vjp(x, dy)
+    _err_ok()
+    rx, mx, rw, mw = of.vjp(f32(x), f32(dy), f32(lin.codes), f32(lin.scales))
+    near(f64(dx), rx, _tol_gemm(mx, 4864, torch.bfloat16, rx), "dx")
+    near(f64(dw), rw, _tol_gemm(mw, 130, torch.float32, rw), "dw")
+
+
 def test_fp8_strides_outputs_and_refusals():
     """Rows of a wider buffer, a transposed input, outputs inside a wider buffer (whose other
     columns stay), no rows at all; and what is refused."""
