@@ -29,32 +29,29 @@ __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2hal
 // Pairs of float32 in one instruction (each half rounds as the scalar operation does): the fused
 // multiply-add of a pair issues as fast as a single one.
 struct F2 {
-  float x, y;
+  uint64_t b;   // held as the packed operations take it: a pair of registers, not two
+  F2() = default;
+  __device__ __forceinline__ F2(float x, float y) {
+    asm("mov.b64 %0, {%1, %2};" : "=l"(b) : "f"(x), "f"(y));
+  }
+  __device__ __forceinline__ explicit F2(uint64_t bits) : b(bits) {}
+  __device__ __forceinline__ float x() const { return __uint_as_float((uint32_t)b); }
+  __device__ __forceinline__ float y() const { return __uint_as_float((uint32_t)(b >> 32)); }
 };
-__device__ __forceinline__ uint64_t f2_bits(F2 v) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(v.x), "f"(v.y));
+__device__ __forceinline__ F2 f2_fma(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.b) : "l"(a.b), "l"(b.b), "l"(c.b));
   return r;
 }
-__device__ __forceinline__ F2 f2_of(uint64_t r) {
-  F2 v;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(r));
-  return v;
-}
-__device__ __forceinline__ F2 f2_fma(F2 a, F2 b, F2 c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(f2_bits(a)), "l"(f2_bits(b)), "l"(f2_bits(c)));
-  return f2_of(r);
-}
 __device__ __forceinline__ F2 f2_mul(F2 a, F2 b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(f2_bits(a)), "l"(f2_bits(b)));
-  return f2_of(r);
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.b) : "l"(a.b), "l"(b.b));
+  return r;
 }
 __device__ __forceinline__ F2 f2_add(F2 a, F2 b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(f2_bits(a)), "l"(f2_bits(b)));
-  return f2_of(r);
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.b) : "l"(a.b), "l"(b.b));
+  return r;
 }
 __device__ __forceinline__ F2 f2_same(float v) { return {v, v}; }
 
@@ -74,12 +71,12 @@ template <typename T>
 __device__ __forceinline__ uint32_t f2_pack(F2 v);
 template <>
 __device__ __forceinline__ uint32_t f2_pack<__nv_bfloat16>(F2 v) {
-  const __nv_bfloat162 h = __floats2bfloat162_rn(v.x, v.y);
+  const __nv_bfloat162 h = __floats2bfloat162_rn(v.x(), v.y());
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 template <>
 __device__ __forceinline__ uint32_t f2_pack<__half>(F2 v) {
-  const __half2 h = __floats2half2_rn(v.x, v.y);
+  const __half2 h = __floats2half2_rn(v.x(), v.y());
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
@@ -150,8 +147,8 @@ constexpr float kFp8AmaxMin = 7.8886090522101181e-31f;  // 2^-100
 
 // Bits of the largest magnitude of four (magnitudes compare as their bits, NaN above infinity).
 __device__ __forceinline__ uint32_t amax4(const F2 v[2]) {
-  return max(max(__float_as_uint(fabsf(v[0].x)), __float_as_uint(fabsf(v[0].y))),
-             max(__float_as_uint(fabsf(v[1].x)), __float_as_uint(fabsf(v[1].y))));
+  return max(max(__float_as_uint(fabsf(v[0].x())), __float_as_uint(fabsf(v[0].y()))),
+             max(__float_as_uint(fabsf(v[1].x())), __float_as_uint(fabsf(v[1].y()))));
 }
 
 __device__ __forceinline__ uint32_t cvt4_e4m3(float a, float b, float c, float d) {
@@ -163,7 +160,7 @@ __device__ __forceinline__ uint32_t cvt4_e4m3(float a, float b, float c, float d
 
 __device__ __forceinline__ uint32_t encode4(const F2 v[2], float r) {
   const F2 a = f2_mul(v[0], f2_same(r)), b = f2_mul(v[1], f2_same(r));
-  return cvt4_e4m3(a.x, a.y, b.x, b.y);
+  return cvt4_e4m3(a.x(), a.y(), b.x(), b.y());
 }
 
 // Writes a chunk's codes (as raw4 deals columns): one word, or a byte each.

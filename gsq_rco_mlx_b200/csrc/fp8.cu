@@ -218,9 +218,9 @@ quant_tile_kernel(const T* __restrict__ x, int64_t ld_x, int rows, int cols,
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const Four<T>* f = raw + 4 * g;
-        const F2 a = f2_mul({to_f32(f[0].e[j]), to_f32(f[1].e[j])}, r),
-                 b = f2_mul({to_f32(f[2].e[j]), to_f32(f[3].e[j])}, r);
-        q[g] = cvt4_e4m3(a.x, a.y, b.x, b.y);
+        const F2 a = f2_mul(F2(to_f32(f[0].e[j]), to_f32(f[1].e[j])), r),
+                 b = f2_mul(F2(to_f32(f[2].e[j]), to_f32(f[3].e[j])), r);
+        q[g] = cvt4_e4m3(a.x(), a.y(), b.x(), b.y());
       }
       const int at = w ^ ((VEC ? c >> 2 : c) & 7);
       *reinterpret_cast<uint4*>(&tile[COLS ? c : 0][at * 16]) = make_uint4(q[0], q[1], q[2], q[3]);
@@ -500,8 +500,8 @@ __device__ __forceinline__ void store_row(const GemmArgs& p, int m, int n0,
   T* o = reinterpret_cast<T*>(p.out) + (int64_t)m * p.ld_o + n0;
 #pragma unroll
   for (int c = 0; c < CW; ++c) {
-    const F2 a = f2_of(acc[c >> 1]);
-    const float v = c & 1 ? a.y : a.x;
+    const F2 a(acc[c >> 1]);
+    const float v = c & 1 ? a.y() : a.x();
     if (n0 + c < p.N) o[c] = from_f32<T>(p.accumulate ? v + to_f32(o[c]) : v);
   }
 }
@@ -526,12 +526,11 @@ __device__ __forceinline__ void store_boxes(const GemmArgs& p, uint8_t* stage, i
         uint4 v;
         if constexpr (sizeof(T) == 2) {
           const uint64_t* a = acc + (c0 + c * 8) / 2;
-          v = make_uint4(f2_pack<T>(f2_of(a[0])), f2_pack<T>(f2_of(a[1])), f2_pack<T>(f2_of(a[2])),
-                         f2_pack<T>(f2_of(a[3])));
+          v = make_uint4(f2_pack<T>(F2(a[0])), f2_pack<T>(F2(a[1])), f2_pack<T>(F2(a[2])),
+                         f2_pack<T>(F2(a[3])));
         } else {
-          const F2 a = f2_of(acc[(c0 + c * 4) / 2]), b = f2_of(acc[(c0 + c * 4) / 2 + 1]);
-          v = make_uint4(__float_as_uint(a.x), __float_as_uint(a.y), __float_as_uint(b.x),
-                         __float_as_uint(b.y));
+          const uint64_t a = acc[(c0 + c * 4) / 2], b = acc[(c0 + c * 4) / 2 + 1];
+          v = make_uint4((uint32_t)a, (uint32_t)(a >> 32), (uint32_t)b, (uint32_t)(b >> 32));
         }
         *reinterpret_cast<uint4*>(box + lane * 128 + ((c ^ (lane & 7)) << 4)) = v;
       }
@@ -761,7 +760,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
         at.next();
         float s = ring_s[e][q * 32 + lane];
         if (!BROWS) s *= ring_s[e][kBM + part * CW / kBlk];
-        const uint64_t s2 = f2_bits(f2_same(s));
+        const uint64_t s2 = f2_same(s).b;
         const float* sbw = ring_s[e] + kBM + part * CW;
         uint32_t r[64];
 #pragma unroll

@@ -91,10 +91,10 @@ __device__ __forceinline__ void put4(T* __restrict__ row, int q, int t, int tpr,
       if constexpr (sizeof(T) == 2)
         *reinterpret_cast<uint2*>(row + c0) = make_uint2(f2_pack<T>(v[0]), f2_pack<T>(v[1]));
       else
-        *reinterpret_cast<float4*>(row + c0) = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+        *reinterpret_cast<float4*>(row + c0) = make_float4(v[0].x(), v[0].y(), v[1].x(), v[1].y());
     }
   } else {
-    const float f[4] = {v[0].x, v[0].y, v[1].x, v[1].y};
+    const float f[4] = {v[0].x(), v[0].y(), v[1].x(), v[1].y()};
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       if (c0 + j * tpr < H) row[c0 + j * tpr] = from_f32<T>(f[j]);
@@ -103,10 +103,10 @@ __device__ __forceinline__ void put4(T* __restrict__ row, int q, int t, int tpr,
 
 __device__ __forceinline__ float f2_dot(const F2 a[2], const F2 b[2]) {
   const F2 s = f2_fma(a[1], b[1], f2_mul(a[0], b[0]));
-  return s.x + s.y;
+  return s.x() + s.y();
 }
 __device__ __forceinline__ float f2_at(const F2 v[2], int j) {
-  return j & 1 ? v[j >> 1].y : v[j >> 1].x;
+  return j & 1 ? v[j >> 1].y() : v[j >> 1].x();
 }
 
 // 1 / sqrt(m): the hardware's estimate (2 steps off at most) after one Newton iteration
@@ -348,7 +348,7 @@ __device__ __forceinline__ void fetch_row(const Bwd& p, int row, uint8_t* slot, 
 
 constexpr int kMaxSlots = 4;
 
-// Where a thread's alpha a g and b are kept: in registers up to 512 threads a team, in shared
+// Where a thread's alpha a g and b are kept: in registers up to 768 threads a team, in shared
 // memory up to 1024, and read anew for every row where a row does not fit shared memory.
 enum Weights { W_REG, W_SMEM, W_MEM };
 
@@ -356,7 +356,7 @@ enum Weights { W_REG, W_SMEM, W_MEM };
 // bulk copies, `slots` rows ahead, so that the loads run on through the two sums of a row, and
 // dh2 is read only after the first of them: 6 of 8 registers a column.
 template <typename T, bool VEC, bool WARP, int Q, int W, int THREADS>
-__global__ void __launch_bounds__(THREADS, 1) bwd_kernel(const __grid_constant__ Bwd p) {
+__global__ void __launch_bounds__(THREADS, WARP ? 2 : 1) bwd_kernel(const __grid_constant__ Bwd p) {
   constexpr bool STAGED = W != W_MEM;
   constexpr int QW = W == W_REG ? Q : 1;
   extern __shared__ __align__(16) uint8_t dyn[];
@@ -424,13 +424,17 @@ __global__ void __launch_bounds__(THREADS, 1) bwd_kernel(const __grid_constant__
     // (after a timeout the rows run on unread, so that the block's barriers keep their count)
     if (STAGED && alive) alive = tc::mbar_wait(&bar[slot], phase, p.err, 6);
     auto read = [&](int i, int q, F2 v[2]) {
-      const T* src = reinterpret_cast<const T*>(p.in[i]) + (int64_t)row * p.ld[i];
-      if (STAGED)
-        get4<T, VEC, true>(reinterpret_cast<const T*>(mine + slot * slot_bytes + i * p.row_bytes +
-                                                      ((uint32_t)(uintptr_t)src & 15u)),
-                           q, t, tpr, p.H, v);
-      else
-        get4<T, VEC, false>(src, q, t, tpr, p.H, v);
+      if (STAGED) {
+        // (a row that does not start on 16 bytes lies that far into its copy)
+        uint32_t off = i * p.row_bytes;
+        if (!VEC)
+          off += (uint32_t)(uintptr_t)(reinterpret_cast<const T*>(p.in[i]) + (int64_t)row * p.ld[i]) & 15u;
+        get4<T, VEC, true>(reinterpret_cast<const T*>(mine + slot * slot_bytes + off), q, t, tpr,
+                           p.H, v);
+      } else {
+        get4<T, VEC, false>(reinterpret_cast<const T*>(p.in[i]) + (int64_t)row * p.ld[i], q, t, tpr,
+                            p.H, v);
+      }
     };
     F2 y[Q][2], h[Q][2], u[Q][2];
     float s = 0.f;
@@ -612,12 +616,12 @@ static Plan bwd_plan(int T, int H, int dtype, int groups, bool gate) {
   // room for the whole team's columns (a row is read past H) and for an unaligned start
   const int room = 4 * q * (warp ? 32 : pl.threads);
   pl.row_bytes = (uint32_t)(room * dtype_size(dtype) + 32);
-  pl.weights = H <= 4096 ? W_REG : W_SMEM;
+  pl.weights = H <= 6144 ? W_REG : W_SMEM;
   const size_t slot = (size_t)kArrays * pl.row_bytes;
   const size_t fix = pl.weights == W_SMEM ? (size_t)8 * room : 0;
   if (q > 2 || slot + fix > kSmemTeam) pl.weights = W_MEM;
-  // teams of an SM: 512 threads of 128 registers
-  const int sm_blocks = pl.weights == W_REG ? 512 / pl.threads : 1;
+  // teams of an SM: 640 threads of 96 registers (two blocks of eight warp teams)
+  const int sm_blocks = warp ? 2 : (pl.weights == W_REG && pl.threads <= 640 ? 640 / pl.threads : 1);
   pl.slots = 1;
   pl.smem = 0;
   if (pl.weights != W_MEM) {
@@ -654,10 +658,10 @@ static int bwd_launch(const Bwd& p, const Plan& pl, cudaStream_t st) {
 template <typename T, bool VEC>
 static int bwd_any(const Bwd& p, const Plan& pl, cudaStream_t st) {
   if (p.H <= 256) return bwd_launch<T, VEC, true, 2, W_REG, 256>(p, pl, st);
-  if (pl.weights == W_REG) return bwd_launch<T, VEC, false, 2, W_REG, 512>(p, pl, st);
-  if (pl.weights == W_SMEM) return pl.threads <= 768
-                                       ? bwd_launch<T, VEC, false, 2, W_SMEM, 768>(p, pl, st)
-                                       : bwd_launch<T, VEC, false, 2, W_SMEM, 1024>(p, pl, st);
+  if (pl.weights == W_REG) return pl.threads <= 640
+                                      ? bwd_launch<T, VEC, false, 2, W_REG, 640>(p, pl, st)
+                                      : bwd_launch<T, VEC, false, 2, W_REG, 768>(p, pl, st);
+  if (pl.weights == W_SMEM) return bwd_launch<T, VEC, false, 2, W_SMEM, 1024>(p, pl, st);
   if (p.H <= 8192) return bwd_launch<T, VEC, false, 2, W_MEM, 1024>(p, pl, st);
   if (p.H <= 16384) return bwd_launch<T, VEC, false, 4, W_MEM, 1024>(p, pl, st);
   return bwd_launch<T, VEC, false, 8, W_MEM, 1024>(p, pl, st);
