@@ -126,10 +126,17 @@ __device__ __forceinline__ Four<T> raw4(const T* row, int q, int t, int tpr, int
   return v;
 }
 
-template <typename T>
+// The chunk's values as two pairs (VEC: unpacked a word at a time).
+template <typename T, bool VEC>
 __device__ __forceinline__ void pairs(const Four<T>& r, F2 v[2]) {
-  v[0] = {to_f32(r.e[0]), to_f32(r.e[1])};
-  v[1] = {to_f32(r.e[2]), to_f32(r.e[3])};
+  if constexpr (VEC && sizeof(T) == 2) {
+    const uint2 w = *reinterpret_cast<const uint2*>(&r);
+    v[0] = f2_unpack<T>(w.x);
+    v[1] = f2_unpack<T>(w.y);
+  } else {
+    v[0] = {to_f32(r.e[0]), to_f32(r.e[1])};
+    v[1] = {to_f32(r.e[2]), to_f32(r.e[3])};
+  }
 }
 
 // maximum that keeps NaN (fmaxf drops it)

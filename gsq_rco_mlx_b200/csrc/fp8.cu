@@ -113,7 +113,7 @@ __device__ __forceinline__ void put_rows(const Four<T> raw[R], const uint32_t m[
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     F2 v[2];
-    pairs(raw[i], v);
+    pairs<T, VEC>(raw[i], v);
     const float r = __shfl_sync(0xffffffffu, quot, 2 * i + 1);
     if (FULL || i < rows) put_codes<VEC>(dst, 0, lane, 32, FULL ? kBlk : H, encode4(v, r));
     dst += ld_c;
@@ -248,7 +248,7 @@ quant_tile_kernel(const T* __restrict__ x, int64_t ld_x, int rows, int cols,
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       F2 u[2];
-      pairs(raw[i], u);
+      pairs<T, VEC>(raw[i], u);
       if (i < left) put_codes<VEC>(dst + i * ld_c, 0, lane, 32, H, encode4(u, r));
     }
   }

@@ -79,7 +79,7 @@ __device__ __forceinline__ float team_sum(float v, float (*red)[32], int& turn) 
 
 template <typename T, bool VEC, bool PAD>
 __device__ __forceinline__ void get4(const T* row, int q, int t, int tpr, int H, F2 v[2]) {
-  pairs(raw4<T, VEC, PAD>(row, q, t, tpr, H), v);
+  pairs<T, VEC>(raw4<T, VEC, PAD>(row, q, t, tpr, H), v);
 }
 
 template <typename T, bool VEC>
@@ -190,7 +190,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) fwd_kernel(const __gr
     F2 y[Q][2], h[Q][2];
     if (!HOLD) load(row);
 #pragma unroll
-    for (int q = 0; q < Q; ++q) pairs(yn[q], y[q]), pairs(hn[q], h[q]);
+    for (int q = 0; q < Q; ++q) pairs<T, VEC>(yn[q], y[q]), pairs<T, VEC>(hn[q], h[q]);
     if (HOLD && row + teams < p.T) load(row + teams);
     const int g = p.gate ? row / p.per_gate : 0;
     if (HOLD && g != held) {
@@ -323,27 +323,17 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
       : "memory");
 }
 
-// Copies a row of every array into a slot: from the 16-byte boundary at or below its start to
-// that at or above its end (the few bytes around a row that does not start or end there lie in
-// the same 16 bytes as the row's own).
+// Copies a row of array i into a slot (the team's thread i does): from the 16-byte boundary at or
+// below its start to that at or above its end (the few bytes around a row that does not start or
+// end there lie in the same 16 bytes as the row's own).
 template <typename T>
-__device__ __forceinline__ void fetch_row(const Bwd& p, int row, uint8_t* slot, uint64_t* bar) {
-  uint32_t total = 0, bytes[kArrays];
-  const uint8_t* from[kArrays];
-#pragma unroll
-  for (int i = 0; i < kArrays; ++i) {
-    bytes[i] = 0;
-    if (!p.in[i]) continue;
-    const uintptr_t s = (uintptr_t)(reinterpret_cast<const T*>(p.in[i]) + (int64_t)row * p.ld[i]);
-    const uintptr_t lo = s & ~(uintptr_t)15, hi = (s + p.H * sizeof(T) + 15) & ~(uintptr_t)15;
-    from[i] = reinterpret_cast<const uint8_t*>(lo);
-    bytes[i] = (uint32_t)(hi - lo);
-    total += bytes[i];
-  }
-  tc::mbar_arrive_expect_tx(bar, total);
-#pragma unroll
-  for (int i = 0; i < kArrays; ++i)
-    if (bytes[i]) bulk_load(slot + i * p.row_bytes, from[i], bytes[i], bar);
+__device__ __forceinline__ void fetch_row(const Bwd& p, int row, int i, uint8_t* slot,
+                                          uint64_t* bar) {
+  if (!p.in[i]) return;
+  const uintptr_t s = (uintptr_t)(reinterpret_cast<const T*>(p.in[i]) + (int64_t)row * p.ld[i]);
+  const uintptr_t lo = s & ~(uintptr_t)15, hi = (s + p.H * sizeof(T) + 15) & ~(uintptr_t)15;
+  tc::mbar_arrive_expect_tx(bar, (uint32_t)(hi - lo));
+  bulk_load(slot + i * p.row_bytes, reinterpret_cast<const void*>(lo), (uint32_t)(hi - lo), bar);
 }
 
 constexpr int kMaxSlots = 4;
@@ -355,40 +345,46 @@ enum Weights { W_REG, W_SMEM, W_MEM };
 // Persistent teams, 4 Q columns a thread. Unless W_MEM, a team's rows arrive in shared memory by
 // bulk copies, `slots` rows ahead, so that the loads run on through the two sums of a row, and
 // dh2 is read only after the first of them: 6 of 8 registers a column.
-template <typename T, bool VEC, bool WARP, int Q, int W, int THREADS>
+// ALL: both norms and both cotangents are there.
+template <typename T, bool VEC, bool WARP, int Q, int W, int THREADS, bool ALL>
 __global__ void __launch_bounds__(THREADS, WARP ? 2 : 1) bwd_kernel(const __grid_constant__ Bwd p) {
   constexpr bool STAGED = W != W_MEM;
   constexpr int QW = W == W_REG ? Q : 1;
   extern __shared__ __align__(16) uint8_t dyn[];
   __shared__ __align__(16) float red[2][32];
   __shared__ __align__(8) uint64_t bars[WARP ? 8 : 1][kMaxSlots];
-  __shared__ Rows ahead_s[WARP ? 8 : 1];   // the next row to fetch (the first thread's)
   int turn = 0;
-  const int w = WARP ? threadIdx.x >> 5 : 0;
+  const int w = WARP ? threadIdx.x >> 5 : 0, per = WARP ? blockDim.x >> 5 : 1;
   const int t = WARP ? threadIdx.x & 31 : threadIdx.x, tpr = WARP ? 32 : blockDim.x;
-  const int team = WARP ? blockIdx.x * 8 + w : blockIdx.x;
-  const int teams = WARP ? gridDim.x * 8 : gridDim.x;
+  const int team = blockIdx.x * per + w, teams = gridDim.x * per;
   const float inv_H = 1.f / (float)p.H;
   uint64_t* bar = bars[w];
   const uint32_t slot_bytes = kArrays * p.row_bytes;
   uint8_t* mine = dyn + (size_t)w * p.slots * slot_bytes;
-  float* ag_s = reinterpret_cast<float*>(dyn + (size_t)(WARP ? 8 : 1) * p.slots * slot_bytes);
-  float* b_s = ag_s + 4 * Q * tpr;
+  // W_SMEM: b and alpha a g
+  const int room = 4 * Q * tpr;
+  float* b_s = reinterpret_cast<float*>(dyn + (size_t)per * p.slots * slot_bytes);
+  float* ag_s = b_s + room;
   if (!WARP && threadIdx.x < 64) red[threadIdx.x >> 5][threadIdx.x & 31] = 0.f;
+  if (W == W_SMEM)
+    for (int c = threadIdx.x; c < room; c += blockDim.x)
+      b_s[c] = p.w_pre && c < p.H ? to_f32(reinterpret_cast<const T*>(p.w_pre)[c]) + p.offset : 0.f;
   if (STAGED && t == 0) {
-    for (int i = 0; i < p.slots; ++i) tc::mbar_init(&bar[i], 1);
+    int arrays = 0;
+#pragma unroll
+    for (int i = 0; i < kArrays; ++i) arrays += p.in[i] != nullptr;
+    for (int i = 0; i < p.slots; ++i) tc::mbar_init(&bar[i], arrays);
     tc::fence_barrier_init();
   }
   __syncthreads();
-  Rows it;
+  Rows it, ahead;   // the row at work, and the next to fetch
   it.open(p, team);
-  if (STAGED && t == 0) {
-    Rows ahead = it;
+  ahead = it;
+  if (STAGED)
     for (int i = 0; i < p.slots && ahead.item >= 0; ++i, ahead.next(p, teams))
-      fetch_row<T>(p, ahead.row, mine + i * slot_bytes, &bar[i]);
-    ahead_s[w] = ahead;
-  }
-  const bool post = p.w_post != nullptr, pre = p.w_pre != nullptr;
+      if (t < kArrays) fetch_row<T>(p, ahead.row, t, mine + i * slot_bytes, &bar[i]);
+  const bool post = ALL || p.w_post != nullptr, pre = ALL || p.w_pre != nullptr,
+             cot = ALL || p.in[3] != nullptr;   // (the cotangent of h')
   const Params pa = {p.w_post, p.w_pre, p.gate, p.alpha, p.offset, p.H};
   const Columns<T, VEC> cols{pa, t, tpr};
   F2 S[Q][2], sw[Q][2];     // sums of d y r1 and of dx h' r2
@@ -409,13 +405,12 @@ __global__ void __launch_bounds__(THREADS, WARP ? 2 : 1) bwd_kernel(const __grid
       for (int q = 0; q < Q; ++q) {
         F2 v[2], u[2];
         cols.alpha_ag(g, q, v);
-        cols.b(q, u);
         if (W == W_REG) {
+          cols.b(q, u);
 #pragma unroll
           for (int j = 0; j < 2; ++j) ag[W == W_REG ? q : 0][j] = v[j], bw[W == W_REG ? q : 0][j] = u[j];
         } else {   // (each thread reads only what it wrote)
-          put4<float, VEC>(ag_s, q, t, tpr, 4 * Q * tpr, v);
-          put4<float, VEC>(b_s, q, t, tpr, 4 * Q * tpr, u);
+          put4<float, VEC>(ag_s, q, t, tpr, room, v);
         }
       }
       held = it.item;
@@ -443,7 +438,7 @@ __global__ void __launch_bounds__(THREADS, WARP ? 2 : 1) bwd_kernel(const __grid
       F2 wv[2];
       read(0, q, y[q]);
       read(1, q, h[q]);
-      if (W == W_SMEM) get4<float, VEC, true>(ag_s, q, t, tpr, 4 * Q * tpr, wv);
+      if (W == W_SMEM) get4<float, VEC, true>(ag_s, q, t, tpr, room, wv);
       if (W == W_MEM) cols.alpha_ag(it.item / p.splits, q, wv);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
@@ -453,7 +448,7 @@ __global__ void __launch_bounds__(THREADS, WARP ? 2 : 1) bwd_kernel(const __grid
       }
       if (pre) {
         read(2, q, u[q]);
-        if (W == W_SMEM) get4<float, VEC, true>(b_s, q, t, tpr, 4 * Q * tpr, wv);
+        if (W == W_SMEM) get4<float, VEC, true>(b_s, q, t, tpr, room, wv);
         if (W == W_MEM) cols.b(q, wv);
       }
 #pragma unroll
@@ -469,12 +464,12 @@ __global__ void __launch_bounds__(THREADS, WARP ? 2 : 1) bwd_kernel(const __grid
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
       F2 wv[2], d[2], e[2];
-      if (p.in[3]) read(3, q, d);
-      if (W == W_SMEM) get4<float, VEC, true>(ag_s, q, t, tpr, 4 * Q * tpr, wv);
+      if (cot) read(3, q, d);
+      if (W == W_SMEM) get4<float, VEC, true>(ag_s, q, t, tpr, room, wv);
       if (W == W_MEM) cols.alpha_ag(it.item / p.splits, q, wv);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        if (!p.in[3]) d[j] = f2_same(0.f);
+        if (!cot) d[j] = f2_same(0.f);
         if (pre) d[j] = f2_fma(f2_same(r2), f2_fma(f2_same(-mu), h[q][j], u[q][j]), d[j]);
         e[j] = f2_mul(d[j], y[q][j]);
         S[q][j] = f2_add(S[q][j], e[j]);
@@ -486,9 +481,10 @@ __global__ void __launch_bounds__(THREADS, WARP ? 2 : 1) bwd_kernel(const __grid
     float mv = team_sum<WARP>(s, red, turn) * inv_H;
     if (!post) mv = 0.f;
     // every thread has read the slot (the sum's barrier; a warp's shuffles): the next row may land
-    if (STAGED && t == 0 && alive && ahead_s[w].item >= 0) {
-      fetch_row<T>(p, ahead_s[w].row, mine + slot * slot_bytes, &bar[slot]);
-      ahead_s[w].next(p, teams);
+    if (STAGED && ahead.item >= 0) {
+      if (t < kArrays && alive)
+        fetch_row<T>(p, ahead.row, t, mine + slot * slot_bytes, &bar[slot]);
+      ahead.next(p, teams);
     }
     if (++slot == p.slots) {
       slot = 0;
@@ -599,7 +595,8 @@ static int fwd_any(const Fwd& p, cudaStream_t st) {
 // How the backward pass runs: as many teams as stay resident, the parts each gate row's rows
 // are cut into so that the teams share them evenly, and the rows in flight per team.
 struct Plan {
-  int threads, blocks, teams, splits, slots, weights;
+  bool warp;
+  int q, threads, blocks, teams, splits, slots, weights;
   uint32_t row_bytes;
   size_t smem;
   int64_t ws;  // floats of workspace
@@ -611,8 +608,13 @@ static Plan bwd_plan(int T, int H, int dtype, int groups, bool gate) {
   Plan pl;
   const bool warp = H <= 256;
   const int q = H <= 8192 ? 2 : (H <= 16384 ? 4 : 8);
-  const int per = warp ? 8 : 1;
-  pl.threads = warp ? 256 : team_threads(H, q);
+  // warps of a block of warp teams: fewer where there are too few rows to give every SM eight
+  int per = 1;
+  if (warp) per = (int)((T + (int64_t)num_sms() - 1) / num_sms());
+  if (per > 8) per = 8;
+  pl.warp = warp;
+  pl.q = q;
+  pl.threads = warp ? 32 * per : team_threads(H, q);
   // room for the whole team's columns (a row is read past H) and for an unaligned start
   const int room = 4 * q * (warp ? 32 : pl.threads);
   pl.row_bytes = (uint32_t)(room * dtype_size(dtype) + 32);
@@ -620,7 +622,7 @@ static Plan bwd_plan(int T, int H, int dtype, int groups, bool gate) {
   const size_t slot = (size_t)kArrays * pl.row_bytes;
   const size_t fix = pl.weights == W_SMEM ? (size_t)8 * room : 0;
   if (q > 2 || slot + fix > kSmemTeam) pl.weights = W_MEM;
-  // teams of an SM: 640 threads of 96 registers (two blocks of eight warp teams)
+  // teams of an SM: 640 threads of 96 registers, or blocks of eight warp teams
   const int sm_blocks = warp ? 2 : (pl.weights == W_REG && pl.threads <= 640 ? 640 / pl.threads : 1);
   pl.slots = 1;
   pl.smem = 0;
@@ -645,7 +647,8 @@ static Plan bwd_plan(int T, int H, int dtype, int groups, bool gate) {
 
 template <typename T, bool VEC, bool WARP, int Q, int W, int THREADS>
 static int bwd_launch(const Bwd& p, const Plan& pl, cudaStream_t st) {
-  auto kern = bwd_kernel<T, VEC, WARP, Q, W, THREADS>;
+  auto kern = p.w_post && p.w_pre && p.in[3] ? bwd_kernel<T, VEC, WARP, Q, W, THREADS, true>
+                                             : bwd_kernel<T, VEC, WARP, Q, W, THREADS, false>;
   if (pl.smem > 48 * 1024 &&
       cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pl.smem) !=
           cudaSuccess)
@@ -657,13 +660,13 @@ static int bwd_launch(const Bwd& p, const Plan& pl, cudaStream_t st) {
 
 template <typename T, bool VEC>
 static int bwd_any(const Bwd& p, const Plan& pl, cudaStream_t st) {
-  if (p.H <= 256) return bwd_launch<T, VEC, true, 2, W_REG, 256>(p, pl, st);
+  if (pl.warp) return bwd_launch<T, VEC, true, 2, W_REG, 256>(p, pl, st);
   if (pl.weights == W_REG) return pl.threads <= 640
                                       ? bwd_launch<T, VEC, false, 2, W_REG, 640>(p, pl, st)
                                       : bwd_launch<T, VEC, false, 2, W_REG, 768>(p, pl, st);
   if (pl.weights == W_SMEM) return bwd_launch<T, VEC, false, 2, W_SMEM, 1024>(p, pl, st);
-  if (p.H <= 8192) return bwd_launch<T, VEC, false, 2, W_MEM, 1024>(p, pl, st);
-  if (p.H <= 16384) return bwd_launch<T, VEC, false, 4, W_MEM, 1024>(p, pl, st);
+  if (pl.q == 2) return bwd_launch<T, VEC, false, 2, W_MEM, 1024>(p, pl, st);
+  if (pl.q == 4) return bwd_launch<T, VEC, false, 4, W_MEM, 1024>(p, pl, st);
   return bwd_launch<T, VEC, false, 8, W_MEM, 1024>(p, pl, st);
 }
 
