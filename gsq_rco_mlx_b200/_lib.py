@@ -86,6 +86,8 @@ SIGNATURES = {
                      _vp, _i32, _i64, _i32, _vp, _vp],
     "gsq_fp8_linear": [_vp, _i32, _i32, _i32, _i64, _vp, _i64, _vp, _i64, _i32, _vp, _i32, _i64,
                        _vp, _i64, _vp, _vp],
+    "gsq_fp8_linear_vjp": [_vp, _i32, _i32, _i32, _i64, _vp, _i32, _i32, _i64, _vp, _i64, _vp,
+                           _i64, _vp, _i64, _vp, _i64, _i32, _vp, _i64, _vp, _vp],
     "gsq_rope": [_vp, _i64, _i64, _i32, _vp, _i64, _i64, _i32, _i64, _i32, _i32, _i32, _i32, _vp,
                  _i32, _vp, _f32, _i32, _vp, _i64, _i64, _vp, _i64, _i64, _vp],
     "gsq_residual_norm": [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _f32,

@@ -7,7 +7,7 @@ holding affine packed weights). Here the checkpoint's packed words stay packed i
 
   PackedLinear   words / scales / biases of one linear; __call__ is qgemm_packed (M <= 8: one
                  fused dequant-GEMV HBM stream; larger M: dequant + tensor-core GEMM)
-  PackedModel    the decoder with packed linears; block(L) dequantizes layer L's seven linears
+  PackedModel    the decoder with packed linears (or Fp8Linear, common/fp8.py); block(L) dequantizes layer L's seven linears
                  into one bf16 scratch set (14.9M weights, 30 MB: it stays in L2 for the block's
                  GEMMs) and returns the block weights the forward engine reads
   LogitHead      bf16(h E^T) chunks of the tied embedding and the NLL row pass
@@ -26,8 +26,8 @@ import torch
 from .. import _lib
 from ..gemm import Terms, gemm
 from ..gsq.e2e import LIN_ORDER, BlockConfig, BlockWeights, Qwen2Block
-from .fp8 import Fp8Linear
 from ..gsq.export import BKEY, NKEY, SafetensorsFile, mlx_bits, module_path, to_mlx_affine
+from .fp8 import Fp8Linear
 
 QGEMV_MAX_ROWS = 8
 
@@ -177,6 +177,14 @@ class PackedModel:
                     q["codes"], q["scales"], q["bits"], q["group_size"], scale_dtype,
                     device=model.embed.device)
             layers.append(d)
+        return cls(model.cfg, model.embed, model.norm, layers)
+
+    @classmethod
+    def from_fp8(cls, model, names=LIN_ORDER):
+        """A QwenModel (bf16 on the GPU) with the linears `names` of every layer in e4m3 with a
+        scale per 128 x 128 (Fp8Linear); the others stay dense."""
+        layers = [{k: Fp8Linear.from_weight(v) if k in names else v for k, v in W.items()}
+                  for W in model.layers]
         return cls(model.cfg, model.embed, model.norm, layers)
 
     @classmethod

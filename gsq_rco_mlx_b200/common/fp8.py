@@ -94,8 +94,9 @@ def _padded(codes):
 
 class Fp8Linear:
     """One linear W [N, K] in e4m3: codes float8_e4m3fn [N, K], scales float32
-    [ceil(N / 128), ceil(K / 128)]. codes_t: the codes transposed [K, N], which the
-    vector-Jacobian product reads (made on its first use otherwise)."""
+    [ceil(N / 128), ceil(K / 128)], both kept as they are where the codes' rows lie on 16 bytes
+    (copied otherwise). codes_t: the codes transposed [K, N], which the vector-Jacobian product
+    reads (made on its first use otherwise)."""
 
     def __init__(self, codes, scales, codes_t=None):
         if codes.dtype != E4M3 or codes.dim() != 2 or not codes.numel():
@@ -116,8 +117,6 @@ class Fp8Linear:
             same_device(codes_t, "codes_t", self.dev)
             self._t = _padded(codes_t)
         self._err = err_flag(codes.device)
-        self._weight = (self.codes.data_ptr(), self.codes.stride(0), self.scales.data_ptr(),
-                        self.scales.shape[1], self.N)
         self._width = pad16(self.K) + 4 * _blocks(self.K)   # workspace bytes of a row
 
     @classmethod
@@ -152,15 +151,10 @@ class Fp8Linear:
             raise ValueError(f"unsupported out dtype {out.dtype}")
         dev = on_device(self.codes, "the weight")
         _, ld = output(out, self.N, self.K, out.dtype, self.codes, "out")
-        _lib.call("gsq_fp8_dequant", *self._weight[:4], self.N, self.K, out.data_ptr(),
+        _lib.call("gsq_fp8_dequant", self.codes.data_ptr(), self.codes.stride(0),
+                  self.scales.data_ptr(), self.scales.shape[1], self.N, self.K, out.data_ptr(),
                   DTYPES[out.dtype], ld, stream_of(dev))
         return out
-
-    def _gemm(self, M, N, K, a, sa, b, sb, sb_rows, sb_n, sb_k, out, ld, accumulate=False):
-        _lib.call("gsq_fp8_gemm", M, N, K, a.data_ptr(), a.stride(0), sa.data_ptr(), M,
-                  b.data_ptr(), b.stride(0), sb.data_ptr(), sb_rows, sb_n, sb_k, out.data_ptr(),
-                  DTYPES[out.dtype], ld, int(accumulate), self._err.data_ptr(),
-                  stream_of(self.dev))
 
     def __call__(self, x, out=None, y_f32=False):
         """y = x W^T [M, N] in x's type (or float32): x [M, K] (bf16, float16 or float32),
@@ -174,8 +168,11 @@ class Fp8Linear:
             y, ld = output(out, M, self.N, torch.float32 if y_f32 else torch.bfloat16,
                            self.codes, "out")
             if M:
-                self._gemm(M, self.N, self.K, x.codes, x.scales, self.codes, self.scales, 0,
-                           self.scales.shape[1], 1, y, ld)
+                _lib.call("gsq_fp8_gemm", M, self.N, self.K, x.codes.data_ptr(), x.codes.stride(0),
+                          x.scales.data_ptr(), x.scales.stride(1) if x.scales.shape[1] > 1 else M,
+                          self.codes.data_ptr(), self.codes.stride(0),
+                          self.scales.data_ptr(), 0, self.scales.shape[1], 1, y.data_ptr(),
+                          DTYPES[y.dtype], ld, 0, self._err.data_ptr(), stream_of(dev))
             return y
         x, ld_x = matrix(x, "x", cols=self.K)
         same_device(x, "x", dev)
@@ -186,9 +183,10 @@ class Fp8Linear:
         # allocated per call on the calling stream: nothing is shared between calls
         nbytes = M * self._width
         ws = x.new_empty((nbytes,), dtype=torch.uint8)
-        _lib.call("gsq_fp8_linear", x.data_ptr(), DTYPES[x.dtype], M, self.K, ld_x, *self._weight,
-                  y.data_ptr(), DTYPES[y.dtype], ld, ws.data_ptr(), nbytes, self._err.data_ptr(),
-                  stream_of(dev))
+        _lib.call("gsq_fp8_linear", x.data_ptr(), DTYPES[x.dtype], M, self.K, ld_x,
+                  self.codes.data_ptr(), self.codes.stride(0), self.scales.data_ptr(),
+                  self.scales.shape[1], self.N, y.data_ptr(), DTYPES[y.dtype], ld, ws.data_ptr(),
+                  nbytes, self._err.data_ptr(), stream_of(dev))
         return y
 
     def vjp(self, x, dy, dx=None, dw=None, accumulate=False):
@@ -210,20 +208,12 @@ class Fp8Linear:
             if not accumulate:
                 dw.zero_()
             return dx, dw
-        wt, sw = self.codes_t(), self.scales
-        st = stream_of(dev)
-        lm, ln, mb = pad16(M), pad16(N), _blocks(M)
+        wt = self.codes_t()
+        nbytes = M * pad16(N) + (N + K) * pad16(M) + 4 * (M * _blocks(N) + (N + K) * _blocks(M))
         # allocated per call on the calling stream: nothing is shared between calls
-        q = x.new_empty((M * ln + (N + K) * lm,), dtype=torch.uint8)
-        s = x.new_empty((_blocks(N) * M + mb * (N + K),), dtype=torch.float32)
-        dyq, dyt, xt = q[:M * ln].view(M, ln), q[M * ln:M * ln + N * lm].view(N, lm), \
-            q[M * ln + N * lm:].view(K, lm)
-        s0, s1 = _blocks(N) * M, _blocks(N) * M + mb * N
-        _lib.call("gsq_fp8_quant", dy.data_ptr(), DTYPES[dy.dtype], M, N, ld_dy,
-                  dyq.data_ptr(), ln, s.data_ptr(), M, dyt.data_ptr(), lm, s[s0:].data_ptr(), N,
-                  st)
-        _lib.call("gsq_fp8_quant", x.data_ptr(), DTYPES[x.dtype], M, K, ld_x, None, 0, None, 0,
-                  xt.data_ptr(), lm, s[s1:].data_ptr(), K, st)
-        self._gemm(M, K, N, dyq, s, wt, sw, 0, 1, sw.shape[1], dx, ld_dx)
-        self._gemm(N, K, M, dyt, s[s0:], xt, s[s1:], 1, 0, K, dw, ld_dw, accumulate)
+        ws = x.new_empty((nbytes,), dtype=torch.uint8)
+        _lib.call("gsq_fp8_linear_vjp", x.data_ptr(), DTYPES[x.dtype], M, K, ld_x, dy.data_ptr(),
+                  DTYPES[dy.dtype], N, ld_dy, wt.data_ptr(), wt.stride(0), self.scales.data_ptr(),
+                  self.scales.shape[1], dx.data_ptr(), ld_dx, dw.data_ptr(), ld_dw, accumulate,
+                  ws.data_ptr(), nbytes, self._err.data_ptr(), stream_of(dev))
         return dx, dw

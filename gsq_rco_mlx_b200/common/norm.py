@@ -84,8 +84,8 @@ def residual_norm(h, y, w_post=None, w_pre=None, gate=None, scale=1.0, eps=1e-6,
         xp = x.data_ptr()
     if T:
         _lib.call("gsq_residual_norm", h.data_ptr(), ld_h, y.data_ptr(), ld_y, _ptr(w_post),
-                  _ptr(w_pre), _ptr(gate), rows, T, H, DTYPES[dt], scale, eps, offset,
-                  h2.data_ptr(), ld_h2, xp, H, codes, ld_c, scales, T, stats.data_ptr(),
+                  _ptr(w_pre), _ptr(gate), rows, T, H, DTYPES[dt], float(scale),
+                  float(eps), float(offset), h2.data_ptr(), ld_h2, xp, H, codes, ld_c, scales, T, stats.data_ptr(),
                   stream_of(dev))
     return h2, x, stats
 
@@ -128,7 +128,7 @@ def residual_norm_vjp(h, y, w_post, w_pre, stats, dh, dx, gate=None, scale=1.0, 
     ws = h.new_empty((n.value,), dtype=torch.uint8)
     _lib.call("gsq_residual_norm_bwd", h.data_ptr(), ld_h, y.data_ptr(), ld_y, _ptr(w_post),
               _ptr(w_pre), _ptr(gate), rows, stats.data_ptr(), _ptr(dh), ld_dh, _ptr(dx), ld_dx, T,
-              H, DTYPES[dt], scale, offset, g["dh"].data_ptr(), H, g["dy"].data_ptr(), H,
+              H, DTYPES[dt], float(scale), float(offset), g["dh"].data_ptr(), H, g["dy"].data_ptr(), H,
               _ptr(g["dw_post"]), _ptr(g["dw_pre"]), _ptr(g["dgate"]), ws.data_ptr(), n.value,
               err_flag(h.device).data_ptr(), stream_of(dev))
     return g

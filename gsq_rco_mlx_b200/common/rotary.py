@@ -90,7 +90,6 @@ class Rotary:
         self.layout = layout
         self.freqs, self.factor = frequencies(self.rotary_dim, theta, scaling)
         self.turns = torch.from_numpy(self.freqs / (2 * math.pi)).to(device or _lib.device())
-        self._turns, self._pairs = self.turns.data_ptr(), int(layout == "interleaved")
 
     def _side(self, x, T, dtype, dev, what):
         """Strides of tokens and heads, and the heads, of x [T, heads, head_dim]."""
@@ -144,8 +143,8 @@ class Rotary:
             ko_t, ko_h = (0, 0) if k is None else self._out_side(ko, k, T, dt, dev, "k_out")
         if T:
             _lib.call("gsq_rope", q.data_ptr(), q_t, q_h, nq, k.data_ptr() if nk else None, k_t,
-                      k_h, nk, T, hd, self.rotary_dim, self._pairs, code, positions.data_ptr(),
-                      wide, self._turns, self.factor, inverse, qo.data_ptr(), qo_t, qo_h,
+                      k_h, nk, T, hd, self.rotary_dim, self.layout == "interleaved", code, positions.data_ptr(),
+                      wide, self.turns.data_ptr(), self.factor, inverse, qo.data_ptr(), qo_t, qo_h,
                       ko.data_ptr() if nk else None, ko_t, ko_h, stream_of(dev))
         return qo, ko
 

@@ -1338,3 +1338,40 @@ extern "C" int gsq_fp8_linear(const void* x, int dtype, int M, int K, int64_t ld
   return fp8_gemm(M, N, K, q, ld_q, sq, M, codes, ld_codes, scales, 0, ld_scales, 1, y, y_dtype,
                   ld_y, 0, err, true, stream);
 }
+
+extern "C" int gsq_fp8_linear_vjp(const void* x, int dtype, int M, int K, int64_t ld_x,
+                                  const void* dy, int dy_dtype, int N, int64_t ld_dy,
+                                  const void* codes_t, int64_t ld_codes_t, const float* scales,
+                                  int64_t ld_scales, void* dx, int64_t ld_dx, float* dw,
+                                  int64_t ld_dw, int accumulate, void* workspace,
+                                  int64_t workspace_bytes, int* err, void* stream) {
+  if (M <= 0 || K <= 0 || N <= 0 || !workspace || (uintptr_t)workspace % 16) return GSQ_EINVAL;
+  const auto blocks = [](int64_t n) { return (n + fp8::kBlk - 1) / fp8::kBlk; };
+  const int64_t ln = ((int64_t)N + 15) / 16 * 16, lm = ((int64_t)M + 15) / 16 * 16;
+  const int64_t codes = M * ln + ((int64_t)N + K) * lm,
+                need = codes + 4 * (blocks(N) * M + blocks(M) * ((int64_t)N + K));
+  if (workspace_bytes < need || ld_scales < blocks(K) || blocks(M) > 65535) return GSQ_EINVAL;
+  // dy in rows along N, dy and x in columns (blocks of 128 rows), transposed
+  auto* dyq = (uint8_t*)workspace;
+  auto* dyt = dyq + M * ln;
+  auto* xt = dyt + N * lm;
+  auto* s_dy = (float*)(dyq + codes);
+  float *s_dyt = s_dy + blocks(N) * M, *s_xt = s_dyt + blocks(M) * N;
+  if (!fp8::quant_ok(x, dtype, M, K, ld_x) || !fp8::quant_ok(dy, dy_dtype, M, N, ld_dy) ||
+      !fp8::gemm_ok(M, K, N, dyq, ln, s_dy, M, codes_t, ld_codes_t, scales, 0, 1, ld_scales, dx,
+                    dtype, ld_dx, 0, err) ||
+      !fp8::gemm_ok(N, K, M, dyt, lm, s_dyt, N, xt, lm, s_xt, 1, 0, K, dw, F32, ld_dw, accumulate,
+                    err))
+    return GSQ_EINVAL;
+  cudaStream_t st = (cudaStream_t)stream;
+  int s = fp8::quant_any(dy, dy_dtype, M, N, ld_dy, dyq, ln, s_dy, M, dyt, lm, s_dyt, N, false, st);
+  if (s == GSQ_OK)
+    s = fp8::quant_any(x, dtype, M, K, ld_x, nullptr, 0, nullptr, 0, xt, lm, s_xt, K, false, st);
+  if (s == GSQ_OK)
+    s = fp8_gemm(M, K, N, dyq, ln, s_dy, M, codes_t, ld_codes_t, scales, 0, 1, ld_scales, dx, dtype,
+                 ld_dx, 0, err, false, stream);
+  if (s == GSQ_OK)
+    s = fp8_gemm(N, K, M, dyt, lm, s_dyt, N, xt, lm, s_xt, 1, 0, K, dw, F32, ld_dw, accumulate, err,
+                 false, stream);
+  return s;
+}

@@ -545,6 +545,18 @@ int gsq_fp8_linear(const void *x, int dtype, int M, int K, int64_t ld_x, const v
                    int y_dtype, int64_t ld_y, void *workspace, int64_t workspace_bytes, int *err,
                    void *stream);
 
+/* Its vector-Jacobian product for the cotangent dy [M][ld_dy], the rounding counted as the
+ * identity: dx [M][ld_dx] = dy W in dtype (x's) with dy quantized in row form along N and W's own
+ * codes, given transposed (codes_t [K][ld_codes_t]); dw float32 [N][ld_dw] = dy^T x (added if
+ * accumulate) with dy and x quantized in column form (blocks of 128 rows). Four launches.
+ * workspace: 16-byte aligned, >= M ceil16(N) + (N + K) ceil16(M) + 4 (M ceil(N / 128) +
+ * (N + K) ceil(M / 128)) bytes. */
+int gsq_fp8_linear_vjp(const void *x, int dtype, int M, int K, int64_t ld_x, const void *dy,
+                       int dy_dtype, int N, int64_t ld_dy, const void *codes_t, int64_t ld_codes_t,
+                       const float *scales, int64_t ld_scales, void *dx, int64_t ld_dx, float *dw,
+                       int64_t ld_dw, int accumulate, void *workspace, int64_t workspace_bytes,
+                       int *err, void *stream);
+
 /* ---- rotary positions ----
  * q [T][nq][head_dim] and k [T][nk][head_dim] (nk 0: none) through element strides of tokens
  * and heads (the head's elements contiguous) to q_out, k_out (strides of their own; the inputs

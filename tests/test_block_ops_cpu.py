@@ -197,6 +197,16 @@ def test_fp8_entry_points_refuse_bad_arguments():
               (13, odd), (14, 8 * 216 - 1), (15, None)])
 
 
+def test_fp8_vjp_entry_point_refuses_bad_arguments():
+    lib = _lib.load()
+    need = 8 * 16 + (16 + 200) * 16 + 4 * (8 * 1 + (16 + 200) * 1)
+    ok = [P, 0, 8, 200, 200, P, 0, 16, 16, P, 16, P, 2, P, 200, P, 200, 0, P, need, P, None]
+    _refused(lib.gsq_fp8_linear_vjp, ok,
+             [(0, None), (1, 3), (2, 0), (3, 0), (4, 199), (5, None), (6, -1), (7, 0), (8, 15),
+              (9, None), (10, 15), (11, None), (12, 1), (13, None), (14, 199), (15, None),
+              (16, 199), (18, None), (18, C.c_void_p(4100)), (19, need - 1), (20, None)])
+
+
 def test_rope_entry_point_refuses_bad_arguments():
     lib = _lib.load()
     ok = [P, 128, 64, 2, P, 128, 64, 1, 4, 64, 32, 0, 0, P, 0, P, 1.0, 0, P, 128, 64, P, 64, 64, None]

@@ -2,6 +2,8 @@
 oracles, at the sizes, layouts and values where they can go wrong. The tolerances count roundings:
 u = 2^-24 of float32, half a step of the output's type, and the number of float32 operations
 between input and output, each applied to the magnitudes that the operation adds up."""
+from types import SimpleNamespace
+
 import numpy as np
 import pytest
 import torch
@@ -159,6 +161,11 @@ def test_fp8_strides_outputs_and_refusals():
     assert bool((buf[:, :3] == 7).all()) and bool((buf[:, 3 + N:] == 7).all())
     xt = x.t().contiguous().t()
     assert torch.equal(lin(xt), want)
+    # rows of a quantized tensor (scales of a larger pitch), one of them, and from its first block
+    q = quantize_rows(x)
+    for r0, r1 in ((2, 7), (4, 5), (0, 9)):
+        part = Fp8Tensor(q.codes[r0:r1], q.scales[r0:r1])
+        assert torch.equal(lin(part), want[r0:r1]), (r0, r1)
     e = lin(x[:0])
     assert e.shape == (0, N)
     dx, dw = lin.vjp(x[:0], want[:0])
@@ -621,24 +628,28 @@ def test_fp8_layers_in_the_packed_eval():
     shapes = {"q_proj": (128, 128), "k_proj": (64, 128), "v_proj": (64, 128), "o_proj": (128, 128),
               "gate_proj": (256, 128), "up_proj": (256, 128), "down_proj": (128, 256)}
     bf = torch.bfloat16
-    layers8, layers16 = [], []
+    layers, layers16 = [], []
     for L in range(2):
         d = {"q_bias": rnd((128,), 100 + L, bf, 0.1), "k_bias": rnd((64,), 110 + L, bf, 0.1),
              "v_bias": rnd((64,), 120 + L, bf, 0.1),
              "in_norm": torch.ones(128, device="cuda", dtype=bf),
              "post_norm": torch.ones(128, device="cuda", dtype=bf)}
-        d8, d16 = dict(d), dict(d)
+        d16 = dict(d)
         for i, name in enumerate(LIN_ORDER):
-            lin = Fp8Linear.from_weight(rnd(shapes[name], 10 * L + i, bf, 0.08))
-            d8[name] = lin
+            d[name] = rnd(shapes[name], 10 * L + i, bf, 0.08)
             d16[name] = torch.empty(shapes[name], device="cuda", dtype=bf)
-            lin.dequant(d16[name])
-        layers8.append(d8)
+            Fp8Linear.from_weight(d[name]).dequant(d16[name])
+        layers.append(d)
         layers16.append(d16)
     embed, nw = rnd((512, 128), 200, bf), torch.ones(128, device="cuda", dtype=bf)
     win = np.random.default_rng(0).integers(0, 512, (3, 128))
-    m8, m16 = PackedModel(cfg, embed, nw, layers8), PackedModel(cfg, embed, nw, layers16)
+    m8 = PackedModel.from_fp8(SimpleNamespace(cfg=cfg, embed=embed, norm=nw, layers=layers))
+    m16 = PackedModel(cfg, embed, nw, layers16)
     a, b = perplexity(m8, win), perplexity(m16, win)
     assert a == b and np.isfinite(a["ppl"])
     n = sum(r * c + 4 * -(-r // 128) * -(-c // 128) for r, c in shapes.values())
     assert m8.packed_bytes() == 2 * n and m16.packed_bytes() == 0
+    some = PackedModel.from_fp8(SimpleNamespace(cfg=cfg, embed=embed, norm=nw, layers=layers),
+                                names=("up_proj",))
+    assert some.packed_bytes() == 2 * (256 * 128 + 4 * 2) and some.layers[0]["q_proj"] is \
+        layers[0]["q_proj"]
