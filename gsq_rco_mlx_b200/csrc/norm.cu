@@ -554,9 +554,16 @@ reduce_kernel(Reduce r0, Reduce r1, Reduce r2, int H) {
   const Reduce& r = blockIdx.y == 0 ? r0 : (blockIdx.y == 1 ? r1 : r2);
   if (!r.out) return;
   float a = 0.f;
-  if (col < H) {
-#pragma unroll 8
-    for (int i = w; i < r.n; i += 32) a += r.part[(o * r.outer + i) * r.stride + col];
+  // eight loads in flight a thread, also where fewer are left
+  for (int i0 = w; i0 < r.n; i0 += 256) {
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int i = i0 + 32 * j;
+      v[j] = col < H && i < r.n ? r.part[(o * r.outer + i) * r.stride + col] : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) a += v[j];
   }
   s[w][lane] = a;
   __syncthreads();

@@ -76,7 +76,7 @@ __device__ __forceinline__ T* side_out(const Args& p, int h, int64_t t) {
              : reinterpret_cast<T*>(p.k.out) + t * p.k.out_t + (h - p.q.heads) * p.k.out_h;
 }
 
-constexpr int kBatch = 4;  // heads a thread turns at most
+constexpr int kBatch = 4;  // heads whose loads are in flight before the first is turned
 
 // V elements a load. Halves: lane v < rot / 2 / V holds elements v V.. and their partners
 // rot / 2 further. Pairs (INTER): lane v < rot / V holds V / 2 pairs (V = 1: a pair, two
@@ -98,16 +98,18 @@ __global__ void __launch_bounds__(256) rope_kernel(const __grid_constant__ Args 
     const int d = INTER ? 1 : p.rot / 2;  // where the partner of an element lies
     constexpr bool kTwo = !INTER || V == 1;
     Vec<T, V> x[kBatch], y[kTwo ? kBatch : 1];
-    // all of the thread's heads are on their way while the angles are worked out
+    auto load = [&](int h0) {
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b) {
-      const int h = c + b * p.chunks;
-      if (h < heads) {
-        const T* in = side_in<T>(p, h, t) + o1;
-        x[b] = ld<T, V>(in);
-        if (kTwo && turn) y[kTwo ? b : 0] = ld<T, V>(in + d);
+      for (int b = 0; b < kBatch; ++b) {
+        const int h = h0 + b * p.chunks;
+        if (h < heads) {
+          const T* in = side_in<T>(p, h, t) + o1;
+          x[b] = ld<T, V>(in);
+          if (kTwo && turn) y[kTwo ? b : 0] = ld<T, V>(in + d);
+        }
       }
-    }
+    };
+    load(c);   // the first heads are on their way while the angles are worked out
     float cs[NP], sn[NP];
     if (turn) {
       const double pos = p.pos64 ? (double)reinterpret_cast<const int64_t*>(p.pos)[t]
@@ -122,31 +124,34 @@ __global__ void __launch_bounds__(256) rope_kernel(const __grid_constant__ Args 
         sn[j] = s * (p.factor * p.sign);
       }
     }
+    for (int h0 = c; h0 < heads; h0 += kBatch * p.chunks) {
+      if (h0 != c) load(h0);
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b) {
-      const int h = c + b * p.chunks;
-      if (h < heads) {
-        T* out = side_out<T>(p, h, t) + o1;
-        if (turn) {
-          if (!kTwo) {
+      for (int b = 0; b < kBatch; ++b) {
+        const int h = h0 + b * p.chunks;
+        if (h < heads) {
+          T* out = side_out<T>(p, h, t) + o1;
+          if (turn) {
+            if (!kTwo) {
 #pragma unroll
-            for (int j = 0; j < NP; ++j) {
-              const float u = to_f32(x[b].e[2 * j]), w = to_f32(x[b].e[V > 1 ? 2 * j + 1 : 0]);
-              x[b].e[2 * j] = from_f32<T>(u * cs[j] - w * sn[j]);
-              x[b].e[V > 1 ? 2 * j + 1 : 0] = from_f32<T>(u * sn[j] + w * cs[j]);
+              for (int j = 0; j < NP; ++j) {
+                const float u = to_f32(x[b].e[2 * j]), w = to_f32(x[b].e[V > 1 ? 2 * j + 1 : 0]);
+                x[b].e[2 * j] = from_f32<T>(u * cs[j] - w * sn[j]);
+                x[b].e[V > 1 ? 2 * j + 1 : 0] = from_f32<T>(u * sn[j] + w * cs[j]);
+              }
+            } else {
+              Vec<T, V>& z = y[kTwo ? b : 0];
+#pragma unroll
+              for (int j = 0; j < NP; ++j) {
+                const float u = to_f32(x[b].e[j]), w = to_f32(z.e[j]);
+                x[b].e[j] = from_f32<T>(u * cs[j] - w * sn[j]);
+                z.e[j] = from_f32<T>(u * sn[j] + w * cs[j]);
+              }
+              st<T, V>(out + d, z);
             }
-          } else {
-            Vec<T, V>& z = y[kTwo ? b : 0];
-#pragma unroll
-            for (int j = 0; j < NP; ++j) {
-              const float u = to_f32(x[b].e[j]), w = to_f32(z.e[j]);
-              x[b].e[j] = from_f32<T>(u * cs[j] - w * sn[j]);
-              z.e[j] = from_f32<T>(u * sn[j] + w * cs[j]);
-            }
-            st<T, V>(out + d, z);
           }
+          st<T, V>(out, x[b]);
         }
-        st<T, V>(out, x[b]);
       }
     }
   }
@@ -172,7 +177,7 @@ static int launch(Args& p, cudaStream_t st) {
   p.lanes = rot_lanes + (same ? 0 : (p.hd - p.rot) / V);
   const int heads = p.q.heads + p.k.heads;
   // Heads a thread turns by its angles: four (16384 x 16 heads of 64: 16.5 us, with two 21.6;
-  // 8191 x 40 of 128: 32.0, with two 48.3, with eight in two turns 35.2), fewer for few tokens,
+  // 8191 x 40 of 128: 32.0, with two 48.3, with eight in two batches 35.2), fewer for few tokens,
   // down to one (a decoded token's heads all at once).
   int walk = kBatch;
   while (walk > 1 && p.T * p.lanes * ((heads + walk - 1) / walk) < (int64_t)num_sms() * 1024)
