@@ -12,10 +12,16 @@
 // The inner sums run on the tensor cores (kind::f8f6f4: exact products, float32 accumulators in
 // TMEM), one accumulator per 128-wide k-block. The scales differ from block to block, so an
 // accumulator cannot run on over k: the epilogue warps read it back, and fold it into float32
-// registers with one multiply-add per value. At the tensor cores' e4m3 rate a 128 x 256 tile
-// takes 512 cycles per k-block; the fold takes 128 x 256 / (4 x 32 lanes) = 256 issue slots of
-// the same cycles on the four schedulers, so it can hide behind the MMAs as long as an
-// accumulator is free to go on: two of 256 columns (or four of 128) fill TMEM.
+// registers with one multiply-add per value, two values an instruction.
+//
+// What bounds it (8191 x 8192 x 4096 on B200: 260 us, 2.1 PFLOP/s, at the 1.35 GHz or so that the
+// power cap leaves): at the e4m3 rate a 128 x 256 tile takes 512 cycles per k-block, and these
+// 260 us are about 790 each. The fold of one takes 128 packed multiply-adds on each of the four
+// schedulers, measured alone at 2.2 cycles each with two warps and 5.4 with one, and the reads of
+// TMEM and the waits between leave a warp alone for part of the time. Tried and dropped: 16
+// epilogue warps (327 against 296 us), the next columns read while these are folded (321 against
+// 285). The loops of the other warps have to stay shorter than the fold: run by one lane, the MMA
+// warp's took 840 cycles a k-block, so its control is uniform over the warp.
 #include <cuda_fp8.h>
 
 #include <type_traits>
@@ -122,7 +128,7 @@ __device__ __forceinline__ void put_rows(const Four<T> raw[R], const uint32_t m[
 
 // Rows: a warp takes eight rows of one 128-column block, four columns a lane (a row's maximum is
 // one warp reduction, the eight scales are neighbours). One pass over x, eight rows' loads in
-// flight: bound by its bytes.
+// flight: bound by its bytes (8191 x 4096 float16: 19 us, 5.3 TB/s).
 constexpr int kRowsWarp = 8;
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256, 4)
@@ -161,6 +167,7 @@ quant_rows_kernel(const T* __restrict__ x, int64_t ld_x, int rows, int cols, int
 //           lane's sixteen rows of a column are one 16-byte chunk of the transposed row, swizzled
 //           in shared memory so that neither the writes nor the reads of chunks conflict
 //   BLOCKS  one scale for the tile   -> codes, scales [rows / 128][ld_s]
+// 4094 x 4864 bf16 in rows and columns: 18.5 us, 4.3 TB/s.
 template <typename T, bool VEC, bool ROWS, bool COLS, bool BLOCKS>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 && (VEC || !ROWS) ? 3 : 2)
 quant_tile_kernel(const T* __restrict__ x, int64_t ld_x, int rows, int cols,
@@ -931,6 +938,7 @@ static int launch_gemm(GemmArgs& p, const void* b, int64_t ldb, int dtype, bool 
 // k-blocks through kSkStages stages and folds each with the scales of its 128 x 128 block and of
 // the columns; the partial sums meet in the first CTAs' shared memory in the order of the ranks.
 // The weight's first stages are loaded before the activations are quantized (grid_wait).
+// 16 x 8192 x 8192: 67 MB in 16.5 us, 4.1 TB/s; 1 x 896 x 1152: 5.3 us with the quantization.
 constexpr int kSkStages = 5;
 constexpr int kSkThreads = 256;
 
@@ -1284,17 +1292,19 @@ static int fp8_gemm(int M, int N, int K, const void* a, int64_t lda, const float
   if (p.boxes && !fp8::out_map(&p.o, out, dtype, M, N, ld_out)) return GSQ_ECUDA;
   p.err = err;
   cudaStream_t st = (cudaStream_t)stream;
-  // Few rows: bound by the weight's bytes (16 x 8192 x 8192: 31 us on 128-row tiles of A, half of
-  // the SMs idle; see skinny_kernel for its figure).
+  // Few rows: bound by the weight's bytes (16 x 8192 x 8192 with its quantization: 31 us on
+  // 128-row tiles of A, which leave half of the SMs idle, 16.5 us with the weight's rows as the tile
+  // and k shared out over clusters).
   if (M <= fp8::kSkRows && !sb_rows && !accumulate)
     return M <= 16   ? fp8::launch_skinny<16>(p, a, lda, b, ldb, dtype, follows, st)
            : M <= 32 ? fp8::launch_skinny<32>(p, a, lda, b, ldb, dtype, follows, st)
                      : fp8::launch_skinny<64>(p, a, lda, b, ldb, dtype, follows, st);
   // Tile by the time of the rounds that the busiest SM walks: 256 x 256 of a pair, 256 x 128 of a
-  // pair, or 128 x 128 of one SM. A k-block of the narrow tiles takes 0.64 and 0.7 of the wide
-  // one's time (8191 x 8192 x 4096: 251, 330 and 365 us), so they are taken where they need
-  // fewer rounds (4864 x 896 x 4094: 76 wide tiles are two rounds of 74 pairs, 133 narrow ones
-  // two of 0.64).
+  // pair, or 128 x 128 of one SM. A k-block of the narrow tiles takes 0.64 to 0.7 of the wide
+  // one's time (with the quantization, 8191 x 4096 -> 8192: 288, 398 and 400 us, 16384 x 896 ->
+  // 4864: 94, 118 and 117), so they are taken where they need fewer rounds (4864 x 896 x 4094: 76
+  // wide tiles are two rounds of 74 pairs, 133 narrow ones two of 0.64: the whole vjp of 4094 x
+  // 896 -> 4864 takes 132, 96 and 94 us with one tile for both products, 88 with this choice).
   const auto rounds = [&](int rows, int bn, int sms) {
     return (double)(((int64_t)((M + rows - 1) / rows) * ((N + bn - 1) / bn) * sms + num_sms() - 1) /
                     num_sms());

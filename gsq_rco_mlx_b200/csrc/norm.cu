@@ -12,10 +12,15 @@
 // With p = d y r1 the three parameter sums come from one: S = sum p over the rows of one gate row,
 //   dg = alpha a S,  dw_post = sum over gate rows of alpha g S.
 // Both directions are one pass over their rows, held in registers by a team of threads (a warp
-// up to 256 columns, a block above: eight columns a thread), so they are bound by the bytes of
-// the rows. Rows that start on 16 bytes are read as vectors of eight columns; others column by
-// column with the columns dealt round the team, which keeps every access of a warp one segment
-// (eight neighbouring columns a thread would touch each sector eight times).
+// up to 256 columns, a block above: eight columns a thread), so they should be bound by the bytes
+// of the rows. Rows that start on 16 bytes are read in fours of neighbouring columns; others
+// column by column with the columns dealt round the team, which keeps every access of a warp one
+// segment (neighbouring columns a thread would touch each sector several times).
+// Measured: 16384 x 896 bf16 into e4m3 rows 31 us (3.3 TB/s, an instruction issued on 70 % of the
+// schedulers' cycles), its gradient with a gate 50 us (3.5 TB/s, 56 %), the gradient of 6141 x 5121
+// float16, column by column, 157 us. At the same bytes' time the gradient of 16384 x 896 reaches
+// 71 % of the copy rate in float32 and 54 % in bf16: what bounds the 16-bit forms is the
+// instructions of a column and the barriers of a row's sums, not the bytes.
 // The column sums of the backward pass: each team adds its rows in registers and writes one
 // partial row; a second kernel adds the partials in a fixed order (no atomics: the same inputs
 // give the same bits).
@@ -156,7 +161,8 @@ struct Columns {
 
 // Persistent teams: team i takes rows i, i + teams, ...; the parameters' columns stay in
 // registers (HOLD) where the team leaves room for them, and the next row's loads are issued
-// before this row is worked on.
+// before this row is worked on (16384 x 896 into e4m3 rows: 44 us before the two, 35 with
+// them).
 template <typename T, bool VEC, bool WARP, int Q, bool HOLD, bool FP8, int THREADS>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) fwd_kernel(const __grid_constant__ Fwd p) {
   __shared__ __align__(16) float red[2][32];
