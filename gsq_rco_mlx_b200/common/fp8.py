@@ -96,7 +96,8 @@ class Fp8Linear:
     """One linear W [N, K] in e4m3: codes float8_e4m3fn [N, K], scales float32
     [ceil(N / 128), ceil(K / 128)], both kept as they are where the codes' rows lie on 16 bytes
     (copied otherwise). codes_t: the codes transposed [K, N], which the vector-Jacobian product
-    reads (made on its first use otherwise)."""
+    reads (made on its first use otherwise, and not while a graph is captured). The codes are not
+    to be written to afterwards."""
 
     def __init__(self, codes, scales, codes_t=None):
         if codes.dtype != E4M3 or codes.dim() != 2 or not codes.numel():
@@ -140,8 +141,14 @@ class Fp8Linear:
     def codes_t(self):
         """The codes transposed [K, N]."""
         if self._t is None:
+            if torch.cuda.is_current_stream_capturing():
+                # they would be written at the graph's replays only, and read by every call
+                raise RuntimeError("the transposed codes cannot be made during a graph capture: "
+                                   "call codes_t() before it")
             t = torch.zeros(self.K, pad16(self.N), device=self.codes.device, dtype=torch.uint8)
             t[:, :self.N].copy_(self.codes.view(torch.uint8).t())
+            # the next call may come on any stream (once a weight)
+            torch.cuda.current_stream(self.dev).synchronize()
             self._t = t.view(E4M3)[:, :self.N]
         return self._t
 

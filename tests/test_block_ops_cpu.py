@@ -171,6 +171,16 @@ def _refused(fn, ok, bad, status=_lib.GSQ_EINVAL):
         assert fn(*args) == status, (i, v)
 
 
+def test_transposed_codes_are_not_made_during_a_capture(monkeypatch):
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    lin = fp8.Fp8Linear.__new__(fp8.Fp8Linear)
+    lin.N, lin.K, lin._t = 16, 32, None
+    lin.codes = torch.zeros(16, 32, dtype=torch.uint8).view(torch.float8_e4m3fn)
+    with pytest.raises(RuntimeError, match="before it"):
+        lin.codes_t()
+    assert lin._t is None
+
+
 def test_fp8_entry_points_refuse_bad_arguments():
     lib = _lib.load()
     odd = C.c_void_p(4097)

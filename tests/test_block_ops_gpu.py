@@ -618,6 +618,40 @@ def test_captured_graphs_streams_and_overlapping_calls():
     _err_ok()
 
 
+def test_transposed_codes_are_there_for_every_stream():
+    """A weight's first vjp behind other work of its stream, the second at once on another one; and
+    a capture that would have to make the codes is refused, with eager calls as right after it."""
+    from gsq_rco_mlx_b200.common.fp8 import Fp8Linear
+    W, x, dy = rnd((640, 512), 1, torch.bfloat16), rnd((96, 512), 2, torch.bfloat16), \
+        rnd((96, 640), 3, torch.bfloat16)
+    want = Fp8Linear.from_weight(W, transposed=True).vjp(x, dy)
+    lin = Fp8Linear.from_weight(W)
+    busy = torch.zeros(1 << 28, device="cuda")
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s1):
+        for _ in range(20):
+            busy.add_(1.0)
+        a = lin.vjp(x, dy)
+    with torch.cuda.stream(s2):
+        b = lin.vjp(x, dy)
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for g in (a, b) for p, q in zip(g, want))
+    lin = Fp8Linear.from_weight(W)
+    with pytest.raises(RuntimeError, match="before it"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            lin.vjp(x, dy)
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(lin.vjp(x, dy), want))
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        c = lin.vjp(x, dy)
+    gr.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(c, want))
+    _err_ok()
+
+
 def test_fp8_layers_in_the_packed_eval():
     """PackedModel takes Fp8Linear layers: its scratch weights are their dequantized values, and
     the perplexity is that of the dense model with those weights."""
