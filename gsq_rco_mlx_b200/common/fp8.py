@@ -18,8 +18,7 @@ from __future__ import annotations
 import torch
 
 from .. import _lib
-from ..gemm import err_flag
-from .operands import DTYPES, matrix, on_device, output, same_device, stream_of
+from .operands import DTYPES, error_word, matrix, on_device, output, same_device, stream_of
 
 BLOCK = 128
 E4M3 = torch.float8_e4m3fn
@@ -117,7 +116,7 @@ class Fp8Linear:
                 raise ValueError(f"codes_t must be float8_e4m3fn [{self.K}, {self.N}]")
             same_device(codes_t, "codes_t", self.dev)
             self._t = _padded(codes_t)
-        self._err = err_flag(codes.device)
+        self._err = error_word(codes.device)
         self._width = pad16(self.K) + 4 * _blocks(self.K)   # workspace bytes of a row
 
     @classmethod

@@ -17,9 +17,8 @@ import ctypes as C
 import torch
 
 from .. import _lib
-from ..gemm import err_flag
 from .fp8 import Fp8Tensor, pad16
-from .operands import DTYPES, matrix, on_device, output, same_device, stream_of
+from .operands import DTYPES, error_word, matrix, on_device, output, same_device, stream_of
 
 MAX_WIDTH = 32768
 
@@ -130,5 +129,5 @@ def residual_norm_vjp(h, y, w_post, w_pre, stats, dh, dx, gate=None, scale=1.0, 
               _ptr(w_pre), _ptr(gate), rows, stats.data_ptr(), _ptr(dh), ld_dh, _ptr(dx), ld_dx, T,
               H, DTYPES[dt], float(scale), float(offset), g["dh"].data_ptr(), H, g["dy"].data_ptr(), H,
               _ptr(g["dw_post"]), _ptr(g["dw_pre"]), _ptr(g["dgate"]), ws.data_ptr(), n.value,
-              err_flag(h.device).data_ptr(), stream_of(dev))
+              error_word(h.device).data_ptr(), stream_of(dev))
     return g

@@ -5,6 +5,8 @@ from __future__ import annotations
 
 import torch
 
+from .. import gemm
+
 DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
@@ -29,6 +31,14 @@ def same_device(t, what, dev):
 def stream_of(dev):
     """The current stream's handle on device `dev`."""
     return torch._C._cuda_getCurrentRawStream(dev)
+
+
+def error_word(device):
+    """The device's error word of bounded waits (gemm.check_err). Made during a capture it would be
+    cleared by every replay, and with it an error that another call left."""
+    if device not in gemm._ERR and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("the first call on a device cannot be captured: make one before")
+    return gemm.err_flag(device)
 
 
 def matrix(t, what, rows=None, cols=None, dtype=None):

@@ -181,6 +181,20 @@ def test_transposed_codes_are_not_made_during_a_capture(monkeypatch):
     assert lin._t is None
 
 
+def test_the_error_word_is_not_made_during_a_capture(monkeypatch):
+    """Nor is one that is there asked for again."""
+    from gsq_rco_mlx_b200 import gemm
+    from gsq_rco_mlx_b200.common import operands
+    dev = torch.device("cpu")
+    monkeypatch.setattr(gemm, "_ERR", {})
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="before"):
+        operands.error_word(dev)
+    assert not gemm._ERR
+    word = gemm.err_flag(dev)
+    assert operands.error_word(dev) is word
+
+
 def test_fp8_entry_points_refuse_bad_arguments():
     lib = _lib.load()
     odd = C.c_void_p(4097)
