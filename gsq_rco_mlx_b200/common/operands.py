@@ -71,3 +71,19 @@ def output(out, rows, cols, dtype, like, what):
     if s1 != 1 and cols > 1 or s0 < cols and rows > 1:
         raise ValueError(f"{what} must have contiguous rows that do not overlap")
     return out, s0 if s0 > cols else cols
+
+
+def row_by_row(out, ld_out, x, ld_x, what, name):
+    """out [rows, cols] is x's own rows, or shares no element with x (of the same type and shape):
+    what a kernel that reads and writes row by row may be given."""
+    rows, cols = x.shape
+    d = out.data_ptr() - x.data_ptr()
+    if not rows or d == 0 and (ld_out == ld_x or rows == 1):
+        return
+    n = x.element_size()
+    if d >= ((rows - 1) * ld_x + cols) * n or -d >= ((rows - 1) * ld_out + cols) * n:
+        return
+    # columns of one wider buffer
+    if ld_out == ld_x and cols * n <= d % (ld_x * n) <= (ld_x - cols) * n:
+        return
+    raise ValueError(f"{what} overlaps {name} without being the same rows")

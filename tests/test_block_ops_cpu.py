@@ -195,6 +195,30 @@ def test_the_error_word_is_not_made_during_a_capture(monkeypatch):
     assert operands.error_word(dev) is word
 
 
+def test_outputs_over_inputs():
+    """row_by_row against the elements themselves: it takes the same rows and every pair without a
+    common element of one pitch or apart as a whole, and no pair with one."""
+    from gsq_rco_mlx_b200.common.operands import row_by_row
+    base = torch.zeros(256, dtype=torch.bfloat16)
+    cell = torch.arange(256)
+    for rows in (1, 2, 3):
+        for cols in (1, 4):
+            for lx in (4, 9):
+                for lo in (4, 9):
+                    for at in range(0, 41):
+                        view = lambda t, ld, o: t[o:].as_strided((rows, cols), (ld, 1), o)  # noqa: E731
+                        xs = set(view(cell, lx, 20).flatten().tolist())
+                        os = set(view(cell, lo, at).flatten().tolist())
+                        same = at == 20 and (lo == lx or rows == 1)
+                        spans = max(os) < min(xs) or min(os) > max(xs)
+                        args = (view(base, lo, at), lo, view(base, lx, 20), lx, "out", "h")
+                        if same or not (os & xs) and (lo == lx or spans):
+                            row_by_row(*args)
+                        elif os & xs:
+                            with pytest.raises(ValueError, match="overlaps h"):
+                                row_by_row(*args)
+
+
 def test_fp8_entry_points_refuse_bad_arguments():
     lib = _lib.load()
     odd = C.c_void_p(4097)

@@ -618,6 +618,24 @@ def test_captured_graphs_streams_and_overlapping_calls():
     _err_ok()
 
 
+def test_residual_norm_refuses_outputs_across_its_inputs():
+    from gsq_rco_mlx_b200.common.norm import residual_norm
+    buf = rnd((9, 64), 5, torch.bfloat16)
+    h, y = buf[:8, :24], buf[:8, 32:56]
+    want = residual_norm(h, y)[0]
+    for out in (buf[1:, :24], buf[:8, 8:32], buf[1:, 32:56], buf[:8, 40:64],
+                buf.flatten()[:8 * 24].view(8, 24)):
+        with pytest.raises(ValueError, match="overlaps"):
+            residual_norm(h, y, out=out)
+    over = h.clone()
+    assert torch.equal(residual_norm(over, y, out=over)[0], want)
+    over = y.clone()
+    assert torch.equal(residual_norm(h, over, out=over)[0], want)
+    wide = buf.clone()
+    assert torch.equal(residual_norm(wide[:8, :24], wide[:8, 24:48], out=wide[:8, 24:48])[0],
+                       residual_norm(h, buf[:8, 24:48])[0])
+
+
 def test_transposed_codes_are_there_for_every_stream():
     """A weight's first vjp behind other work of its stream, the second at once on another one; and
     a capture that would have to make the codes is refused, with eager calls as right after it."""
