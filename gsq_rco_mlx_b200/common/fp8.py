@@ -18,7 +18,7 @@ from __future__ import annotations
 import torch
 
 from .. import _lib
-from .operands import DTYPES, error_word, matrix, on_device, output, same_device, stream_of
+from .operands import DTYPES, MAX_DIM, error_word, matrix, on_device, output, same_device, stream_of
 
 BLOCK = 128
 E4M3 = torch.float8_e4m3fn
@@ -39,6 +39,8 @@ class Fp8Tensor:
 
     def __init__(self, codes, scales):
         R, C = codes.shape
+        if R > MAX_DIM or C > MAX_DIM:
+            raise ValueError(f"codes have more than {MAX_DIM} rows or columns: {(R, C)}")
         if codes.dtype != E4M3 or scales.dtype != torch.float32:
             raise ValueError("codes must be float8_e4m3fn and scales float32")
         if tuple(scales.shape) != (R, _blocks(C)):
@@ -103,6 +105,9 @@ class Fp8Linear:
             raise ValueError(f"codes must be a float8_e4m3fn matrix, got {codes.dtype} "
                              f"{tuple(codes.shape)}")
         self.N, self.K = int(codes.shape[0]), int(codes.shape[1])
+        if self.N > MAX_DIM or self.K > MAX_DIM:
+            raise ValueError(f"codes have more than {MAX_DIM} rows or columns: "
+                             f"{tuple(codes.shape)}")
         if scales.dtype != torch.float32 or \
                 tuple(scales.shape) != (_blocks(self.N), _blocks(self.K)):
             raise ValueError(f"scales must be float32 [{_blocks(self.N)}, {_blocks(self.K)}], "

@@ -7,6 +7,7 @@ import torch
 
 from .. import gemm
 
+MAX_DIM = 1 << 30   # rows or columns of an operand (32-bit counts in the kernels)
 DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
@@ -53,6 +54,8 @@ def matrix(t, what, rows=None, cols=None, dtype=None):
     if rows is not None and r != rows or cols is not None and c != cols:
         raise ValueError(f"{what} must be [{'any' if rows is None else rows}, "
                          f"{'any' if cols is None else cols}], got {tuple(t.shape)}")
+    if r > MAX_DIM or c > MAX_DIM:
+        raise ValueError(f"{what} has more than {MAX_DIM} rows or columns: {tuple(t.shape)}")
     s0, s1 = t.stride()
     if s1 != 1 and c > 1 or s0 < c and r > 1:
         t = t.contiguous()

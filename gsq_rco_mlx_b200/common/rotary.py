@@ -28,6 +28,7 @@ import torch
 from .. import _lib
 from .operands import DTYPES, on_device, same_device, stream_of
 
+MAX_HEADS = 65536
 _KEYS = {"linear": set(), "ntk": set(), "yarn": {"original", "slow", "fast", "attention"},
          "bands": {"original", "low", "high"}}
 
@@ -97,6 +98,8 @@ class Rotary:
         if len(shape) != 3 or x.dtype != dtype or shape[2] != self.head_dim or shape[0] != T:
             raise ValueError(f"{what} must be {dtype} [{T}, heads, {self.head_dim}], got "
                              f"{x.dtype} {tuple(shape)}")
+        if shape[1] > MAX_HEADS:
+            raise ValueError(f"{what} has more than {MAX_HEADS} heads")
         same_device(x, what, dev)
         st, sh, se = x.stride()
         if se != 1 and self.head_dim > 1:

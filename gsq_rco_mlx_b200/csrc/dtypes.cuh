@@ -7,6 +7,9 @@
 
 namespace gsq {
 
+// Rows and columns that a launch takes: 32-bit counts plus a grid's step stay in range.
+constexpr int kMaxDim = 1 << 30;
+
 enum DType { BF16 = 0, F16 = 1, F32 = 2 };
 
 inline size_t dtype_size(int dtype) { return dtype == F32 ? 4 : 2; }

@@ -1201,14 +1201,16 @@ inline bool gemm_ok(int M, int N, int K, const void* a, int64_t lda, const float
                     int64_t ld_sa, const void* b, int64_t ldb, const float* sb, int sb_rows,
                     int64_t sb_n, int64_t sb_k, const void* out, int dtype, int64_t ld_out,
                     int accumulate, const int* err) {
-  return M > 0 && N > 0 && K > 0 && codes_ok(a, lda, K) && codes_ok(b, ldb, K) && sa &&
+  return M > 0 && N > 0 && K > 0 && M <= kMaxDim && N <= kMaxDim && K <= kMaxDim &&
+         codes_ok(a, lda, K) && codes_ok(b, ldb, K) && sa &&
          ld_sa >= M && sb && sb_n >= 0 && sb_k >= 0 && out && dtype >= 0 && dtype <= 2 &&
          ld_out >= N && err && (uintptr_t)out % dtype_size(dtype) == 0 &&
          !(accumulate && dtype != F32) && !(sb_rows && sb_k < N);
 }
 
 inline bool quant_ok(const void* x, int dtype, int rows, int cols, int64_t ld_x) {
-  return x && dtype >= 0 && dtype <= 2 && rows > 0 && cols > 0 && ld_x >= cols &&
+  return x && dtype >= 0 && dtype <= 2 && rows > 0 && cols > 0 && rows <= kMaxDim &&
+         cols <= kMaxDim && ld_x >= cols &&
          (uintptr_t)x % dtype_size(dtype) == 0;
 }
 
@@ -1245,6 +1247,7 @@ extern "C" int gsq_fp8_dequant(const void* codes, int64_t ld_codes, const float*
                                int64_t ld_scales, int N, int K, void* out, int dtype,
                                int64_t ld_out, void* stream) {
   if (!fp8::codes_ok(codes, ld_codes, K) || !scales || N <= 0 || K <= 0 ||
+      N > kMaxDim || K > kMaxDim ||
       ld_scales < (K + 127) / 128 || !out || dtype < 0 || dtype > 2 || ld_out < K ||
       (uintptr_t)out % dtype_size(dtype))
     return GSQ_EINVAL;
@@ -1333,7 +1336,9 @@ extern "C" int gsq_fp8_linear(const void* x, int dtype, int M, int K, int64_t ld
                               const void* codes, int64_t ld_codes, const float* scales,
                               int64_t ld_scales, int N, void* y, int y_dtype, int64_t ld_y,
                               void* workspace, int64_t workspace_bytes, int* err, void* stream) {
-  if (M <= 0 || K <= 0 || N <= 0 || !workspace || (uintptr_t)workspace % 16) return GSQ_EINVAL;
+  if (M <= 0 || K <= 0 || N <= 0 || M > kMaxDim || K > kMaxDim || N > kMaxDim || !workspace ||
+      (uintptr_t)workspace % 16)
+    return GSQ_EINVAL;
   const int64_t ld_q = ((int64_t)K + 15) / 16 * 16;
   const int64_t need = M * ld_q + (int64_t)4 * M * ((K + fp8::kBlk - 1) / fp8::kBlk);
   if (workspace_bytes < need || ld_scales < (K + fp8::kBlk - 1) / fp8::kBlk) return GSQ_EINVAL;
@@ -1355,7 +1360,9 @@ extern "C" int gsq_fp8_linear_vjp(const void* x, int dtype, int M, int K, int64_
                                   int64_t ld_scales, void* dx, int64_t ld_dx, float* dw,
                                   int64_t ld_dw, int accumulate, void* workspace,
                                   int64_t workspace_bytes, int* err, void* stream) {
-  if (M <= 0 || K <= 0 || N <= 0 || !workspace || (uintptr_t)workspace % 16) return GSQ_EINVAL;
+  if (M <= 0 || K <= 0 || N <= 0 || M > kMaxDim || K > kMaxDim || N > kMaxDim || !workspace ||
+      (uintptr_t)workspace % 16)
+    return GSQ_EINVAL;
   const auto blocks = [](int64_t n) { return (n + fp8::kBlk - 1) / fp8::kBlk; };
   const int64_t ln = ((int64_t)N + 15) / 16 * 16, lm = ((int64_t)M + 15) / 16 * 16;
   const int64_t codes = M * ln + ((int64_t)N + K) * lm,

@@ -702,7 +702,7 @@ extern "C" int gsq_residual_norm(const void* h, int64_t ld_h, const void* y, int
                                  float offset, void* h_out, int64_t ld_ho, void* x, int64_t ld_x,
                                  void* codes, int64_t ld_codes, float* scales, int64_t ld_scales,
                                  float* stats, void* stream) {
-  if (T <= 0 || H <= 0 || dtype < 0 || dtype > 2 || !stats) return GSQ_EINVAL;
+  if (T <= 0 || T > kMaxDim || H <= 0 || dtype < 0 || dtype > 2 || !stats) return GSQ_EINVAL;
   const size_t es = dtype_size(dtype);
   if (!norm::row_ok(h, ld_h, H, es) || !norm::row_ok(y, ld_y, H, es)) return GSQ_EINVAL;
   if (gate && (gate_rows <= 0 || T % gate_rows)) return GSQ_EINVAL;
@@ -736,7 +736,7 @@ extern "C" int gsq_residual_norm(const void* h, int64_t ld_h, const void* y, int
 
 extern "C" int gsq_residual_norm_bwd_workspace(int T, int H, int dtype, int gate_rows,
                                                int64_t* bytes) {
-  if (T <= 0 || H <= 0 || dtype < 0 || dtype > 2 || gate_rows < 0 || (gate_rows && T % gate_rows) || !bytes)
+  if (T <= 0 || T > kMaxDim || H <= 0 || dtype < 0 || dtype > 2 || gate_rows < 0 || (gate_rows && T % gate_rows) || !bytes)
     return GSQ_EINVAL;
   *bytes = norm::bwd_plan(T, H, dtype, gate_rows ? gate_rows : 1, gate_rows > 0).ws *
            (int64_t)sizeof(float);
@@ -751,7 +751,7 @@ extern "C" int gsq_residual_norm_bwd(const void* h, int64_t ld_h, const void* y,
                                      int64_t ld_dh, void* dy, int64_t ld_dy, float* dw_post,
                                      float* dw_pre, float* dgate, float* workspace,
                                      int64_t workspace_bytes, int* err, void* stream) {
-  if (T <= 0 || H <= 0 || dtype < 0 || dtype > 2 || !stats || !err) return GSQ_EINVAL;
+  if (T <= 0 || T > kMaxDim || H <= 0 || dtype < 0 || dtype > 2 || !stats || !err) return GSQ_EINVAL;
   const size_t es = dtype_size(dtype);
   if (!norm::row_ok(h, ld_h, H, es) || !norm::row_ok(y, ld_y, H, es) ||
       !norm::row_ok(dh, ld_dh, H, es) || !norm::row_ok(dy, ld_dy, H, es))

@@ -219,6 +219,40 @@ def test_outputs_over_inputs():
                                 row_by_row(*args)
 
 
+def test_sizes_past_32_bit_counts_are_refused():
+    """Not cut to their low 32 bits (2^32 + 4 rows are not four), nor run with counts that a grid's
+    step would overflow."""
+    from gsq_rco_mlx_b200.common.operands import matrix
+    cell = torch.zeros(1, 1, dtype=torch.bfloat16)
+    code = cell.to(torch.float8_e4m3fn)
+    for n in ((1 << 30) + 1, (1 << 32) + 4):
+        for shape in ((n, 1), (1, n)):
+            with pytest.raises(ValueError, match="more than"):
+                matrix(cell.expand(*shape), "x")
+            with pytest.raises(ValueError, match="more than"):
+                fp8.Fp8Tensor(code.expand(*shape), torch.zeros(1, 1))
+            with pytest.raises(ValueError, match="more than"):
+                fp8.Fp8Linear(code.expand(*shape), torch.zeros(1, 1))
+    rot = rotary.Rotary(2, device="cpu")
+    with pytest.raises(ValueError, match="heads"):
+        rot._side(cell.expand(1, (1 << 32) + 4, 2), 1, torch.bfloat16, -1, "q")
+    lib, n = _lib.load(), (1 << 30) + 1
+    assert lib.gsq_fp8_quant(P, 0, n, 1, 1, P, 16, P, n, None, 0, None, 0, None) == _lib.GSQ_EINVAL
+    assert lib.gsq_fp8_gemm(n, 1, 1, P, 16, P, n, P, 16, P, 0, 1, 1, P, 0, 1, 0, P,
+                            None) == _lib.GSQ_EINVAL
+    assert lib.gsq_fp8_dequant(P, 16, P, 1, n, 1, P, 0, 1, None) == _lib.GSQ_EINVAL
+    assert lib.gsq_fp8_linear(P, 0, n, 1, 1, P, 16, P, 1, 1, P, 0, 1, P, 1 << 40, P,
+                              None) == _lib.GSQ_EINVAL
+    assert lib.gsq_fp8_linear_vjp(P, 0, n, 1, 1, P, 0, 1, 1, P, 16, P, 1, P, 1, P, 1, 0, P, 1 << 40,
+                                  P, None) == _lib.GSQ_EINVAL
+    assert lib.gsq_residual_norm(P, 1, P, 1, P, P, None, 0, n, 1, 0, 1.0, 1e-6, 0.0, P, 1, P, 1,
+                                 None, 0, None, 0, P, None) == _lib.GSQ_EINVAL
+    size = C.c_int64()
+    assert lib.gsq_residual_norm_bwd_workspace(n, 1, 0, 0, C.byref(size)) == _lib.GSQ_EINVAL
+    assert lib.gsq_residual_norm_bwd(P, 1, P, 1, P, P, None, 0, P, P, 1, P, 1, n, 1, 0, 1.0, 0.0, P,
+                                     1, P, 1, P, P, None, P, 1 << 40, P, None) == _lib.GSQ_EINVAL
+
+
 def test_fp8_entry_points_refuse_bad_arguments():
     lib = _lib.load()
     odd = C.c_void_p(4097)
