@@ -6,6 +6,8 @@
 """
 from __future__ import annotations
 
+import threading
+
 import torch
 
 from . import _lib
@@ -109,13 +111,31 @@ def split_into(x, terms: Terms, transpose=False):
     return terms
 
 
-_ERR = {}
+_ERR = {}            # device -> the word of its bounded waits
+_UNFILLED = set()    # devices whose word was made in a capture: its fill is the graph's
+_ERR_LOCK = threading.Lock()
 
 
 def err_flag(dev):
-    if dev not in _ERR:
-        _ERR[dev] = torch.zeros(1, device=dev, dtype=torch.int32)
-    return _ERR[dev]
+    """The device's error word, shared by all streams and zero before any of them can have it: a
+    kernel whose wait read what lay there before would give up, and the fill would clear an error
+    set meanwhile. So the fill is waited for, once a device. It cannot be in a capture; the next
+    call outside of one makes up for it."""
+    word = _ERR.get(dev)
+    if word is not None and dev not in _UNFILLED:
+        return word
+    with _ERR_LOCK:
+        word = _ERR.get(dev)
+        if torch.cuda.is_current_stream_capturing():
+            if word is None:
+                word = _ERR[dev] = torch.zeros(1, device=dev, dtype=torch.int32)
+                _UNFILLED.add(dev)
+        elif word is None or dev in _UNFILLED:
+            word = torch.zeros(1, device=dev, dtype=torch.int32) if word is None else word.zero_()
+            torch.cuda.current_stream(dev).synchronize()
+            _ERR[dev] = word
+            _UNFILLED.discard(dev)
+        return word
 
 
 def check_err(dev):

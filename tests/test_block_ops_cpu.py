@@ -195,6 +195,45 @@ def test_the_error_word_is_not_made_during_a_capture(monkeypatch):
     assert operands.error_word(dev) is word
 
 
+class _Waited:
+    """A stream that notes whether the device's word could be had before its fill was waited for."""
+
+    def __init__(self, words, dev, seen):
+        self.words, self.dev, self.seen = words, dev, seen
+
+    def synchronize(self):
+        self.seen.append(self.dev in self.words)
+
+
+def test_the_error_word_is_filled_before_it_can_be_had(monkeypatch):
+    """Another stream's kernels read it: the fill is waited for before the word is kept."""
+    from gsq_rco_mlx_b200 import gemm
+    dev, seen, words = torch.device("cpu"), [], {}
+    monkeypatch.setattr(gemm, "_ERR", words)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda d=None: _Waited(words, dev, seen))
+    word = gemm.err_flag(dev)
+    assert seen == [False] and words[dev] is word and int(word) == 0
+    assert gemm.err_flag(dev) is word and seen == [False]
+
+
+def test_an_error_word_made_in_a_capture_is_filled_by_the_next_eager_call(monkeypatch):
+    """In a capture the fill only runs with the graph; kernels outside of it do not wait for that."""
+    from gsq_rco_mlx_b200 import gemm
+    dev, seen, words = torch.device("cpu"), [], {}
+    monkeypatch.setattr(gemm, "_ERR", words)
+    monkeypatch.setattr(gemm, "_UNFILLED", set())
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda d=None: _Waited(words, dev, seen))
+    word = gemm.err_flag(dev)
+    assert gemm.err_flag(dev) is word and seen == []
+    word.fill_(77)   # what lay there
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    assert gemm.err_flag(dev) is word and int(word) == 0 and len(seen) == 1
+    word.fill_(3)    # an error from then on stays
+    assert gemm.err_flag(dev) is word and int(word) == 3 and len(seen) == 1
+
+
 def test_outputs_over_inputs():
     """row_by_row against the elements themselves: it takes the same rows and every pair without a
     common element of one pitch or apart as a whole, and no pair with one."""

@@ -670,6 +670,33 @@ def test_transposed_codes_are_there_for_every_stream():
     _err_ok()
 
 
+def test_the_error_word_is_there_for_every_stream(monkeypatch):
+    """The device's first call behind other work of its stream, over a block that was left nonzero,
+    and one on another stream at once: the word that both share is zero for both."""
+    from gsq_rco_mlx_b200 import gemm
+    from gsq_rco_mlx_b200.common.fp8 import Fp8Linear
+    W, x = rnd((640, 512), 1, torch.bfloat16), rnd((96, 512), 2, torch.bfloat16)
+    want = Fp8Linear.from_weight(W)(x)
+    busy = torch.zeros(1 << 28, device="cuda")
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    monkeypatch.setattr(gemm, "_ERR", {})
+    with torch.cuda.stream(s1):
+        for n in (1, 8, 64):
+            torch.full((n,), 77, device="cuda", dtype=torch.int32)   # left in s1's pool
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s1):
+        for _ in range(20):
+            busy.add_(1.0)
+        a = Fp8Linear.from_weight(W)(x)
+    with torch.cuda.stream(s2):
+        first = gemm.err_flag(x.device).clone()
+        b = Fp8Linear.from_weight(W)(x)
+    torch.cuda.synchronize()
+    assert int(first) == 0 and len(gemm._ERR) == 1
+    assert torch.equal(a, want) and torch.equal(b, want)
+    _err_ok()
+
+
 def test_fp8_layers_in_the_packed_eval():
     """PackedModel takes Fp8Linear layers: its scratch weights are their dequantized values, and
     the perplexity is that of the dense model with those weights."""
