@@ -3,6 +3,7 @@ on every call of operators that take a few microseconds on the GPU, so they ask 
 and build messages only to raise them."""
 from __future__ import annotations
 
+import numpy as np
 import torch
 
 from .. import gemm
@@ -90,3 +91,107 @@ def row_by_row(out, ld_out, x, ld_x, what, name):
     if ld_out == ld_x and cols * n <= d % (ld_x * n) <= (ld_x - cols) * n:
         return
     raise ValueError(f"{what} overlaps {name} without being the same rows")
+
+
+def runs(t):
+    """Where t [..., C] lies whose last dimension is contiguous: (address, [(bytes from one to the
+    next, how many), ...] of the other dimensions, widest first, bytes of a run of C)."""
+    n = t.element_size()
+    dims = [(s * n, c) for s, c in zip(t.stride()[:-1], t.shape[:-1]) if c > 1]
+    dims.sort(reverse=True)
+    return t.data_ptr(), dims, t.shape[-1] * n
+
+
+def _extent(dims, width):
+    return width + sum((c - 1) * s for s, c in dims)
+
+
+def _surely_apart(da, wa, db, wb, d):
+    """Whether runs of `da`, `wa` at 0 and of `db`, `wb` at d have no byte in common, by their
+    extents: as a whole, or inside a step that both repeat."""
+    if d >= _extent(da, wa) or -d >= _extent(db, wb):
+        return True
+    for s, _ in da:
+        if s and any(s == x for x, _ in db):
+            ia, ib = [x for x in da if x[0] != s], [x for x in db if x[0] != s]
+            if _extent(ia, wa) <= s and _extent(ib, wb) <= s:
+                # bytes in common are so many whole steps apart as bring b to d mod s or s before
+                return _surely_apart(ia, wa, ib, wb, d % s) and \
+                    _surely_apart(ia, wa, ib, wb, d % s - s)
+    return False
+
+
+def box(t):
+    """Where t [T, n, C] lies, in bytes: (address, the wider step, what lies inside it, the whole
+    extent, whether its runs of C are one behind the other as this says). None: nowhere."""
+    if t is None:
+        return 0, 0, 0, 0, True
+    T, n, C = t.shape
+    st, sh, _ = t.stride()
+    e = t.element_size()
+    if T == 1 or n > 1 and sh > st:
+        st, T, sh, n = sh, n, st, T
+    if T == 1:
+        st = 0
+    inner = (n - 1) * sh + C if n > 1 else C
+    return (t.data_ptr(), st * e, inner * e, ((T - 1) * st + inner) * e,
+            (T == 1 or st >= inner) and (n == 1 or sh >= C))
+
+
+def same_rows(a, b):
+    """Whether tensors of one shape and type are the same elements in the same places."""
+    if a.data_ptr() != b.data_ptr():
+        return False
+    s, t = a.stride(), b.stride()
+    return s == t or all(x == y for x, y, c in zip(s, t, a.shape) if c > 1)
+
+
+def boxes_apart(a, b):
+    """Whether two boxes have no byte in common as far as these figures show it."""
+    d = b[0] - a[0]
+    return d >= a[3] or -d >= b[3] or a[1] == b[1] and b[2] <= a[1] and \
+        a[2] <= d % a[1] <= a[1] - b[2]
+
+
+_MOST_RUNS = 1 << 22   # that are compared one by one
+
+
+def _starts(dims):
+    at = np.zeros(1, np.int64)
+    for s, c in dims:
+        at = (at[:, None] + s * np.arange(c, dtype=np.int64)).reshape(-1)
+    return np.sort(at)
+
+
+def _count(dims):
+    n = 1
+    for _, c in dims:
+        n *= c
+    return n
+
+
+def meet(a, b):
+    """Whether two sets of runs have a byte in common (True also for more runs than are compared
+    one by one, where the extents do not settle it)."""
+    (pa, da, wa), (pb, db, wb) = a, b
+    if _surely_apart(da, wa, db, wb, pb - pa):
+        return False
+    if max(_count(da), _count(db)) > _MOST_RUNS:
+        return True
+    A, B = _starts(da), _starts(db) + (pb - pa)
+    i = np.searchsorted(A, B - wa, "right")   # the first run of a that ends behind b's start
+    return bool(np.any(A[np.minimum(i, len(A) - 1)][i < len(A)] < B[i < len(A)] + wb))
+
+
+def repeats(a):
+    """Whether runs lie over one another (True also where it is not settled, as in meet)."""
+    _, dims, width = a
+    room = width
+    for s, c in reversed(dims):
+        if s < room:
+            if _count(dims) > _MOST_RUNS:
+                return True
+            at = _starts(dims)
+            return bool(np.any(at[1:] - at[:-1] < width))
+        room += (c - 1) * s
+    return False

@@ -26,7 +26,8 @@ import numpy as np
 import torch
 
 from .. import _lib
-from .operands import DTYPES, on_device, same_device, stream_of
+from .operands import DTYPES, box, boxes_apart, meet, on_device, repeats, runs, same_device, \
+    same_rows, stream_of
 
 MAX_HEADS = 65536
 _KEYS = {"linear": set(), "ntk": set(), "yarn": {"original", "slow", "fast", "attention"},
@@ -110,11 +111,32 @@ class Rotary:
         st, sh, n = self._side(o, T, dtype, dev, what)
         if n != x.shape[1]:
             raise ValueError(f"{what} must be {tuple(x.shape)}, got {tuple(o.shape)}")
-        if st == 0 and T > 1 or sh == 0 and n > 1:
-            raise ValueError(f"{what} must not repeat its elements")
-        if o.data_ptr() == x.data_ptr() and (st, sh) != x.stride()[:2]:
-            raise ValueError(f"{what} in place must have the strides of its input")
         return st, sh
+
+    @staticmethod
+    def _outputs(q, k, qo, ko):
+        """Refuses outputs that a thread could write before another one has read its input: each
+        lies on its own input, or apart from both inputs, and apart from the other output."""
+        if k is None or not k.numel():
+            k = ko = None
+        # the usual layouts are settled by a few comparisons (every call with `out` comes here)
+        bq, bk, bqo, bko = box(q), box(k), box(qo), box(ko)
+        if bqo[4] and bko[4] and boxes_apart(bqo, bko) and boxes_apart(bqo, bk) and \
+                boxes_apart(bko, bq) and (same_rows(qo, q) or boxes_apart(bqo, bq)) and \
+                (k is None or same_rows(ko, k) or boxes_apart(bko, bk)):
+            return
+        ins = [("q", q, runs(q))] + ([] if k is None else [("k", k, runs(k))])
+        outs = []
+        for (name, x, _), o in zip(ins, (qo, ko)):
+            to, what = runs(o), name + "_out"
+            if repeats(to):
+                raise ValueError(f"{what} must not repeat its elements")
+            for other, _, rows in ins:
+                if not (other == name and same_rows(o, x)) and meet(to, rows):
+                    raise ValueError(f"{what} overlaps {other} without being the same rows")
+            outs.append(to)
+        if len(outs) == 2 and meet(*outs):
+            raise ValueError("k_out overlaps q_out")
 
     def _turn(self, q, k, positions, out, inverse):
         code = DTYPES.get(q.dtype)
@@ -144,6 +166,8 @@ class Rotary:
                 raise ValueError("out must be (q_out, k_out), k_out None without k")
             qo_t, qo_h = self._out_side(qo, q, T, dt, dev, "q_out")
             ko_t, ko_h = (0, 0) if k is None else self._out_side(ko, k, T, dt, dev, "k_out")
+            if T:
+                self._outputs(q, k, qo, ko)
         if T:
             _lib.call("gsq_rope", q.data_ptr(), q_t, q_h, nq, k.data_ptr() if nk else None, k_t,
                       k_h, nk, T, hd, self.rotary_dim, self.layout == "interleaved", code, positions.data_ptr(),
@@ -156,7 +180,7 @@ class Rotary:
         float32), rotated by the tokens' positions int32 / int64 [T]: (q', k'), new contiguous
         tensors or out = (q_out, k_out). Tokens and heads may be strided (views of a packed
         q | k | v buffer, head-major buffers transposed). In place with out = (q, k); any other
-        overlap of input and output is not supported."""
+        overlap of an output with an input or with the other output is refused."""
         return self._turn(q, k, positions, out, False)
 
     def vjp(self, dq, dk, positions, out=None):

@@ -258,6 +258,80 @@ def test_outputs_over_inputs():
                                 row_by_row(*args)
 
 
+def test_runs_that_meet():
+    """meet and repeats against the elements themselves, over strided tensors of three dimensions
+    in one buffer; settled by the extents where they lie as buffers of tokens and heads do."""
+    from gsq_rco_mlx_b200.common import operands
+    rng = np.random.default_rng(7)
+    base = torch.zeros(4096, dtype=torch.float16)
+    cell = torch.arange(4096)
+
+    def some():
+        T, n, hd = (int(rng.integers(1, 5)) for _ in range(3))
+        st, sh = int(rng.integers(0, 40)), int(rng.integers(0, 40))
+        return (T, n, hd), (st, sh, 1), int(rng.integers(0, 200))
+
+    met = apart = again = 0
+    for _ in range(3000):
+        a, b = some(), some()
+        if rng.random() < 0.5:   # two parts of one packed buffer, often
+            b = (b[0], a[1], b[2])
+        va, vb = (base.as_strided(*x) for x in (a, b))
+        ea, eb = (cell.as_strided(*x).flatten().tolist() for x in (a, b))
+        want = bool(set(ea) & set(eb))
+        assert operands.meet(operands.runs(va), operands.runs(vb)) == want, (a, b)
+        assert operands.repeats(operands.runs(va)) == (len(set(ea)) < len(ea)), a
+        xa, xb = operands.box(va), operands.box(vb)
+        assert not (want and operands.boxes_apart(xa, xb)), (a, b)
+        assert not (xa[4] and len(set(ea)) < len(ea)), a
+        if a[0] == b[0]:
+            assert operands.same_rows(va, vb) == (ea == eb), (a, b)
+        met, apart, again = met + want, apart + (not want), again + (len(set(ea)) < len(ea))
+    assert min(met, apart, again) > 300
+    # q | k | v rows, a buffer of heads, one of pairs of heads: no run is looked at by itself
+    rows = base[:6 * 5 * 8].view(6, 5, 8)
+    heads = base[:6 * 5 * 8].view(5, 6, 8).transpose(0, 1)
+    for x in (rows, heads):
+        for p, q in ((x[:, :3], x[:, 3:4]), (x[:, 4:], x[:, 0:4]), (x[:, 0::2], x[:, 1::2]),
+                     (x[:2], x[2:]), (x[..., :4], x[..., 4:])):
+            a, b = operands.runs(p), operands.runs(q)
+            assert operands._surely_apart(a[1], a[2], b[1], b[2], b[0] - a[0])
+    for x in (rows, heads):
+        assert operands.boxes_apart(operands.box(x[:, :3]), operands.box(x[:, 3:4]))
+    square = base[:4 * 4 * 8].view(4, 4, 8)
+    assert not operands.same_rows(square, square.transpose(0, 1))
+
+
+def test_rotary_outputs_over_inputs():
+    """On their own inputs, or apart from both and from one another; a buffer's elements once."""
+    rot = rotary.Rotary(8, device="cpu")
+    buf = torch.zeros(9, 6 * 8)
+    part = lambda t0, t1, h0, h1: buf.view(9, 6, 8)[t0:t1, h0:h1]  # noqa: E731
+    q, k = part(0, 4, 0, 2), part(0, 4, 2, 4)
+    new = torch.zeros(4, 2, 8)
+    hm = torch.zeros(2, 4, 8).transpose(0, 1)
+    for out in ((q, k), (new, k), (q, new), (new, hm), (hm, new), (new, new.clone()),
+                (part(4, 8, 0, 2), k), (part(0, 4, 4, 6), k), (q, part(5, 9, 2, 4))):
+        rot._outputs(q, k, *out)
+    rot._outputs(q, None, q, None)
+    rot._outputs(q[:1], None, buf[:1, :16].view(1, 2, 8), None)   # (one token: its stride is none)
+    slide = lambda t, d: t.as_strided(t.shape, t.stride(), t.storage_offset() + d)  # noqa: E731
+    for out, match in (((part(1, 5, 0, 2), k), "overlaps q"), ((k, q), "overlaps"),
+                       ((slide(q, 1), new), "overlaps"), ((slide(q, 8), new), "overlaps"),
+                       ((new, part(3, 7, 0, 2)), "overlaps q"), ((part(0, 4, 2, 4), new), "overlaps k"),
+                       ((new, new), "overlaps"), ((q[:, :1].expand(4, 2, 8), new), "repeat"), ((new, slide(new, 0)), "overlaps"),
+                       ((buf.view(-1)[:64].view(4, 2, 8), new), "overlaps q"),
+                       ((torch.zeros(64).as_strided((4, 2, 8), (1, 8, 1)), k), "repeat"),
+                       ((torch.zeros(64).as_strided((4, 2, 8), (16, 4, 1)), k), "repeat")):
+        with pytest.raises(ValueError, match=match):
+            rot._outputs(q, k, *out)
+    square = torch.zeros(4, 4, 8)
+    with pytest.raises(ValueError, match="overlaps q"):
+        rot._outputs(square, None, square.transpose(0, 1), None)
+    with pytest.raises(ValueError, match="overlaps"):
+        rot._outputs(q, q, q, q)   # one buffer twice: it would be turned twice
+
+
 def test_sizes_past_32_bit_counts_are_refused():
     """Not cut to their low 32 bits (2^32 + 4 rows are not four), nor run with counts that a grid's
     step would overflow."""

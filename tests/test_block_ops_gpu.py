@@ -324,6 +324,32 @@ def test_rotary_far_positions_and_layouts():
             bad()
 
 
+def test_rotary_refuses_outputs_across_its_inputs():
+    """Outputs over other rows than their own input's; in place and beside, as usual buffers lie."""
+    from gsq_rco_mlx_b200.common.rotary import Rotary
+    r, T = Rotary(64, 1e6), 6
+    p = torch.arange(T, device="cuda") + 9
+    buf = rnd((T + 2, 8 * 64), 3, torch.bfloat16)
+    part = lambda b, t, h, n: b.view(T + 2, 8, 64)[t:t + T, h:h + n]  # noqa: E731
+    q, k = part(buf, 0, 0, 2), part(buf, 0, 2, 2)
+    want = r(q, k, p)
+    keep = buf.clone()
+    for f in (r, r.vjp):
+        for out in ((k, q), (part(buf, 1, 0, 2), want[1]), (want[0], part(buf, 0, 1, 2)),
+                    (want[0], want[0]), (q, part(buf, 0, 1, 2))):
+            with pytest.raises(ValueError, match="overlaps"):
+                f(q, k, p, out=out)
+    assert torch.equal(buf, keep)
+    for h, g in ((0, 2), (4, 6), (4, 2)):   # in place, behind them in the same rows, one of both
+        b = buf.clone()
+        qb, kb = part(b, 0, 0, 2), part(b, 0, 2, 2)
+        out = part(b, 0, h, 2), part(b, 0, g, 2)
+        r(qb, kb, p, out=out)
+        assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+    heads = buf[:, :2 * 64].reshape(T + 2, 2, 64).transpose(0, 1).contiguous().transpose(0, 1)[:T]
+    assert torch.equal(r(heads, None, p, out=(heads, None))[0], want[0])
+
+
 def test_rotary_values_that_are_not_finite():
     """NaN and infinity stay inside their pair."""
     from gsq_rco_mlx_b200.common.rotary import Rotary
