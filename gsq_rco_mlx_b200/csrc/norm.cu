@@ -662,8 +662,11 @@ template <typename T, bool VEC, bool WARP, int Q, int W, int THREADS>
 static int bwd_launch(const Bwd& p, const Plan& pl, cudaStream_t st) {
   auto kern = p.w_post && p.w_pre && p.in[3] ? bwd_kernel<T, VEC, WARP, Q, W, THREADS, true>
                                              : bwd_kernel<T, VEC, WARP, Q, W, THREADS, false>;
-  if (pl.smem > 48 * 1024 &&
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pl.smem) !=
+  // The limit is the function's, for all host threads: one value for every call (bwd_plan gives no
+  // team more), so that none lowers it between another's setting and launch.
+  if (pl.smem > kSmemTeam) return GSQ_ENOTSUP;
+  if (W != W_MEM &&
+      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemTeam) !=
           cudaSuccess)
     return GSQ_ECUDA;
   kern<<<pl.blocks, pl.threads, pl.smem, st>>>(p);

@@ -644,6 +644,54 @@ def test_captured_graphs_streams_and_overlapping_calls():
     _err_ok()
 
 
+def test_norm_gradients_from_two_host_threads(monkeypatch):
+    """Two widths of one kernel that need different amounts of shared memory (82 and 131 KB), called
+    by two threads at once: the limit that one sets must not fall below what the other launches.
+    The threads repeat the entry point's calls alone, so that they meet in it often."""
+    import threading
+    from gsq_rco_mlx_b200 import _lib
+    from gsq_rco_mlx_b200.common.norm import residual_norm, residual_norm_vjp
+    jobs, seen, status = [], [], [[], []]
+    real = _lib.call
+
+    def call(name, *args):
+        seen.append((name, args))
+        real(name, *args)
+
+    for H in (2560, 4096):
+        v = _norm_inputs(8, H, "bf16", True, True, 0, H)
+        st = residual_norm(v["h"], v["y"], v["w_post"], v["w_pre"])[2]
+        side = torch.cuda.Stream()
+        with monkeypatch.context() as m, torch.cuda.stream(side):
+            side.wait_stream(torch.cuda.default_stream())
+            m.setattr(_lib, "call", call)
+            got = residual_norm_vjp(v["h"], v["y"], v["w_post"], v["w_pre"], st, v["dh"], v["dx"])
+        torch.cuda.synchronize()
+        name, args = seen.pop()
+        assert name == "gsq_residual_norm_bwd"
+        ws = torch.empty(args[-3], device="cuda", dtype=torch.uint8)
+        args = args[:-4] + (ws.data_ptr(),) + args[-3:]
+        jobs.append((args, got, {n: t.clone() for n, t in got.items() if t is not None},
+                     (v, st, ws, side)))
+    fn = _lib.lib().gsq_residual_norm_bwd
+    start = threading.Barrier(len(jobs))
+
+    def work(i):
+        start.wait(30)
+        status[i] = [n for n in (fn(*jobs[i][0]) for _ in range(20000)) if n]
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(jobs))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert status == [[], []]
+    for _, got, want, _ in jobs:
+        assert all(torch.equal(got[n], want[n]) for n in want)
+    _err_ok()
+
+
 def test_residual_norm_refuses_outputs_across_its_inputs():
     from gsq_rco_mlx_b200.common.norm import residual_norm
     buf = rnd((9, 64), 5, torch.bfloat16)
