@@ -84,6 +84,7 @@ SIGNATURES = {
     "gsq_fp8_dequant": [_vp, _i64, _vp, _i64, _i32, _i32, _vp, _i32, _i64, _vp],
     "gsq_fp8_gemm": [_i32, _i32, _i32, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i32, _i64, _i64,
                      _vp, _i32, _i64, _i32, _vp, _vp],
+    "gsq_fp8_gemm_tile": [_i32, _i32, _i32, _i32, _i32, _i32, _vp, _vp],
     "gsq_fp8_linear": [_vp, _i32, _i32, _i32, _i64, _vp, _i64, _vp, _i64, _i32, _vp, _i32, _i64,
                        _vp, _i64, _vp, _vp],
     "gsq_fp8_linear_vjp": [_vp, _i32, _i32, _i32, _i64, _vp, _i32, _i32, _i64, _vp, _i64, _vp,

@@ -903,6 +903,16 @@ static int launch_cluster(K kern, int blocks, int threads, uint32_t smem, int cl
   return GSQ_OK;
 }
 
+// Whether the wide kernel was compiled to the register count that its split was made for (another
+// count would leave a setmaxnreg waiting, or registers unused): if not, the narrow tiles serve.
+template <bool BROWS>
+static int wide_fits(bool& fits) {
+  cudaFuncAttributes at;
+  if (cudaFuncGetAttributes(&at, gemm_kernel<256, BROWS, true>) != cudaSuccess) return GSQ_ECUDA;
+  fits = at.numRegs == kLaunchRegs;
+  return GSQ_OK;
+}
+
 template <int BN, bool BROWS, bool PAIR>
 static int launch_gemm(GemmArgs& p, const void* b, int64_t ldb, int dtype, bool follows,
                        cudaStream_t st) {
@@ -914,12 +924,6 @@ static int launch_gemm(GemmArgs& p, const void* b, int64_t ldb, int dtype, bool 
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) !=
       cudaSuccess)
     return GSQ_ECUDA;
-  if (BN == 256) {
-    // the register split is only right for the register count it was made for
-    cudaFuncAttributes at;
-    if (cudaFuncGetAttributes(&at, kern) != cudaSuccess) return GSQ_ECUDA;
-    if (at.numRegs != kLaunchRegs) return GSQ_ENOTSUP;
-  }
   constexpr int rows = PAIR ? 2 * kBM : kBM;
   p.mt = (p.M + rows - 1) / rows;
   p.nt = (p.N + BN - 1) / BN;
@@ -1145,6 +1149,31 @@ static int launch_skinny(const GemmArgs& g, const void* x, int64_t ld_x, const v
   return launch_cluster(kern, tiles * s, kSkThreads, smem, s, follows, st, p, dtype);
 }
 
+// A product's tile: rows x columns of the output that one CTA, or a pair of CTAs, works on; for few
+// rows, all of them by 128 columns.
+enum Tile { FEW_16, FEW_32, FEW_64, PAIR_256, PAIR_128, ONE_128 };
+
+static Tile tile_of(int M, int N, bool sb_rows, bool accumulate, int sms, bool wide) {
+  // Few rows: bound by the weight's bytes (16 x 8192 x 8192 with its quantization: 31 us on
+  // 128-row tiles of A, which leave half of the SMs idle, 16.5 us with the weight's rows as the tile
+  // and k shared out over clusters).
+  if (M <= kSkRows && !sb_rows && !accumulate)
+    return M <= 16 ? FEW_16 : M <= 32 ? FEW_32 : FEW_64;
+  // Tile by the time of the rounds that the busiest SM walks: 256 x 256 of a pair, 256 x 128 of a
+  // pair, or 128 x 128 of one SM. A k-block of the narrow tiles takes 0.64 to 0.7 of the wide
+  // one's time (with the quantization, 8191 x 4096 -> 8192: 288, 398 and 400 us, 16384 x 896 ->
+  // 4864: 94, 118 and 117), so they are taken where they need fewer rounds (4864 x 896 x 4094: 76
+  // wide tiles are two rounds of 74 pairs, 133 narrow ones two of 0.64: the whole vjp of 4094 x
+  // 896 -> 4864 takes 132, 96 and 94 us with one tile for both products, 88 with this choice).
+  const auto rounds = [&](int rows, int bn, int per) {
+    return (double)(((int64_t)((M + rows - 1) / rows) * ((N + bn - 1) / bn) * per + sms - 1) / sms);
+  };
+  const double r256 = rounds(256, 256, 2), r128 = 0.64 * rounds(256, 128, 2),
+               r1 = 0.7 * rounds(128, 128, 1);
+  if (wide && r256 <= r128 && r256 <= r1) return PAIR_256;
+  return r128 <= r1 ? PAIR_128 : ONE_128;
+}
+
 template <typename T>
 static int quant_launch(const T* x, int rows, int cols, int64_t ld_x, uint8_t* codes, int64_t ld_c,
                         float* scales, int64_t ld_s, uint8_t* codes_t, int64_t ld_ct,
@@ -1295,33 +1324,38 @@ static int fp8_gemm(int M, int N, int K, const void* a, int64_t lda, const float
   if (p.boxes && !fp8::out_map(&p.o, out, dtype, M, N, ld_out)) return GSQ_ECUDA;
   p.err = err;
   cudaStream_t st = (cudaStream_t)stream;
-  // Few rows: bound by the weight's bytes (16 x 8192 x 8192 with its quantization: 31 us on
-  // 128-row tiles of A, which leave half of the SMs idle, 16.5 us with the weight's rows as the tile
-  // and k shared out over clusters).
-  if (M <= fp8::kSkRows && !sb_rows && !accumulate)
-    return M <= 16   ? fp8::launch_skinny<16>(p, a, lda, b, ldb, dtype, follows, st)
-           : M <= 32 ? fp8::launch_skinny<32>(p, a, lda, b, ldb, dtype, follows, st)
-                     : fp8::launch_skinny<64>(p, a, lda, b, ldb, dtype, follows, st);
-  // Tile by the time of the rounds that the busiest SM walks: 256 x 256 of a pair, 256 x 128 of a
-  // pair, or 128 x 128 of one SM. A k-block of the narrow tiles takes 0.64 to 0.7 of the wide
-  // one's time (with the quantization, 8191 x 4096 -> 8192: 288, 398 and 400 us, 16384 x 896 ->
-  // 4864: 94, 118 and 117), so they are taken where they need fewer rounds (4864 x 896 x 4094: 76
-  // wide tiles are two rounds of 74 pairs, 133 narrow ones two of 0.64: the whole vjp of 4094 x
-  // 896 -> 4864 takes 132, 96 and 94 us with one tile for both products, 88 with this choice).
-  const auto rounds = [&](int rows, int bn, int sms) {
-    return (double)(((int64_t)((M + rows - 1) / rows) * ((N + bn - 1) / bn) * sms + num_sms() - 1) /
-                    num_sms());
-  };
-  const double r256 = rounds(256, 256, 2), r128 = 0.64 * rounds(256, 128, 2),
-               r1 = 0.7 * rounds(128, 128, 1);
-  const int pick = r256 <= r128 && r256 <= r1 ? 0 : (r128 <= r1 ? 1 : 2);
-  if (sb_rows)
-    return pick == 0   ? fp8::launch_gemm<256, true, true>(p, b, ldb, dtype, follows, st)
-           : pick == 1 ? fp8::launch_gemm<128, true, true>(p, b, ldb, dtype, follows, st)
-                       : fp8::launch_gemm<128, true, false>(p, b, ldb, dtype, follows, st);
-  return pick == 0   ? fp8::launch_gemm<256, false, true>(p, b, ldb, dtype, follows, st)
-         : pick == 1 ? fp8::launch_gemm<128, false, true>(p, b, ldb, dtype, follows, st)
+  fp8::Tile t = fp8::tile_of(M, N, sb_rows, accumulate, num_sms(), true);
+  if (t == fp8::PAIR_256) {
+    bool fits;
+    const int r = sb_rows ? fp8::wide_fits<true>(fits) : fp8::wide_fits<false>(fits);
+    if (r != GSQ_OK) return r;
+    if (!fits) t = fp8::tile_of(M, N, sb_rows, accumulate, num_sms(), false);
+  }
+  switch (t) {
+    case fp8::FEW_16: return fp8::launch_skinny<16>(p, a, lda, b, ldb, dtype, follows, st);
+    case fp8::FEW_32: return fp8::launch_skinny<32>(p, a, lda, b, ldb, dtype, follows, st);
+    case fp8::FEW_64: return fp8::launch_skinny<64>(p, a, lda, b, ldb, dtype, follows, st);
+    case fp8::PAIR_256:
+      return sb_rows ? fp8::launch_gemm<256, true, true>(p, b, ldb, dtype, follows, st)
+                     : fp8::launch_gemm<256, false, true>(p, b, ldb, dtype, follows, st);
+    case fp8::PAIR_128:
+      return sb_rows ? fp8::launch_gemm<128, true, true>(p, b, ldb, dtype, follows, st)
+                     : fp8::launch_gemm<128, false, true>(p, b, ldb, dtype, follows, st);
+    default:
+      return sb_rows ? fp8::launch_gemm<128, true, false>(p, b, ldb, dtype, follows, st)
                      : fp8::launch_gemm<128, false, false>(p, b, ldb, dtype, follows, st);
+  }
+}
+
+extern "C" int gsq_fp8_gemm_tile(int M, int N, int sb_rows, int accumulate, int sms, int wide,
+                                 int* rows, int* cols) {
+  if (M <= 0 || N <= 0 || M > kMaxDim || N > kMaxDim || sms <= 0 || !rows || !cols)
+    return GSQ_EINVAL;
+  const fp8::Tile t = fp8::tile_of(M, N, sb_rows, accumulate, sms, wide);
+  *rows = t == fp8::FEW_16 ? 16 : t == fp8::FEW_32 ? 32 : t == fp8::FEW_64 ? 64
+          : t == fp8::ONE_128 ? 128 : 256;
+  *cols = t == fp8::PAIR_256 ? 256 : 128;
+  return GSQ_OK;
 }
 
 extern "C" int gsq_fp8_gemm(int M, int N, int K, const void* a, int64_t lda, const float* sa,

@@ -538,6 +538,13 @@ int gsq_fp8_gemm(int M, int N, int K, const void *a, int64_t lda, const float *s
                  int64_t sb_k, void *out, int dtype, int64_t ld_out, int accumulate, int *err,
                  void *stream);
 
+/* The tile that gsq_fp8_gemm works on for these sizes on a device of `sms` multiprocessors, as rows
+ * x columns of out: 256 x 256 or 256 x 128 (a pair of them shares a tile), 128 x 128, or 16, 32 or
+ * 64 rows x 128 (all of few rows). wide: whether the 256 x 256 kernel may be taken (it was compiled
+ * to the register count that it needs). Host only. */
+int gsq_fp8_gemm_tile(int M, int N, int sb_rows, int accumulate, int sms, int wide, int *rows,
+                      int *cols);
+
 /* y [M][ld_y] = x W^T with x [M][ld_x] quantized in row form on the way and W in weight form.
  * workspace: 16-byte aligned, >= M ceil16(K) + 4 M ceil(K / 128) bytes. */
 int gsq_fp8_linear(const void *x, int dtype, int M, int K, int64_t ld_x, const void *codes,

@@ -392,6 +392,41 @@ def test_fp8_entry_points_refuse_bad_arguments():
               (13, odd), (14, 8 * 216 - 1), (15, None)])
 
 
+def _tile(M, N, rows=0, accumulate=0, wide=1, sms=148):
+    r, c = C.c_int(), C.c_int()
+    assert _lib.load().gsq_fp8_gemm_tile(M, N, rows, accumulate, sms, wide, C.byref(r),
+                                         C.byref(c)) == _lib.GSQ_OK
+    return r.value, c.value
+
+
+def test_fp8_product_tiles():
+    """Few rows by themselves (not where a scale per row of both sides or a sum into the output is
+    asked for), else by the rounds of the busiest multiprocessor; every tile is some size's."""
+    assert [_tile(m, 4096) for m in (1, 16, 17, 32, 33, 64)] == \
+        [(16, 128)] * 2 + [(32, 128)] * 2 + [(64, 128)] * 2
+    assert _tile(64, 4096, rows=1)[0] >= 128 and _tile(64, 4096, accumulate=1)[0] >= 128
+    assert _tile(16384, 4864) == (256, 256) and _tile(4864, 4864, rows=1) == (256, 256)
+    assert _tile(300, 1000) == (256, 128)
+    assert _tile(100, 19000) == (128, 128) and _tile(100, 19000, rows=1) == (128, 128)
+    lib, r, c = _lib.load(), C.c_int(), C.c_int()
+    for bad in ((0, 1, 148), (1, 0, 148), ((1 << 30) + 1, 1, 148), (1, 1, 0)):
+        assert lib.gsq_fp8_gemm_tile(bad[0], bad[1], 0, 0, bad[2], 1, C.byref(r),
+                                     C.byref(c)) == _lib.GSQ_EINVAL
+    assert lib.gsq_fp8_gemm_tile(1, 1, 0, 0, 148, 1, None, C.byref(c)) == _lib.GSQ_EINVAL
+
+
+def test_fp8_product_without_the_wide_kernel():
+    """A build whose wide kernel has another register count than its split needs takes the narrow
+    tiles, and the others stay."""
+    sizes = [(m, n, s) for m in (65, 129, 300, 2047, 8191, 16384, 1 << 20, 1 << 30)
+             for n in (1, 896, 4864, 19000, 1 << 30) for s in (0, 1)]
+    for m, n, s in sizes:
+        usual, narrow = _tile(m, n, s), _tile(m, n, s, wide=0)
+        assert narrow in ((256, 128), (128, 128))
+        assert narrow == usual or usual == (256, 256)
+    assert any(_tile(m, n, s) == (256, 256) for m, n, s in sizes)
+
+
 def test_fp8_vjp_entry_point_refuses_bad_arguments():
     lib = _lib.load()
     need = 8 * 16 + (16 + 200) * 16 + 4 * (8 * 1 + (16 + 200) * 1)
