@@ -146,6 +146,82 @@ def test_fp8_long_and_wide():
     near(f64(dw), rw, _tol_gemm(mw, 130, torch.float32, rw), "dw")
 
 
+def _tile(M, N, rows=0, accumulate=0):
+    import ctypes
+    from gsq_rco_mlx_b200 import _lib
+    r, c = ctypes.c_int(), ctypes.c_int()
+    _lib.check(_lib.load().gsq_fp8_gemm_tile(M, N, rows, accumulate, _lib.num_sms(), 1,
+                                             ctypes.byref(r), ctypes.byref(c)), "tile")
+    return r.value, c.value
+
+
+def _product(a, b):
+    """(a b^T, the sum of the products' magnitudes) of float64 arrays, in 64 bits."""
+    a, b = torch.from_numpy(a).cuda(), torch.from_numpy(b).cuda()
+    return (a @ b.t()).cpu().numpy(), (a.abs() @ b.abs().t()).cpu().numpy()
+
+
+# sizes that the rule gives each tile of 128 rows or more, with more tiles than pairs (or CTAs),
+# ten ragged blocks of 128 along the sum, and a ragged last tile on both sides
+TILES = [(2047, 4864, (256, 256)), (1300, 4000, (256, 128)), (100, 19000, (128, 128))]
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("M,N,tile", TILES)
+def test_fp8_linear_in_every_tile(M, N, tile, dtype):
+    """Each k-block's own scales, the stages' and the scale ring's second turn, outputs of every
+    type on 16 bytes (written in boxes) and off them (value by value)."""
+    from gsq_rco_mlx_b200.common.fp8 import Fp8Linear, quantize_rows
+    K = 1200
+    assert _tile(M, N) == tile and -(-M // tile[0]) * -(-N // tile[1]) > \
+        (148 if tile[0] == 128 else 74)
+    lin = Fp8Linear.from_weight(rnd((N, K), 1, scale=0.05) * torch.exp(rnd((N, K), 8)[:, :1]))
+    x = rnd((M, K), 2, DT[dtype])
+    y, y32, yq = lin(x), lin(x, y_f32=True), lin(quantize_rows(x))
+    buf = torch.full((M, N + 5), 7.0, device="cuda", dtype=DT[dtype])
+    lin(x, out=buf[:, 3:3 + N])
+    _err_ok()
+    assert torch.equal(buf[:, 3:3 + N], y)
+    assert bool((buf[:, :3] == 7).all()) and bool((buf[:, 3 + N:] == 7).all())
+    ref, mag = _product(of.rows_value(*of.quantize_rows(f32(x))),
+                        of.blocks_value(f32(lin.codes), f32(lin.scales)))
+    for got in (y, y32, yq):
+        near(f64(got), ref, _tol_gemm(mag, K, got.dtype, ref))
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("N,K,tile", TILES)
+def test_fp8_weight_gradient_in_every_tile(N, K, tile, dtype):
+    """The same of dW (a scale per row of both sides), written and added to what is there, on 16
+    bytes and off them; and of dx from it."""
+    from gsq_rco_mlx_b200.common.fp8 import Fp8Linear
+    M = 1200
+    assert _tile(N, K, rows=1) == _tile(N, K, rows=1, accumulate=1) == tile
+    lin = Fp8Linear.from_weight(rnd((N, K), 3, scale=0.05), transposed=True)
+    x = rnd((M, K), 4, DT[dtype]) * torch.exp(rnd((M, 1), 6)).to(DT[dtype])
+    dy = rnd((M, N), 5, DT[dtype], 0.01)
+    dx, dw = lin.vjp(x, dy)
+    base = rnd((N, K), 7)
+    acc = base.clone()
+    lin.vjp(x, dy, dw=acc, accumulate=True)
+    buf = torch.full((N, K + 7), 7.0, device="cuda")
+    buf[:, 5:5 + K] = base
+    lin.vjp(x, dy, dw=buf[:, 5:5 + K], accumulate=True)
+    _err_ok()
+    assert torch.equal(buf[:, 5:5 + K], acc)
+    assert bool((buf[:, :5] == 7).all()) and bool((buf[:, 5 + K:] == 7).all())
+    lin.vjp(x, dy, dw=buf[:, 5:5 + K])
+    assert torch.equal(buf[:, 5:5 + K], dw)
+    wv = of.blocks_value(f32(lin.codes), f32(lin.scales))
+    rx, mx = _product(of.rows_value(*of.quantize_rows(f32(dy))), np.ascontiguousarray(wv.T))
+    near(f64(dx), rx, _tol_gemm(mx, N, DT[dtype], rx), "dx")
+    rw, mw = _product(of.rows_value(*of.quantize_rows(np.ascontiguousarray(f32(dy).T))),
+                      of.rows_value(*of.quantize_rows(np.ascontiguousarray(f32(x).T))))
+    near(f64(dw), rw, _tol_gemm(mw, M, torch.float32, rw), "dw")
+    total = rw + f64(base)
+    near(f64(acc), total, _tol_gemm(mw, M, torch.float32, rw) + U * np.abs(total), "dw added")
+
+
 def test_fp8_strides_outputs_and_refusals():
     """Rows of a wider buffer, a transposed input, outputs inside a wider buffer (whose other
     columns stay), no rows at all; and what is refused."""
