@@ -14,6 +14,9 @@ enum DType { BF16 = 0, F16 = 1, F32 = 2 };
 
 inline size_t dtype_size(int dtype) { return dtype == F32 ? 4 : 2; }
 
+// A pointer that lies on `size` bytes, as the kernels' accesses need it (or is missing).
+inline bool lies_on(const void* p, size_t size) { return (uintptr_t)p % size == 0; }
+
 __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }

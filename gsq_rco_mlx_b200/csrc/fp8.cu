@@ -1233,7 +1233,8 @@ inline bool gemm_ok(int M, int N, int K, const void* a, int64_t lda, const float
   return M > 0 && N > 0 && K > 0 && M <= kMaxDim && N <= kMaxDim && K <= kMaxDim &&
          codes_ok(a, lda, K) && codes_ok(b, ldb, K) && sa &&
          ld_sa >= M && sb && sb_n >= 0 && sb_k >= 0 && out && dtype >= 0 && dtype <= 2 &&
-         ld_out >= N && err && (uintptr_t)out % dtype_size(dtype) == 0 &&
+         ld_out >= N && err && lies_on(out, dtype_size(dtype)) && lies_on(sa, 4) &&
+         lies_on(sb, 4) && lies_on(err, 4) &&
          !(accumulate && dtype != F32) && !(sb_rows && sb_k < N);
 }
 
@@ -1257,6 +1258,7 @@ extern "C" int gsq_fp8_quant(const void* x, int dtype, int rows, int cols, int64
     return GSQ_EINVAL;
   if (codes_t && (!fp8::codes_ok(codes_t, ld_codes_t, rows) || !scales_t || ld_scales_t < cols))
     return GSQ_EINVAL;
+  if (!lies_on(scales, 4) || !lies_on(scales_t, 4)) return GSQ_EINVAL;
   if (codes_t && (rows + 127) / 128 > 65535) return GSQ_EINVAL;
   return fp8::quant_any(x, dtype, rows, cols, ld_x, codes, ld_codes, scales, ld_scales, codes_t,
                         ld_codes_t, scales_t, ld_scales_t, false, (cudaStream_t)stream);
@@ -1266,6 +1268,7 @@ extern "C" int gsq_fp8_quant_blocks(const void* w, int dtype, int N, int K, int6
                                     void* codes, int64_t ld_codes, float* scales,
                                     int64_t ld_scales, void* stream) {
   if (!fp8::quant_ok(w, dtype, N, K, ld_w) || !fp8::codes_ok(codes, ld_codes, K) || !scales ||
+      !lies_on(scales, 4) ||
       ld_scales < (K + 127) / 128 || (N + 127) / 128 > 65535)
     return GSQ_EINVAL;
   return fp8::quant_any(w, dtype, N, K, ld_w, codes, ld_codes, scales, ld_scales, nullptr, 0,
@@ -1275,7 +1278,7 @@ extern "C" int gsq_fp8_quant_blocks(const void* w, int dtype, int N, int K, int6
 extern "C" int gsq_fp8_dequant(const void* codes, int64_t ld_codes, const float* scales,
                                int64_t ld_scales, int N, int K, void* out, int dtype,
                                int64_t ld_out, void* stream) {
-  if (!fp8::codes_ok(codes, ld_codes, K) || !scales || N <= 0 || K <= 0 ||
+  if (!fp8::codes_ok(codes, ld_codes, K) || !scales || !lies_on(scales, 4) || N <= 0 || K <= 0 ||
       N > kMaxDim || K > kMaxDim ||
       ld_scales < (K + 127) / 128 || !out || dtype < 0 || dtype > 2 || ld_out < K ||
       (uintptr_t)out % dtype_size(dtype))

@@ -708,6 +708,9 @@ extern "C" int gsq_residual_norm(const void* h, int64_t ld_h, const void* y, int
   if (T <= 0 || T > kMaxDim || H <= 0 || dtype < 0 || dtype > 2 || !stats) return GSQ_EINVAL;
   const size_t es = dtype_size(dtype);
   if (!norm::row_ok(h, ld_h, H, es) || !norm::row_ok(y, ld_y, H, es)) return GSQ_EINVAL;
+  if (!lies_on(w_post, es) || !lies_on(w_pre, es) || !lies_on(gate, es) || !lies_on(stats, 4) ||
+      !lies_on(scales, 4))
+    return GSQ_EINVAL;
   if (gate && (gate_rows <= 0 || T % gate_rows)) return GSQ_EINVAL;
   if (h_out && !norm::row_ok(h_out, ld_ho, H, es)) return GSQ_EINVAL;
   if (w_pre ? (!x && !codes) || (x && codes) : x || codes) return GSQ_EINVAL;
@@ -758,6 +761,9 @@ extern "C" int gsq_residual_norm_bwd(const void* h, int64_t ld_h, const void* y,
   const size_t es = dtype_size(dtype);
   if (!norm::row_ok(h, ld_h, H, es) || !norm::row_ok(y, ld_y, H, es) ||
       !norm::row_ok(dh, ld_dh, H, es) || !norm::row_ok(dy, ld_dy, H, es))
+    return GSQ_EINVAL;
+  if (!lies_on(w_post, es) || !lies_on(w_pre, es) || !lies_on(gate, es) || !lies_on(stats, 4) ||
+      !lies_on(dw_post, 4) || !lies_on(dw_pre, 4) || !lies_on(dgate, 4) || !lies_on(err, 4))
     return GSQ_EINVAL;
   if ((gate && (gate_rows <= 0 || T % gate_rows || !dgate)) || (!gate && dgate)) return GSQ_EINVAL;
   if ((dh2 && !norm::row_ok(dh2, ld_dh2, H, es)) || (w_post && !dw_post) || (w_pre && !dw_pre) ||

@@ -437,6 +437,34 @@ def test_fp8_vjp_entry_point_refuses_bad_arguments():
               (16, 199), (18, None), (18, C.c_void_p(4100)), (19, need - 1), (20, None)])
 
 
+def test_entry_points_refuse_pointers_off_their_type():
+    """Scales, statistics, parameters and gradients that do not lie on their own size would be a
+    misaligned access of the kernels."""
+    lib, odd, two = _lib.load(), C.c_void_p(4097), C.c_void_p(4098)
+    _refused(lib.gsq_fp8_quant, [P, 0, 5, 200, 200, P, 208, P, 5, P, 16, P, 200, None],
+             [(7, two), (11, two)])
+    _refused(lib.gsq_fp8_quant_blocks, [P, 0, 5, 200, 200, P, 208, P, 2, None], [(7, two)])
+    _refused(lib.gsq_fp8_dequant, [P, 208, P, 2, 5, 200, P, 0, 200, None], [(2, two)])
+    _refused(lib.gsq_fp8_gemm, [8, 16, 200, P, 208, P, 8, P, 208, P, 0, 2, 1, P, 0, 16, 0, P, None],
+             [(5, two), (9, two), (17, two)])
+    _refused(lib.gsq_fp8_linear, [P, 0, 8, 200, 200, P, 208, P, 2, 16, P, 0, 16, P, 8 * 216, P, None],
+             [(7, two), (15, two)])
+    need = 8 * 16 + (16 + 200) * 16 + 4 * (8 * 1 + (16 + 200) * 1)
+    _refused(lib.gsq_fp8_linear_vjp,
+             [P, 0, 8, 200, 200, P, 0, 16, 16, P, 16, P, 2, P, 200, P, 200, 0, P, need, P, None],
+             [(11, two), (15, two), (20, two)])
+    _refused(lib.gsq_residual_norm,
+             [P, 64, P, 64, P, P, P, 2, 4, 64, 0, 1.0, 1e-6, 0.0, P, 64, P, 64, None, 0, None, 0, P,
+              None], [(4, odd), (5, odd), (6, odd), (22, two)])
+    _refused(lib.gsq_residual_norm,
+             [P, 64, P, 64, P, P, P, 2, 4, 64, 2, 1.0, 1e-6, 0.0, P, 64, None, 0, P, 64, P, 4, P,
+              None], [(4, two), (5, two), (6, two), (20, two)])
+    _refused(lib.gsq_residual_norm_bwd,
+             [P, 64, P, 64, P, P, P, 2, P, P, 64, P, 64, 4, 64, 0, 1.0, 0.0, P, 64, P, 64, P, P, P,
+              P, 1 << 40, P, None],
+             [(4, odd), (5, odd), (6, odd), (8, two), (22, two), (23, two), (24, two), (27, two)])
+
+
 def test_rope_entry_point_refuses_bad_arguments():
     lib = _lib.load()
     ok = [P, 128, 64, 2, P, 128, 64, 1, 4, 64, 32, 0, 0, P, 0, P, 1.0, 0, P, 128, 64, P, 64, 64, None]
