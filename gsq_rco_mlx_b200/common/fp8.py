@@ -18,7 +18,8 @@ from __future__ import annotations
 import torch
 
 from .. import _lib
-from .operands import DTYPES, MAX_DIM, error_word, matrix, on_device, output, same_device, stream_of
+from .operands import DTYPES, MAX_DIM, apart, error_word, matrix, on_device, output, \
+    same_device, stream_of
 
 BLOCK = 128
 E4M3 = torch.float8_e4m3fn
@@ -169,7 +170,8 @@ class Fp8Linear:
 
     def __call__(self, x, out=None, y_f32=False):
         """y = x W^T [M, N] in x's type (or float32): x [M, K] (bf16, float16 or float32),
-        quantized per row and 128 columns on the way; or x an Fp8Tensor (y in bf16)."""
+        quantized per row and 128 columns on the way (out may lie over it); or x an Fp8Tensor (y in
+        bf16, an out over it is refused)."""
         dev = on_device(self.codes, "the weight")
         if isinstance(x, Fp8Tensor):
             M = x.shape[0]
@@ -178,6 +180,9 @@ class Fp8Linear:
             same_device(x.codes, "x", dev)
             y, ld = output(out, M, self.N, torch.float32 if y_f32 else torch.bfloat16,
                            self.codes, "out")
+            if out is not None:
+                apart(out, "out", x.codes, "the codes of x")
+                apart(out, "out", x.scales.t(), "the scales of x")
             if M:
                 _lib.call("gsq_fp8_gemm", M, self.N, self.K, x.codes.data_ptr(), x.codes.stride(0),
                           x.scales.data_ptr(), x.scales.stride(1) if x.scales.shape[1] > 1 else M,
@@ -204,7 +209,8 @@ class Fp8Linear:
         """Vector-Jacobian product at x [M, K] for the cotangent dy [M, N]: (dx, dw).
         dx = dy W [M, K] in x's type, dy quantized per row and 128 columns, W the weight's own
         codes. dw = dy^T x float32 [N, K] (added to dw when accumulate), both quantized per
-        column and 128 rows; rounding counts as the identity (straight through)."""
+        column and 128 rows; rounding counts as the identity (straight through). dx and dw may lie
+        over x and dy, but not over one another."""
         dev = on_device(self.codes, "the weight")
         x, ld_x = matrix(x, "x", cols=self.K)
         M, N, K = x.shape[0], self.N, self.K
@@ -213,8 +219,11 @@ class Fp8Linear:
         same_device(dy, "dy", dev)
         if accumulate and dw is None:
             raise ValueError("accumulate needs dw")
+        both = dx is not None and dw is not None
         dx, ld_dx = output(dx, M, K, x.dtype, x, "dx")
         dw, ld_dw = output(dw, N, K, torch.float32, x, "dw")
+        if both:
+            apart(dx, "dx", dw, "dw")
         if not M:
             if not accumulate:
                 dw.zero_()

@@ -18,7 +18,7 @@ import torch
 
 from .. import _lib
 from .fp8 import Fp8Tensor, pad16
-from .operands import DTYPES, error_word, matrix, on_device, output, row_by_row, \
+from .operands import DTYPES, apart, error_word, matrix, on_device, output, row_by_row, \
     same_device, stream_of
 
 MAX_WIDTH = 32768
@@ -67,7 +67,7 @@ def residual_norm(h, y, w_post=None, w_pre=None, gate=None, scale=1.0, eps=1e-6,
     (i + 1) T / rows). x is None without w_pre; with fp8 an Fp8Tensor (x in e4m3 with a scale per
     row and 128 columns: what Fp8Linear takes). stats float32 [2, T]: the reciprocal root mean
     squares of y and h' (1 where there is no norm), for residual_norm_vjp. out: where h' goes (h
-    itself for a residual stream updated in place; no other overlap with h or y)."""
+    itself for a residual stream updated in place; no other overlap with h, y or the parameters)."""
     dev, h, ld_h, y, ld_y, w_post, w_pre, gate, rows = _inputs(h, y, w_post, w_pre, gate)
     if fp8 and w_pre is None:
         raise ValueError("fp8 needs w_pre (x is what is quantized)")
@@ -77,6 +77,9 @@ def residual_norm(h, y, w_post=None, w_pre=None, gate=None, scale=1.0, eps=1e-6,
     if out is not None:
         row_by_row(out, ld_h2, h, ld_h, "out", "h")
         row_by_row(out, ld_h2, y, ld_y, "out", "y")
+        for w, name in ((w_post, "w_post"), (w_pre, "w_pre"), (gate, "gate")):
+            if w is not None:
+                apart(out, "out", w, name)
     stats = h.new_empty((2, T), dtype=torch.float32)
     x, xp, codes, scales, ld_c = None, None, None, None, 0
     if fp8:

@@ -183,6 +183,16 @@ def meet(a, b):
     return bool(np.any(A[np.minimum(i, len(A) - 1)][i < len(A)] < B[i < len(A)] + wb))
 
 
+def apart(a, what, b, name):
+    """Refuses a that has a byte in common with b (rows whose elements are contiguous)."""
+    d, n = b.data_ptr() - a.data_ptr(), a.element_size()
+    if a.is_contiguous() and d >= a.numel() * n or b.is_contiguous() and \
+            -d >= b.numel() * b.element_size() or not a.numel() or not b.numel():
+        return
+    if meet(runs(a), runs(b)):
+        raise ValueError(f"{what} overlaps {name}")
+
+
 def repeats(a):
     """Whether runs lie over one another (True also where it is not settled, as in meet)."""
     _, dims, width = a

@@ -302,6 +302,33 @@ def test_runs_that_meet():
     assert not operands.same_rows(square, square.transpose(0, 1))
 
 
+def test_outputs_over_other_tensors():
+    """apart against the elements themselves, between types of different size."""
+    from gsq_rco_mlx_b200.common.operands import apart
+    rng = np.random.default_rng(8)
+    buf = torch.zeros(512, dtype=torch.uint8)
+    byte, seen = torch.arange(512), [0, 0]
+
+    def some(dtype, n):
+        r, c = (int(rng.integers(1, 5)) for _ in range(2))
+        ld, at = int(rng.integers(c, 12)), int(rng.integers(0, 20))
+        if rng.random() < 0.4:
+            ld = c
+        t = buf.view(dtype).as_strided((r, c), (ld, 1), at)
+        return t, {int(v) for v in byte.as_strided((r, c, n), (ld * n, n, 1), at * n).flatten()}
+
+    for _ in range(3000):
+        (a, ea), (b, eb) = some(torch.float32, 4), some(torch.bfloat16, 2)
+        seen[bool(ea & eb)] += 1
+        if ea & eb:
+            with pytest.raises(ValueError, match="a overlaps b"):
+                apart(a, "a", b, "b")
+        else:
+            apart(a, "a", b, "b")
+    assert min(seen) > 300
+    apart(buf.view(torch.float32)[:0], "a", buf, "b")
+
+
 def test_rotary_outputs_over_inputs():
     """On their own inputs, or apart from both and from one another; a buffer's elements once."""
     rot = rotary.Rotary(8, device="cpu")

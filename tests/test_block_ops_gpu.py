@@ -786,6 +786,50 @@ def test_residual_norm_refuses_outputs_across_its_inputs():
                        residual_norm(h, buf[:8, 24:48])[0])
 
 
+def test_outputs_over_operands_that_are_still_read():
+    """The 8-bit product into its own codes or scales, both gradients in one place, h' over the
+    norm's parameters: refused, with nothing written. Into the dense rows that were quantized
+    before: the values of a fresh output."""
+    from gsq_rco_mlx_b200.common.fp8 import Fp8Linear, quantize_rows
+    from gsq_rco_mlx_b200.common.norm import residual_norm
+    n = 256
+    lin = Fp8Linear.from_weight(rnd((n, n), 1), transposed=True)
+    x, dy = rnd((n, n), 2), rnd((n, n), 3)
+    q = quantize_rows(x)
+    room = q.codes.view(torch.bfloat16)   # [n, n / 2] over the codes
+    small = Fp8Linear.from_weight(rnd((n // 2, n), 4))
+    keep = q.codes.view(torch.uint8).clone(), q.scales.clone()
+    with pytest.raises(ValueError, match="codes of x"):
+        small(q, out=room)
+    with pytest.raises(ValueError, match="scales of x"):   # (2 blocks of n scales: n rows of two)
+        Fp8Linear.from_weight(rnd((2, n), 5))(q, out=q.scales.t().view(n, 2), y_f32=True)
+    g = torch.zeros(2 * n, n, device="cuda")
+    for a, b in ((g[:n], g[:n]), (g[:n], g[n - 1:2 * n - 1])):
+        with pytest.raises(ValueError, match="dx overlaps dw"):
+            lin.vjp(x, dy, dx=a, dw=b)
+    assert not bool(g.any())
+    want = lin.vjp(x, dy)
+    got = lin.vjp(x, dy, dx=g[:n], dw=g[n:])
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    y = lin(x)
+    over = x.clone()
+    assert torch.equal(lin(over, out=over), y)
+    over = x.clone()
+    got = lin.vjp(over, dy, dx=over)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    buf = rnd((9, 64), 6)
+    h, z = rnd((8, 64), 7), rnd((8, 64), 8)
+    before = buf.clone()
+    for kw in ({"w_post": buf[3]}, {"w_pre": buf[0]}, {"gate": buf[4:6]}):
+        with pytest.raises(ValueError, match="out overlaps " + next(iter(kw))):
+            residual_norm(h, z, out=buf[:8], **kw)
+        residual_norm(h, z, out=buf.clone()[:8], **kw)
+    assert torch.equal(buf, before)
+    assert torch.equal(q.codes.view(torch.uint8), keep[0]) and torch.equal(q.scales, keep[1])
+    residual_norm(h, z, w_post=buf[8], out=buf[:8])
+    _err_ok()
+
+
 def test_transposed_codes_are_there_for_every_stream():
     """A weight's first vjp behind other work of its stream, the second at once on another one; and
     a capture that would have to make the codes is refused, with eager calls as right after it."""
