@@ -305,6 +305,28 @@ def test_fp8_not_finite_and_extreme_values(M):
     near(got[fits], ref[fits], _tol_gemm(mag, K, torch.float32, ref)[fits])
 
 
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("M", [5, 200])
+def test_fp8_gradients_of_values_that_are_not_finite(M, dtype):
+    """A row of dy with NaN or infinity reaches its row of dx and its column's row of dW; one of x
+    a column of dW. A block's values are NaN with it, so a token's whole block of 128 is."""
+    from gsq_rco_mlx_b200.common.fp8 import Fp8Linear
+    K, N = 300, 140
+    lin = Fp8Linear.from_weight(rnd((N, K), 9, scale=0.05), transposed=True)
+    x, dy = rnd((M, K), 4, DT[dtype]), rnd((M, N), 5, DT[dtype], 0.01)
+    x[2, 290], dy[1, 7], dy[M - 1, 139] = float("inf"), float("nan"), float("-inf")
+    dx, dw = lin.vjp(x, dy)
+    _err_ok()
+    nan_x, nan_w = np.zeros((M, K), bool), np.zeros((N, K), bool)
+    nan_x[[1, M - 1]], nan_w[[7, 139]], nan_w[:, 290] = True, True, True
+    assert np.array_equal(np.isnan(f64(dx)), nan_x) and np.array_equal(np.isnan(f64(dw)), nan_w)
+    clean_x, clean_dy = x.clone(), dy.clone()
+    clean_x[2, 290], clean_dy[1, 7], clean_dy[M - 1, 139] = 0, 0, 0
+    rx, mx, rw, mw = of.vjp(f32(clean_x), f32(clean_dy), f32(lin.codes), f32(lin.scales))
+    near(f64(dx)[~nan_x], rx[~nan_x], _tol_gemm(mx, N, DT[dtype], rx)[~nan_x], "dx")
+    near(f64(dw)[~nan_w], rw[~nan_w], _tol_gemm(mw, M, torch.float32, rw)[~nan_w], "dw")
+
+
 # ------------------------------------------------------------------------------------- rotary ---
 SCALINGS = [None, {"type": "linear", "factor": 4.0}, {"type": "ntk", "factor": 8.0},
             {"type": "yarn", "factor": 8.0, "original": 4096},
@@ -606,6 +628,57 @@ def test_residual_norm_rows_strides_and_refusals():
                  lambda: residual_norm_vjp(v["h"], v["y"], v["w_post"], None, st, None, None)):
         with pytest.raises(ValueError):
             call()
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("T,H", [(6, 200), (6, 257), (5, 1000), (4, 1025), (7, 5124), (6, 9001)])
+def test_residual_norm_values_that_are_not_finite(T, H, dtype):
+    """NaN and infinity in h, y and the cotangents, in each kernel's rows: the values of the formula
+    in 64 bits (infinity times a reciprocal root of zero is NaN), also in e4m3, where a block with
+    one NaN is NaN; other rows as without them; the sums over rows NaN where a row is."""
+    from gsq_rco_mlx_b200.common.norm import residual_norm, residual_norm_vjp
+    v = _norm_inputs(T, H, dtype, True, True, 1, seed=40)
+    args = (v["w_post"], v["w_pre"])
+    kw = dict(gate=v["gate"], scale=0.5)
+    clean = residual_norm(v["h"], v["y"], *args, **kw)
+    c8 = residual_norm(v["h"], v["y"], *args, fp8=True, **kw)[1]
+    _, _, st = clean
+    g0 = residual_norm_vjp(v["h"], v["y"], *args, st, v["dh"], v["dx"], **kw)
+    h, y = v["h"].clone(), v["y"].clone()
+    h[0, 3], h[1, H - 1], y[2, 150], y[3, 0] = (float(n) for n in ("nan", "inf", "nan", "-inf"))
+    h2, x, st2 = residual_norm(h, y, *args, **kw)
+    q = residual_norm(h, y, *args, fp8=True, **kw)[1]
+    # rows 0, 2: r1 or h' is NaN, so all of x is; row 1: h' holds one infinity, r2 is 0 and x is 0 but
+    # for inf 0 = NaN; row 3: r1 is 0, the norm of y is 0 but for NaN at its infinity
+    wide = np.ones((T, H), bool)
+    one = np.zeros((T, H), bool)
+    one[0, 3], one[2], one[3, 0] = True, True, True
+    assert np.array_equal(np.isnan(f64(h2)), one)
+    assert np.isinf(f64(h2)[1]).tolist() == [False] * (H - 1) + [True]
+    nan = np.zeros((T, H), bool)
+    nan[[0, 2, 3]], nan[1, H - 1] = True, True
+    assert np.array_equal(np.isnan(f64(x)), nan) and not f64(x)[1, :H - 1].any()
+    blocks = np.zeros((T, H), bool)
+    blocks[[0, 2, 3]], blocks[1, (H - 1) // 128 * 128:] = True, True
+    assert np.array_equal(np.isnan(f64(q.float())), blocks & wide)
+    assert not f64(q.float())[1, :(H - 1) // 128 * 128].any()
+    assert torch.equal(h2[4:], clean[0][4:]) and torch.equal(x[4:], clean[1][4:])
+    assert torch.equal(q.codes[4:].view(torch.uint8), c8.codes[4:].view(torch.uint8))
+    assert torch.equal(q.scales[4:], c8.scales[4:]) and torch.equal(st2[:, 4:], st[:, 4:])
+    # the gradient: one NaN of a cotangent reaches its row, and every sum over rows where it is
+    dh, dx = v["dh"].clone(), v["dx"].clone()
+    dx[0, 5], dh[2, H - 2] = float("nan"), float("inf")
+    g = residual_norm_vjp(v["h"], v["y"], *args, st, dh, dx, **kw)
+    _err_ok()
+    for n in ("dh", "dy"):
+        assert torch.equal(g[n][3:], g0[n][3:]) and torch.equal(g[n][1], g0[n][1]), n
+        assert bool(torch.isnan(g[n][0]).all())
+    assert bool(torch.isinf(g["dh"][2, H - 2])) and bool(torch.isnan(g["dy"][2]).any())
+    keep = torch.ones(H, dtype=torch.bool)
+    keep[5] = False
+    assert bool(torch.isnan(g["dw_pre"][5])) and torch.equal(g["dw_pre"][keep], g0["dw_pre"][keep])
+    for n in ("dw_post", "dgate"):
+        assert bool(torch.isnan(g[n]).all()), n
 
 
 # ------------------------------------------------------------------------------------ together ---
