@@ -211,6 +211,9 @@ class Fp8Linear:
         codes. dw = dy^T x float32 [N, K] (added to dw when accumulate), both quantized per
         column and 128 rows; rounding counts as the identity (straight through). dx and dw may lie
         over x and dy, but not over one another."""
+        if isinstance(x, Fp8Tensor):
+            raise ValueError("x must be dense: dw takes it with other scales (per column and 128 "
+                             "rows) than the rows' codes hold")
         dev = on_device(self.codes, "the weight")
         x, ld_x = matrix(x, "x", cols=self.K)
         M, N, K = x.shape[0], self.N, self.K

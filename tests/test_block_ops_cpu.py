@@ -181,6 +181,14 @@ def test_transposed_codes_are_not_made_during_a_capture(monkeypatch):
     assert lin._t is None
 
 
+def test_quantized_rows_are_no_input_of_the_gradient():
+    """Refused with the reason, not with an error of a missing attribute."""
+    lin = fp8.Fp8Linear.__new__(fp8.Fp8Linear)
+    q = fp8.Fp8Tensor.empty(4, 32, torch.device("cpu"))
+    with pytest.raises(ValueError, match="x must be dense"):
+        lin.vjp(q, torch.zeros(4, 16))
+
+
 def test_the_error_word_is_not_made_during_a_capture(monkeypatch):
     """Nor is one that is there asked for again."""
     from gsq_rco_mlx_b200 import gemm
