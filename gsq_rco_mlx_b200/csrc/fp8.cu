@@ -391,7 +391,9 @@ __device__ __forceinline__ void grid_wait() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
+// (.aligned: the warp's threads arrive together, whatever branches they come from)
 __device__ __forceinline__ void cluster_sync() {
+  __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
                    : "memory");
 }
@@ -816,7 +818,6 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
   if (PAIR) {
     // the second CTA stays until the pair's last commit has arrived here too
     if (rank == 1 && threadIdx.x == 0) tc::mbar_wait(&last, 0, p.err, 9);
-    __syncwarp();
     cluster_sync();   // (the other CTA's MMAs, commits and arrivals are over)
   }
   tc::fence_after_sync();
