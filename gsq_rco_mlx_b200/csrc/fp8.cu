@@ -556,7 +556,8 @@ __device__ __forceinline__ void store_boxes(const GemmArgs& p, uint8_t* stage, i
 
 // Register split of the wide kernel: 12 warps are launched with 168 registers a thread; warps
 // 0-3 give theirs up to 72 and the epilogue's two warpgroups take 216 (128 x 72 + 256 x 216 =
-// 384 x 168), enough for 128 sums and two groups of 32 accumulator columns in flight.
+// 384 x 168): 128 sums and the 64 accumulator columns that are being folded. With a scale per row
+// of both sides the columns' scales come on top, and 112 bytes a thread spill (560 read back).
 constexpr int kLaunchRegs = 168;
 template <int R>
 __device__ __forceinline__ void regs_dec() {
@@ -571,12 +572,13 @@ __device__ __forceinline__ void regs_inc() {
 // issues the MMAs of a k-block into the next accumulator of the ring, warps 4-11 fold it: warp
 // w reads TMEM lanes 32 (w % 4).. (its rows) and half of the columns.
 // BROWS: B has a scale per row and k-block instead of one per 128 x 128.
-// PAIR: two CTAs of a cluster share a tile of 256 rows. Each loads its 128 rows of A and half of
-// B's columns, the first one issues MMAs over both (cta_group::2: each SM multiplies its rows by
-// all columns), and each folds its own rows: half the bytes of B from L2 and in shared memory.
-template <int BN, bool BROWS, bool PAIR>
+// PAIR (256 columns): two CTAs of a cluster share a tile of 256 rows. Each loads its 128 rows of A
+// and half of B's columns, the first one issues MMAs over both (cta_group::2: each SM multiplies its
+// rows by all columns), and each folds its own rows: half the bytes of B from L2 and in shared memory.
+template <int BN, bool BROWS>
 __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant__ GemmArgs p,
                                                            int dtype) {
+  constexpr bool PAIR = BN == 256;
   constexpr int kSlots = kTmemCols / BN;
   constexpr int kBRows = PAIR ? BN / 2 : BN;  // rows of B this CTA loads
   constexpr uint32_t kStage = (kBM + kBRows) * kBlk;
@@ -909,18 +911,19 @@ static int launch_cluster(K kern, int blocks, int threads, uint32_t smem, int cl
 template <bool BROWS>
 static int wide_fits(bool& fits) {
   cudaFuncAttributes at;
-  if (cudaFuncGetAttributes(&at, gemm_kernel<256, BROWS, true>) != cudaSuccess) return GSQ_ECUDA;
+  if (cudaFuncGetAttributes(&at, gemm_kernel<256, BROWS>) != cudaSuccess) return GSQ_ECUDA;
   fits = at.numRegs == kLaunchRegs;
   return GSQ_OK;
 }
 
-template <int BN, bool BROWS, bool PAIR>
+template <int BN, bool BROWS>
 static int launch_gemm(GemmArgs& p, const void* b, int64_t ldb, int dtype, bool follows,
                        cudaStream_t st) {
+  constexpr bool PAIR = BN == 256;
   constexpr int kBRows = PAIR ? BN / 2 : BN;
   constexpr uint32_t kStage = (kBM + kBRows) * kBlk;
   constexpr uint32_t smem = kPipeBytes / kStage * kStage + kStageBytes + 1024;
-  auto kern = gemm_kernel<BN, BROWS, PAIR>;
+  auto kern = gemm_kernel<BN, BROWS>;
   if (!codes_map(&p.b, b, p.N, p.K, ldb, kBRows)) return GSQ_ECUDA;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) !=
       cudaSuccess)
@@ -1152,7 +1155,7 @@ static int launch_skinny(const GemmArgs& g, const void* x, int64_t ld_x, const v
 
 // A product's tile: rows x columns of the output that one CTA, or a pair of CTAs, works on; for few
 // rows, all of them by 128 columns.
-enum Tile { FEW_16, FEW_32, FEW_64, PAIR_256, PAIR_128, ONE_128 };
+enum Tile { FEW_16, FEW_32, FEW_64, PAIR_256, ONE_128 };
 
 static Tile tile_of(int M, int N, bool sb_rows, bool accumulate, int sms, bool wide) {
   // Few rows: bound by the weight's bytes (16 x 8192 x 8192 with its quantization: 31 us on
@@ -1160,19 +1163,19 @@ static Tile tile_of(int M, int N, bool sb_rows, bool accumulate, int sms, bool w
   // and k shared out over clusters).
   if (M <= kSkRows && !sb_rows && !accumulate)
     return M <= 16 ? FEW_16 : M <= 32 ? FEW_32 : FEW_64;
-  // Tile by the time of the rounds that the busiest SM walks: 256 x 256 of a pair, 256 x 128 of a
-  // pair, or 128 x 128 of one SM. A k-block of the narrow tiles takes 0.64 to 0.7 of the wide
-  // one's time (with the quantization, 8191 x 4096 -> 8192: 288, 398 and 400 us, 16384 x 896 ->
-  // 4864: 94, 118 and 117), so they are taken where they need fewer rounds (4864 x 896 x 4094: 76
-  // wide tiles are two rounds of 74 pairs, 133 narrow ones two of 0.64: the whole vjp of 4094 x
-  // 896 -> 4864 takes 132, 96 and 94 us with one tile for both products, 88 with this choice).
+  // Tile by the time of the rounds that the busiest SM walks: 256 x 256 of a pair, or 128 x 128 of
+  // one SM, whose k-block takes 0.66 to 0.7 of the wide one's time (8191 x 4096 -> 8192: 28 rounds
+  // in 348 us for 14 in 253; 16384 x 896 -> 4864: 33 in 114 for 17 in 89; 1024 x 4096 -> 4096: 2 in
+  // 30 for 1 in 22.5), with a scale per row of both sides 0.5 to 0.55 (28 in 454 for 14 in 424; 33
+  // in 156 for 17 in 160; 2 in 37 for 1 in 34). So it is taken where it needs few more rounds (1408
+  // x 2048 -> 3200: 2 in 17.8 for 2 in 22.8; 600 x 4096 -> 9000 with a scale per row: 3 in 54 for 2
+  // in 65, without: 43 for 40). 256 x 128 of a pair was never faster than 128 x 128 (forty
+  // products: equal to 40 % slower) and is not built.
   const auto rounds = [&](int rows, int bn, int per) {
     return (double)(((int64_t)((M + rows - 1) / rows) * ((N + bn - 1) / bn) * per + sms - 1) / sms);
   };
-  const double r256 = rounds(256, 256, 2), r128 = 0.64 * rounds(256, 128, 2),
-               r1 = 0.7 * rounds(128, 128, 1);
-  if (wide && r256 <= r128 && r256 <= r1) return PAIR_256;
-  return r128 <= r1 ? PAIR_128 : ONE_128;
+  return wide && rounds(256, 256, 2) <= (sb_rows ? 0.55 : 0.7) * rounds(128, 128, 1) ? PAIR_256
+                                                                                     : ONE_128;
 }
 
 template <typename T>
@@ -1340,14 +1343,11 @@ static int fp8_gemm(int M, int N, int K, const void* a, int64_t lda, const float
     case fp8::FEW_32: return fp8::launch_skinny<32>(p, a, lda, b, ldb, dtype, follows, st);
     case fp8::FEW_64: return fp8::launch_skinny<64>(p, a, lda, b, ldb, dtype, follows, st);
     case fp8::PAIR_256:
-      return sb_rows ? fp8::launch_gemm<256, true, true>(p, b, ldb, dtype, follows, st)
-                     : fp8::launch_gemm<256, false, true>(p, b, ldb, dtype, follows, st);
-    case fp8::PAIR_128:
-      return sb_rows ? fp8::launch_gemm<128, true, true>(p, b, ldb, dtype, follows, st)
-                     : fp8::launch_gemm<128, false, true>(p, b, ldb, dtype, follows, st);
+      return sb_rows ? fp8::launch_gemm<256, true>(p, b, ldb, dtype, follows, st)
+                     : fp8::launch_gemm<256, false>(p, b, ldb, dtype, follows, st);
     default:
-      return sb_rows ? fp8::launch_gemm<128, true, false>(p, b, ldb, dtype, follows, st)
-                     : fp8::launch_gemm<128, false, false>(p, b, ldb, dtype, follows, st);
+      return sb_rows ? fp8::launch_gemm<128, true>(p, b, ldb, dtype, follows, st)
+                     : fp8::launch_gemm<128, false>(p, b, ldb, dtype, follows, st);
   }
 }
 
@@ -1357,7 +1357,7 @@ extern "C" int gsq_fp8_gemm_tile(int M, int N, int sb_rows, int accumulate, int 
     return GSQ_EINVAL;
   const fp8::Tile t = fp8::tile_of(M, N, sb_rows, accumulate, sms, wide);
   *rows = t == fp8::FEW_16 ? 16 : t == fp8::FEW_32 ? 32 : t == fp8::FEW_64 ? 64
-          : t == fp8::ONE_128 ? 128 : 256;
+          : t == fp8::PAIR_256 ? 256 : 128;
   *cols = t == fp8::PAIR_256 ? 256 : 128;
   return GSQ_OK;
 }

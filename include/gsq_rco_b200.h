@@ -539,8 +539,8 @@ int gsq_fp8_gemm(int M, int N, int K, const void *a, int64_t lda, const float *s
                  void *stream);
 
 /* The tile that gsq_fp8_gemm works on for these sizes on a device of `sms` multiprocessors, as rows
- * x columns of out: 256 x 256 or 256 x 128 (a pair of them shares a tile), 128 x 128, or 16, 32 or
- * 64 rows x 128 (all of few rows). wide: whether the 256 x 256 kernel may be taken (it was compiled
+ * x columns of out: 256 x 256 (a pair of them shares a tile), 128 x 128, or 16, 32 or 64 rows x 128
+ * (all of few rows). wide: whether the 256 x 256 kernel may be taken (it was compiled
  * to the register count that it needs). Host only. */
 int gsq_fp8_gemm_tile(int M, int N, int sb_rows, int accumulate, int sms, int wide, int *rows,
                       int *cols);

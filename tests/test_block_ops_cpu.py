@@ -441,7 +441,7 @@ def test_fp8_product_tiles():
         [(16, 128)] * 2 + [(32, 128)] * 2 + [(64, 128)] * 2
     assert _tile(64, 4096, rows=1)[0] >= 128 and _tile(64, 4096, accumulate=1)[0] >= 128
     assert _tile(16384, 4864) == (256, 256) and _tile(4864, 4864, rows=1) == (256, 256)
-    assert _tile(300, 1000) == (256, 128)
+    assert _tile(600, 9000) == (256, 256) and _tile(600, 9000, rows=1) == (128, 128)
     assert _tile(100, 19000) == (128, 128) and _tile(100, 19000, rows=1) == (128, 128)
     lib, r, c = _lib.load(), C.c_int(), C.c_int()
     for bad in ((0, 1, 148), (1, 0, 148), ((1 << 30) + 1, 1, 148), (1, 1, 0)):
@@ -452,12 +452,12 @@ def test_fp8_product_tiles():
 
 def test_fp8_product_without_the_wide_kernel():
     """A build whose wide kernel has another register count than its split needs takes the narrow
-    tiles, and the others stay."""
+    tile, and the others stay."""
     sizes = [(m, n, s) for m in (65, 129, 300, 2047, 8191, 16384, 1 << 20, 1 << 30)
              for n in (1, 896, 4864, 19000, 1 << 30) for s in (0, 1)]
     for m, n, s in sizes:
         usual, narrow = _tile(m, n, s), _tile(m, n, s, wide=0)
-        assert narrow in ((256, 128), (128, 128))
+        assert narrow == (128, 128)
         assert narrow == usual or usual == (256, 256)
     assert any(_tile(m, n, s) == (256, 256) for m, n, s in sizes)
 

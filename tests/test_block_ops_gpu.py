@@ -162,18 +162,20 @@ def _product(a, b):
 
 
 # sizes that the rule gives each tile of 128 rows or more, with more tiles than pairs (or CTAs),
-# ten ragged blocks of 128 along the sum, and a ragged last tile on both sides
-TILES = [(2047, 4864, (256, 256)), (1300, 4000, (256, 128)), (100, 19000, (128, 128))]
+# ten ragged blocks of 128 along the sum, and ragged last tiles
+TILES = [(2047, 4864, 0, (256, 256)), (1300, 4000, 0, (256, 256)), (100, 19000, 0, (128, 128)),
+         (1400, 3200, 0, (128, 128))]
+TILES_ROWS = [(3000, 3000, 1, (256, 256)), (1300, 4000, 1, (128, 128)), (100, 19000, 1, (128, 128))]
 
 
 @pytest.mark.parametrize("dtype", list(DT))
-@pytest.mark.parametrize("M,N,tile", TILES)
-def test_fp8_linear_in_every_tile(M, N, tile, dtype):
+@pytest.mark.parametrize("M,N,rows,tile", TILES)
+def test_fp8_linear_in_every_tile(M, N, rows, tile, dtype):
     """Each k-block's own scales, the stages' and the scale ring's second turn, outputs of every
     type on 16 bytes (written in boxes) and off them (value by value)."""
     from gsq_rco_mlx_b200.common.fp8 import Fp8Linear, quantize_rows
     K = 1200
-    assert _tile(M, N) == tile and -(-M // tile[0]) * -(-N // tile[1]) > \
+    assert _tile(M, N, rows) == tile and -(-M // tile[0]) * -(-N // tile[1]) > \
         (148 if tile[0] == 128 else 74)
     lin = Fp8Linear.from_weight(rnd((N, K), 1, scale=0.05) * torch.exp(rnd((N, K), 8)[:, :1]))
     x = rnd((M, K), 2, DT[dtype])
@@ -190,13 +192,13 @@ def test_fp8_linear_in_every_tile(M, N, tile, dtype):
 
 
 @pytest.mark.parametrize("dtype", list(DT))
-@pytest.mark.parametrize("N,K,tile", TILES)
-def test_fp8_weight_gradient_in_every_tile(N, K, tile, dtype):
+@pytest.mark.parametrize("N,K,rows,tile", TILES_ROWS)
+def test_fp8_weight_gradient_in_every_tile(N, K, rows, tile, dtype):
     """The same of dW (a scale per row of both sides), written and added to what is there, on 16
     bytes and off them; and of dx from it."""
     from gsq_rco_mlx_b200.common.fp8 import Fp8Linear
     M = 1200
-    assert _tile(N, K, rows=1) == _tile(N, K, rows=1, accumulate=1) == tile
+    assert _tile(N, K, rows) == _tile(N, K, rows, accumulate=1) == tile
     lin = Fp8Linear.from_weight(rnd((N, K), 3, scale=0.05), transposed=True)
     x = rnd((M, K), 4, DT[dtype]) * torch.exp(rnd((M, 1), 6)).to(DT[dtype])
     dy = rnd((M, N), 5, DT[dtype], 0.01)
