@@ -224,6 +224,21 @@ def test_fp8_weight_gradient_in_every_tile(N, K, rows, tile, dtype):
     near(f64(acc), total, _tol_gemm(mw, M, torch.float32, rw) + U * np.abs(total), "dw added")
 
 
+@pytest.mark.parametrize("M", [13, 30, 64])
+def test_fp8_few_rows_long_sums(M):
+    """Each few-row kernel with more k-blocks a CTA than it has stages (5), accumulators (4) and
+    scales staged at a time (16): 21, not shared out; and 41 over a cluster."""
+    from gsq_rco_mlx_b200.common.fp8 import Fp8Linear
+    for K, N in ((2600, 19000), (5200, 3000)):
+        assert _tile(M, N) == (16 if M <= 16 else 32 if M <= 32 else 64, 128)
+        lin = Fp8Linear.from_weight(rnd((N, K), 1, torch.bfloat16, 0.05))
+        x = rnd((M, K), 2, torch.bfloat16) * torch.exp(rnd((M, K), 3)[:, :1]).bfloat16()
+        y = lin(x, y_f32=True)
+        _err_ok()
+        ref, mag = of.linear(f32(x), f32(lin.codes), f32(lin.scales))
+        near(f64(y), ref, _tol_gemm(mag, K, torch.float32, ref))
+
+
 def test_fp8_strides_outputs_and_refusals():
     """Rows of a wider buffer, a transposed input, outputs inside a wider buffer (whose other
     columns stay), no rows at all; and what is refused."""
@@ -572,6 +587,35 @@ def test_residual_norm_vjp(T, H, post, pre, gates, dtype):
     _err_ok()
 
 
+# more rows than teams, so that a team's ring of rows turns more than once and its next row is read
+# ahead; more gate rows than teams; each way of holding the weights, on 16 bytes and off them
+MANY = [(20000, 200, 1), (20000, 100, 0), (6000, 128, 6000), (6000, 896, 3000), (6000, 900, 2),
+        (1500, 2048, 1), (1200, 5121, 3), (1500, 6400, 500), (1300, 7001, 0), (700, 9000, 350)]
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("T,H,gates", MANY)
+def test_residual_norm_many_rows_a_team(T, H, gates, dtype):
+    from gsq_rco_mlx_b200.common.norm import residual_norm, residual_norm_vjp
+    v = _norm_inputs(T, H, dtype, True, True, gates, seed=60)
+    args, kw = (v["w_post"], v["w_pre"]), dict(gate=v["gate"], scale=0.7)
+    h2, x, st = residual_norm(v["h"], v["y"], *args, eps=1e-5, **kw)
+    rx, xt = _check_norm(v, h2, x, st, 0.7, 1e-5, 0.0)
+    h3, q, s3 = residual_norm(v["h"], v["y"], *args, eps=1e-5, fp8=True, **kw)
+    assert torch.equal(h3, h2) and torch.equal(s3, st)
+    sc = np.repeat(f64(q.scales), 128, 1)[:, :H]
+    near(f64(q.float()), rx, xt + np.maximum(2.0 ** -4 * (np.abs(rx) + xt), 2.0 ** -10 * sc)
+         * (1 + 2.0 ** -18) + 2.0 ** -22 * np.abs(rx), "e4m3")
+    over = v["h"].clone()   # in place, the next row read ahead
+    assert torch.equal(residual_norm(over, v["y"], *args, eps=1e-5, out=over, **kw)[1], x)
+    assert torch.equal(over, h2)
+    g, again = (residual_norm_vjp(v["h"], v["y"], *args, st, v["dh"], v["dx"], **kw)
+                for _ in range(2))
+    _check_norm_vjp(v, g, v["dh"], 0.7, 1e-5, 0.0)
+    assert all(g[n] is None or torch.equal(g[n], again[n]) for n in g)
+    _err_ok()
+
+
 def test_residual_norm_rows_strides_and_refusals():
     """Rows of wider and odd buffers, h updated in place, rows behind the last left alone, a row of
     zeros, values that are not finite, no rows; and what is refused."""
@@ -681,6 +725,91 @@ def test_residual_norm_values_that_are_not_finite(T, H, dtype):
     assert bool(torch.isnan(g["dw_pre"][5])) and torch.equal(g["dw_pre"][keep], g0["dw_pre"][keep])
     for n in ("dw_post", "dgate"):
         assert bool(torch.isnan(g[n]).all()), n
+
+
+# ---------------------------------------------------------------------------- beyond 32 bits ---
+@pytest.fixture
+def give_back():
+    """The tens of GB that a test took, to the device."""
+    yield
+    torch.cuda.empty_cache()
+
+
+def test_norms_past_32_bit_offsets(give_back):
+    """2.3e9 elements a tensor: the last rows as of a call on them alone (same width, same kernel)."""
+    from gsq_rco_mlx_b200.common.norm import residual_norm, residual_norm_vjp
+    T, H, n = 70000, 32768, 5
+    g = torch.Generator(device="cuda").manual_seed(1)
+    big = lambda: torch.empty(T, H, device="cuda", dtype=torch.bfloat16).normal_(generator=g)  # noqa: E731
+    h, y = big(), big()
+    w = rnd((H,), 3, torch.bfloat16)
+    h2, q, st = residual_norm(h, y, w, w, fp8=True)
+    a = residual_norm(h[-n:], y[-n:], w, w, fp8=True)
+    assert torch.equal(h2[-n:], a[0]) and torch.equal(st[:, -n:], a[2])
+    assert torch.equal(q.codes[-n:].view(torch.uint8), a[1].codes.view(torch.uint8))
+    assert torch.equal(q.scales[-n:], a[1].scales)
+    del h2, q
+    grads = residual_norm_vjp(h, y, w, w, st, y, h)
+    b = residual_norm_vjp(h[-n:], y[-n:], w, w, st[:, -n:], y[-n:], h[-n:])
+    assert all(torch.equal(grads[k][-n:], b[k]) for k in ("dh", "dy"))
+    _err_ok()
+
+
+def test_rotary_past_32_bit_offsets(give_back):
+    from gsq_rco_mlx_b200.common.rotary import Rotary
+    T, n = 140000, 5
+    g = torch.Generator(device="cuda").manual_seed(2)
+    q = torch.empty(T, 128, 128, device="cuda", dtype=torch.bfloat16).normal_(generator=g)
+    r, pos = Rotary(128), torch.arange(T, device="cuda")
+    want = r(q[-n:], None, pos[-n:])[0]
+    heads = q[:T // 2].transpose(0, 1).contiguous().transpose(0, 1)   # head-major: 9e6 a head
+    hw = r(q[T // 2 - n:T // 2], None, pos[T // 2 - n:T // 2])[0]
+    r(heads, None, pos[:T // 2], out=(heads, None))
+    r(q, None, pos, out=(q, None))
+    assert torch.equal(q[-n:], want) and torch.equal(heads[-n:], hw)
+
+
+def test_fp8_past_32_bit_offsets(give_back):
+    """Rows of 2.5e9 elements through the product and its gradient, a weight of 2.2e9 both ways: some
+    of the last rows and columns against the oracle. More rows and blocks than the quantization's
+    and the dequantization's grids take in one go."""
+    from gsq_rco_mlx_b200.common.fp8 import Fp8Linear
+    g = torch.Generator(device="cuda").manual_seed(3)
+    M, K, N, n = 300001, 8192, 130, 3
+    x = torch.empty(M, K, device="cuda", dtype=torch.bfloat16).normal_(generator=g)
+    lin = Fp8Linear.from_weight(rnd((N, K), 4, scale=0.05), transposed=True)
+    y = lin(x)
+    ref, mag = of.linear(f32(x[-n:]), f32(lin.codes), f32(lin.scales))
+    near(f64(y[-n:]), ref, _tol_gemm(mag, K, torch.bfloat16, ref), "y")
+    dy = torch.empty(M, N, device="cuda", dtype=torch.bfloat16).normal_(generator=g)
+    dx, dw = lin.vjp(x, dy)
+    _err_ok()
+    wv = of.blocks_value(f32(lin.codes), f32(lin.scales))
+    dv = of.rows_value(*of.quantize_rows(f32(dy[-n:])))
+    near(f64(dx[-n:]), dv @ wv, _tol_gemm(np.abs(dv) @ np.abs(wv), N, torch.bfloat16, dv @ wv), "dx")
+    a = of.rows_value(*of.quantize_rows(np.ascontiguousarray(f32(dy[:, -n:]).T)))
+    b = of.rows_value(*of.quantize_rows(np.ascontiguousarray(f32(x[:, -n:]).T)))
+    rw = a @ b.T
+    near(f64(dw[-n:, -n:]), rw, _tol_gemm(np.abs(a) @ np.abs(b).T, M, torch.float32, rw), "dw")
+    del x, y, dx
+    N = 270001
+    W = torch.empty(N, K, device="cuda", dtype=torch.bfloat16).normal_(generator=g)
+    lin = Fp8Linear.from_weight(W)
+    q, s = of.quantize_blocks(f32(W[N // 128 * 128:]))   # the last block of rows
+    m = N - N // 128 * 128
+    assert np.array_equal(f32(lin.codes[-m:]), q) and np.array_equal(f32(lin.scales[-1:]), s)
+    out = torch.empty_like(W)
+    lin.dequant(out)
+    v = of.blocks_value(q, s)
+    near(f64(out[-m:]), v, (half(torch.bfloat16) + U) * np.abs(v) + tiny(torch.bfloat16))
+    near(f64(out[:2]), of.blocks_value(*of.quantize_blocks(f32(W[:128])))[:2],
+         (half(torch.bfloat16) + U) * np.abs(f64(out[:2])) * (1 + 2.0 ** -7) + tiny(torch.bfloat16))
+    for rows in (1, 100):   # 2110 tiles of columns, the last one ragged
+        z = rnd((rows, K), 6, torch.bfloat16)
+        o = lin(z)
+        ref, mag = of.linear(f32(z[-n:]), q, s)
+        near(f64(o[-n:, -m:]), ref, _tol_gemm(mag, K, torch.bfloat16, ref), "wide")
+    _err_ok()
 
 
 # ------------------------------------------------------------------------------------ together ---
