@@ -10,7 +10,7 @@
 // Bound by the bytes of q and k, read once and written once. A thread owns one vector of pairs
 // of one token in up to four heads, so the 64-bit angles and the sines are computed once for
 // several heads, while their loads are in flight: no table of positions is read. 16384 x 16 heads
-// of 64 in bf16: 16.5 us, 4.1 TB/s; 8191 x 40 heads of 128 in float16: 32 us, 5.2 TB/s.
+// of 64 in bf16: 17 us, 3.9 TB/s; 8191 x 40 heads of 128 in float16: 33 us, 5.1 TB/s.
 #include "dtypes.cuh"
 
 namespace gsq {
@@ -176,11 +176,14 @@ static int launch(Args& p, cudaStream_t st) {
   const bool same = p.q.in == p.q.out && (p.k.heads == 0 || p.k.in == p.k.out);
   p.lanes = rot_lanes + (same ? 0 : (p.hd - p.rot) / V);
   const int heads = p.q.heads + p.k.heads;
-  // Heads a thread turns by its angles: four (16384 x 16 heads of 64: 16.5 us, with two 21.6;
-  // 8191 x 40 of 128: 32.0, with two 48.3, with eight in two batches 35.2), fewer for few tokens,
-  // down to one (a decoded token's heads all at once).
+  // Heads a thread turns by its angles: four where that leaves 192 threads an SM (16384 x 16 heads
+  // of 64 in bf16: 18.0 us, with two 23.1, with one 36.4; 2048: 4.8, 5.0, 6.8), fewer for fewer
+  // tokens (1024: 3.7, 3.3, 3.7; 512: 3.6, 3.1, 2.9; 1: 2.9, 2.5, 2.3), unless a token's threads
+  // would no longer be one turn of a block (1 x 40 heads of 128: with two 2.9, with one 3.8). Eight
+  // in two batches: 19.8 at 16384 x 16, 35.9 for 32.8 at 8191 x 40.
   int walk = kBatch;
-  while (walk > 1 && p.T * p.lanes * ((heads + walk - 1) / walk) < (int64_t)num_sms() * 1024)
+  while (walk > 1 && p.T * p.lanes * ((heads + walk - 1) / walk) < (int64_t)num_sms() * 192 &&
+         p.lanes * ((heads + walk / 2 - 1) / (walk / 2)) <= 256)
     walk /= 2;
   p.chunks = (heads + walk - 1) / walk;
   const int per = p.lanes * p.chunks;

@@ -404,6 +404,24 @@ def test_rotary(T, nq, nk, hd, rot, layout, dtype):
     assert torch.equal(packed[:, (nq + nk) * hd:], keep[:, (nq + nk) * hd:])
 
 
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("T,nq,nk,hd,rot", [(1024, 14, 2, 64, 64), (4096, 14, 2, 64, 64),
+                                            (300, 32, 8, 128, 64), (2500, 7, 1, 80, 20)])
+def test_rotary_gives_a_token_the_same_bits_in_any_batch(T, nq, nk, hd, rot, layout):
+    """However many heads a thread turns, which goes by the number of tokens and heads."""
+    from gsq_rco_mlx_b200.common.rotary import Rotary
+    r = Rotary(hd, 1e6, rot, layout, SCALINGS[4])
+    q, k = rnd((T, nq, hd), 1, torch.bfloat16), rnd((T, nk, hd), 2, torch.bfloat16)
+    p = torch.arange(T, device="cuda") * 37
+    qo, ko = r(q, k, p)
+    for t in (0, T // 2, T - 1):
+        for n in (1, 64):
+            a, b = r(q[t:t + n], k[t:t + n], p[t:t + n])
+            assert torch.equal(a, qo[t:t + n]) and torch.equal(b, ko[t:t + n])
+    for h in (0, nq - 1):
+        assert torch.equal(r(q[:, h:h + 1], None, p)[0], qo[:, h:h + 1])
+
+
 def test_rotary_far_positions_and_layouts():
     """int64 positions beyond 2^31, head-major buffers, unaligned rows, a broadcast key input."""
     from gsq_rco_mlx_b200.common.rotary import Rotary
