@@ -182,7 +182,8 @@ class PackedModel:
     @classmethod
     def from_fp8(cls, model, names=LIN_ORDER):
         """A QwenModel (bf16 on the GPU) with the linears `names` of every layer in e4m3 with a
-        scale per 128 x 128 (Fp8Linear); the others stay dense."""
+        scale per 128 x 128 (Fp8Linear); the others stay dense. The eval dequantizes them (block),
+        so its perplexity is that of 8-bit weights with bf16 activations."""
         layers = [{k: Fp8Linear.from_weight(v) if k in names else v for k, v in W.items()}
                   for W in model.layers]
         return cls(model.cfg, model.embed, model.norm, layers)

@@ -1,8 +1,9 @@
 """Linears in 8-bit floating point: e4m3 values with a float32 scale per block of 128.
 
-The packed eval's other weight format beside PackedLinear (common/evaluate.py): half the bytes
-of bf16, both operands of the product in 8 bits on the tensor cores, no calibration. With a the
-largest magnitude of a block and a' = max(a, 2^-100),
+Half the bytes of bf16, both operands of the product in 8 bits on the tensor cores, no
+calibration. The packed eval takes the weight format beside PackedLinear (common/evaluate.py): it
+dequantizes the weights, and its products run on bf16 activations. With a the largest magnitude of
+a block and a' = max(a, 2^-100),
 
   scale = a' / 448,  code = e4m3(x * (448 / a'))        (448: the largest e4m3 value)
 
@@ -10,6 +11,9 @@ largest magnitude of a block and a' = max(a, 2^-100),
   quantize_rows  x -> Fp8Tensor
   Fp8Linear      a weight [N, K] with a scale per 128 x 128: y = x W^T with x quantized in rows,
                  and its vector-Jacobian product
+
+Rows up to 2^30; 65535 blocks of 128 (8.4e6) where they are a weight's, or are quantized by columns
+(vjp).
 
 Reference: none (src/gsq_rco/gsq/export.py:52-91 exports integer codes only).
 """

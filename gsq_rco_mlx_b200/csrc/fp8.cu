@@ -14,14 +14,15 @@
 // accumulator cannot run on over k: the epilogue warps read it back, and fold it into float32
 // registers with one multiply-add per value, two values an instruction.
 //
-// What bounds it (8191 x 8192 x 4096 on B200: 260 us, 2.1 PFLOP/s, at the 1.35 GHz or so that the
-// power cap leaves): at the e4m3 rate a 128 x 256 tile takes 512 cycles per k-block, and these
-// 260 us are about 790 each. The fold of one takes 128 packed multiply-adds on each of the four
-// schedulers, measured alone at 2.2 cycles each with two warps and 5.4 with one, and the reads of
-// TMEM and the waits between leave a warp alone for part of the time. Tried and dropped: 16
-// epilogue warps (327 against 296 us), the next columns read while these are folded (321 against
-// 285). The loops of the other warps have to stay shorter than the fold: run by one lane, the MMA
-// warp's took 840 cycles a k-block, so its control is uniform over the warp.
+// What bounds it: at the e4m3 rate a 128 x 256 tile takes 512 cycles per k-block. 8191 x 8192 x 4096
+// on B200 takes 253 us in bursts at 1965 MHz (2.2 PFLOP/s, the tensor pipe active on 55 % of the
+// cycles in a profile), about 1100 cycles each; run for a second, at the 1550 MHz that the power cap
+// leaves, 295 us. The fold of a k-block takes 128 packed multiply-adds on each of the four
+// schedulers, measured alone at 2.2 cycles each with two warps and 5.4 with one, and the polls of
+// barriers, the reads of TMEM and the waits between leave a warp alone for part of the time. Tried
+// and dropped: 16 epilogue warps (327 against 296 us), the next columns read while these are folded
+// (321 against 285). The loops of the other warps have to stay shorter than the fold: run by one
+// lane, the MMA warp's took 840 cycles a k-block, so its control is uniform over the warp.
 #include <cuda_fp8.h>
 
 #include <type_traits>
@@ -501,7 +502,8 @@ __device__ __forceinline__ void tile_at(const GemmArgs& p, int t, int& m, int& n
 }
 
 // An output row's values of one warp column range, element by element (rows that TMA cannot
-// write, and sums into what is there).
+// write, and sums into what is there): 32 rows an instruction, so an output off 16 bytes costs a
+// large product several times its time (16384 x 896 -> 4863: 822 us, -> 4864: 92).
 template <typename T, int CW>
 __device__ __forceinline__ void store_row(const GemmArgs& p, int m, int n0,
                                           const uint64_t* acc) {

@@ -17,10 +17,13 @@
 // column by column with the columns dealt round the team, which keeps every access of a warp one
 // segment (neighbouring columns a thread would touch each sector several times).
 // Measured: 16384 x 896 bf16 into e4m3 rows 31 us (3.3 TB/s, an instruction issued on 70 % of the
-// schedulers' cycles), its gradient with a gate 50 us (3.5 TB/s, 56 %), the gradient of 6141 x 5121
-// float16, column by column, 157 us. At the same bytes' time the gradient of 16384 x 896 reaches
-// 71 % of the copy rate in float32 and 54 % in bf16: what bounds the 16-bit forms is the
-// instructions of a column and the barriers of a row's sums, not the bytes.
+// schedulers' cycles), its gradient with a gate 50 us (3.5 TB/s, 55 %), the gradient of 6141 x 5121
+// float16, column by column, 157 us. The gradient of 16384 x 896 reaches 73 % of the copy rate in
+// float32 (73 us) and 54 % in bf16: what bounds the 16-bit forms is the instructions of a column and
+// the barriers of a row's sums, not the bytes.
+// Above 8192 columns the rows do not fit shared memory and a thread's 16 or 32 columns do not fit 64
+// registers: the gradient spills 290 to 1700 bytes a thread (2048 x 32768 bf16: 711 us, 1.1 TB/s),
+// the forward pass up to 600 (156 us, 3.5 TB/s).
 // The column sums of the backward pass: each team adds its rows in registers and writes one
 // partial row; a second kernel adds the partials in a fixed order (no atomics: the same inputs
 // give the same bits).

@@ -4,8 +4,9 @@
 // vector-Jacobian product is the same with -t. The rest of the head passes through.
 //
 // Far positions: t is held as turns, p (w_j / 2 pi), in 64 bits; the whole turns are taken off
-// there, and sincospif sees the remainder in [-1/2, 1/2] turns, so the angle's error is a
-// float32 rounding of at most half a turn (2e-7 radians) at any position up to 2^31.
+// there, and sincospif sees the remainder in [-1/2, 1/2] turns. So the angle is off by the float32
+// rounding of that remainder (2^-25 pi, 1e-7 radians) and by 2^-52 of the whole angle (the rounding
+// of the stored frequency and of the product): 1e-8 radians at p w_j = 5e7, 5e-7 at 2^31.
 //
 // Bound by the bytes of q and k, read once and written once. A thread owns one vector of pairs
 // of one token in up to four heads, so the 64-bit angles and the sines are computed once for

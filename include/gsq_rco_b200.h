@@ -570,9 +570,11 @@ int gsq_fp8_linear_vjp(const void *x, int dtype, int M, int K, int64_t ld_x, con
  * themselves for a rotation in place). The first rotary_dim elements of a head turn in pairs
  * (j, j + rotary_dim / 2), or (2 j, 2 j + 1) if interleaved, by positions[t] turns[j] turns:
  * (a, b) -> factor (a cos - b sin, a sin + b cos); inverse: by the opposite angle (the
- * vector-Jacobian product). The rest of the head is copied. dtype 0 / 1 / 2 = bf16 / f16 / f32;
+ * vector-Jacobian product). The rest of the head is copied. Outputs that overlap an input otherwise,
+ * or one another, give wrong rows (the Python call refuses them). dtype 0 / 1 / 2 = bf16 / f16 / f32;
  * positions int32 or int64 [T] of any sign; turns float64 [rotary_dim / 2], the pairs'
- * frequencies over 2 pi. float32 arithmetic, the angle reduced in 64 bits.
+ * frequencies over 2 pi. float32 arithmetic, the angle reduced in 64 bits (off by 1e-7 radians and
+ * 2^-52 of itself).
  * The general form of gsq_rope_split's rotation (src/gsq_rco/gsq/e2e.py:96-108). */
 int gsq_rope(const void *q, int64_t q_t, int64_t q_h, int nq, const void *k, int64_t k_t,
              int64_t k_h, int nk, int64_t T, int head_dim, int rotary_dim, int interleaved,
