@@ -128,8 +128,8 @@ def err_flag(dev):
         word = _ERR.get(dev)
         if torch.cuda.is_current_stream_capturing():
             if word is None:
+                _UNFILLED.add(dev)   # (first: other threads look without the lock)
                 word = _ERR[dev] = torch.zeros(1, device=dev, dtype=torch.int32)
-                _UNFILLED.add(dev)
         elif word is None or dev in _UNFILLED:
             word = torch.zeros(1, device=dev, dtype=torch.int32) if word is None else word.zero_()
             torch.cuda.current_stream(dev).synchronize()

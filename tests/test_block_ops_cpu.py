@@ -242,6 +242,23 @@ def test_an_error_word_made_in_a_capture_is_filled_by_the_next_eager_call(monkey
     assert gemm.err_flag(dev) is word and int(word) == 3 and len(seen) == 1
 
 
+def test_an_error_word_made_in_a_capture_is_known_as_that_from_the_first(monkeypatch):
+    """Another host thread looks it up without the lock: it must not take it for a filled one."""
+    from gsq_rco_mlx_b200 import gemm
+    dev, unfilled, order = torch.device("cpu"), set(), []
+
+    class Words(dict):
+        def __setitem__(self, key, word):
+            order.append(key in unfilled)
+            super().__setitem__(key, word)
+
+    monkeypatch.setattr(gemm, "_ERR", Words())
+    monkeypatch.setattr(gemm, "_UNFILLED", unfilled)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    gemm.err_flag(dev)
+    assert order == [True]
+
+
 def test_outputs_over_inputs():
     """row_by_row against the elements themselves: it takes the same rows and every pair without a
     common element of one pitch or apart as a whole, and no pair with one."""
